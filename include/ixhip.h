@@ -273,6 +273,71 @@ int ixh_lanes_gemm(const IxhLanes *lanes, const uint16_t *x, int64_t ldx, const 
 size_t ixh_lanes_gemm_workspace_bytes(const IxhLanes *lanes, int32_t m);
 
 /*
+ * Routing of tokens to experts.  Per row of `experts` logits (dtype IXH_F32, IXH_F16 or IXH_BF16, a row every `ld` elements) the top_k chosen
+ * experts, best first, to ids [tokens, top_k] and their weights to weights [tokens, top_k].
+ *   scores   p = softmax or sigmoid (IXH_SCORE_*) of the open experts' logits; an expert whose logit is -infinity is closed
+ *   choice   the logits themselves with bias NULL, p + bias[expert] (fp32 [experts], formed in 64 bits) otherwise; equal ones go to the
+ *            lowest index, NaN counts as the largest, -infinity as closed
+ *   groups   experts in n_groups runs of equal length; only those of the top_groups best take part: best by their best choice, with a
+ *            bias by the sum of their two best
+ *   weights  the chosen experts' p, divided by their sum where `renormalize` is set (0 where that is 0), times scale
+ * Places that find no open expert get id -1 and weight 0.  Up to 1024 experts, 64 groups and 64 chosen.  The reference has no counterpart.
+ */
+#define IXH_F32 0
+#define IXH_F16 1
+#define IXH_BF16 2
+#define IXH_SCORE_SOFTMAX 0
+#define IXH_SCORE_SIGMOID 1
+typedef struct IxhRouting {
+    int32_t experts, top_k, n_groups, top_groups, scoring, renormalize;
+    float scale;
+} IxhRouting;
+int ixh_route(const IxhRouting *routing, const void *logits, int32_t dtype, int64_t ld, int64_t tokens, const float *bias, int32_t *ids,
+              float *weights, ixh_stream_t stream);
+
+/*
+ * The experts' products over packed weights, in the lane layout:
+ *   y[t] = bf16( residual[t] + sum_j weights[t, j] * second_e( h ) ),  e = ids[t, j], in the order of j,
+ *   h = bf16( act(gate_e x[t] + b) * (up_e x[t] + b) ),  or bf16( act(first_e x[t] + b) ) if not `gated`.
+ * x bf16 [tokens, ldx], y and residual (may be NULL) bf16 [tokens, ld]; ids and weights (fp32) [tokens, top_k].  A place whose id is none of
+ * 0 .. n_experts - 1 adds nothing, and its weight is not read.  tokens * top_k up to 2^20.  Sums, biases and the sum over the experts are fp32.
+ *
+ * IxhExpertMatrix: one matrix of all experts, out_f x in_f each: planes one after another (ixh_lanes_plane_words each), exc_off of
+ * ixh_lanes_cells + 1 entries for each expert, all of them places in one list, and a scale for each expert.  `first` is inner x hidden, or,
+ * gated, 2 * inner16 x hidden with inner16 = inner rounded up to 16: blocks of 16 rows, of the gate and of the other half in turn, rows past
+ * the last zero.  Its bias (bf16, may be NULL) is [n_experts, 2 * inner], the gate's first ([n_experts, inner] if not gated).  `second` is
+ * hidden x inner, its bias [n_experts, hidden].
+ */
+#define IXH_ACT_NONE 0
+#define IXH_ACT_SILU 1
+#define IXH_ACT_GELU 2      /* 0.5 v (1 + erf(v / sqrt 2)) */
+#define IXH_ACT_GELU_TANH 3 /* 0.5 v (1 + tanh(sqrt(2 / pi) (v + 0.044715 v^3))) */
+#define IXH_ACT_RELU 4
+#define IXH_ACT_RELU2 5     /* max(v, 0)^2 */
+typedef struct IxhExpertMatrix {
+    int32_t bits;
+    int64_t out_f;
+    int64_t in_f;
+    const uint32_t *plane;
+    uint64_t plane_words;
+    const uint32_t *exc_off;
+    const uint16_t *exc_pos;
+    const int8_t *exc_val;
+    uint64_t n_quads;
+    const uint16_t *scale;
+    const uint16_t *bias;
+} IxhExpertMatrix;
+typedef struct IxhExperts {
+    int32_t n_experts, gated, activation;
+    int64_t hidden, inner;
+    IxhExpertMatrix first, second;
+} IxhExperts;
+size_t ixh_experts_workspace_bytes(const IxhExperts *experts, int64_t tokens, int32_t top_k);
+int ixh_experts(const IxhExperts *experts, const uint16_t *x, int64_t ldx, int64_t tokens, const int32_t *ids, const float *weights,
+                int32_t top_k, const uint16_t *residual, int64_t ld_residual, uint16_t *y, int64_t ldy, void *workspace,
+                size_t workspace_bytes, ixh_stream_t stream);
+
+/*
  * The encoder on the device, in two steps because the stream lengths depend on the data.
  * Together they replace int8x_quantize (ixrun/quantize.py:41-122, with pack_bits_stream
  * and pack_bitmap of ixrun/bitpack.py:13-61, :87-89) for a bf16 weight that is already in

@@ -11,6 +11,7 @@ Hand-written gfx950 HIP kernels behind a C ABI (``include/ixhip.h``,
 ``ixrun_amd.fused``    ``fused_gemv``, ``compute_row_prefixes``
 ``ixrun_amd.linear``   ``Int8XLinear``, ``deploy_model``
 ``ixrun_amd.engine``   ``StreamingLinear``, ``GraphLinear``, ``Int8XEngine``
+``ixrun_amd.experts``  ``route_experts``, ``StreamingExperts``
 =====================  =====================================================
 """
 from .config import BIT_TO_THRESHOLD, DEFAULT_LEVELS
@@ -20,5 +21,6 @@ from .fused import fused_gemv, compute_row_prefixes, FUSED_TILE
 from .triton_kernels import decode_weight_triton, decode_weight_scatter, precompute_block_offsets
 from .linear import Int8XLinear, deploy_model, iter_quantizable_linears
 from .engine import Int8XEngine, StreamingLinear, GraphLinear, ResourceScheduler
+from .experts import StreamingExperts, route_experts
 
 __version__ = "0.1.0"

@@ -9,6 +9,8 @@
 
 #include "../../include/ixhip_test.h"
 #include "ixh_dev.h"
+#include "ixh_epilogue.h"
+#include "ixh_experts.h"
 #include "ixh_fast358.h"
 #include "ixh_lanes.h"
 #include "ixh_prefill358.h"
@@ -681,6 +683,104 @@ int ixh_lanes_gemm(const IxhLanes *lanes, const uint16_t *x, int64_t ldx, const 
     }
     LnScratch ws{(float *)workspace, workspace_bytes, 0};
     return lanes_status(launch_lanes_gemm(d, x, m, ldx, bias, true, y, ldy, ws, (hipStream_t)stream), ws, "lanes_gemm");
+}
+
+// ---- experts ----
+int ixh_route(const IxhRouting *r, const void *logits, int32_t dtype, int64_t ld, int64_t tokens, const float *bias, int32_t *ids,
+              float *weights, ixh_stream_t stream) {
+    if (!r) { set_error("route: routing is NULL"); return IXH_EINVAL; }
+    if (r->experts < 1 || r->experts > (int32_t)kRtMostExperts) { set_error("route: %d experts not in 1..%u", r->experts, kRtMostExperts); return IXH_EINVAL; }
+    if (r->top_k < 1 || r->top_k > r->experts || r->top_k > (int32_t)kRtMostChosen) {
+        set_error("route: top_k %d not in 1..%u and at most the %d experts", r->top_k, kRtMostChosen, r->experts);
+        return IXH_EINVAL;
+    }
+    if (r->n_groups < 1 || r->n_groups > (int32_t)kRtMostGroups || r->experts % r->n_groups) {
+        set_error("route: %d groups of %d experts: at most %u, of equal length", r->n_groups, r->experts, kRtMostGroups);
+        return IXH_EINVAL;
+    }
+    if (r->top_groups < 1 || r->top_groups > r->n_groups) { set_error("route: top_groups %d not in 1..%d", r->top_groups, r->n_groups); return IXH_EINVAL; }
+    if (r->top_k > r->top_groups * (r->experts / r->n_groups)) {
+        set_error("route: top_k %d of the %d experts that the best groups have", r->top_k, r->top_groups * (r->experts / r->n_groups));
+        return IXH_EINVAL;
+    }
+    if (r->scoring != IXH_SCORE_SOFTMAX && r->scoring != IXH_SCORE_SIGMOID) { set_error("route: scoring %d", r->scoring); return IXH_EINVAL; }
+    if (dtype != IXH_F32 && dtype != IXH_F16 && dtype != IXH_BF16) { set_error("route: dtype %d", dtype); return IXH_EINVAL; }
+    if (tokens < 0 || tokens >= (1ll << 31) / r->top_k) { set_error("route: %lld tokens", (long long)tokens); return IXH_EINVAL; }
+    if (tokens == 0) return IXH_OK;
+    if (!logits || !ids || !weights) { set_error("route: logits, ids or weights is NULL"); return IXH_EINVAL; }
+    if (tokens > 1 && ld < r->experts) { set_error("route: ld shorter than a row"); return IXH_EINVAL; }
+    const RouteDev d{(uint32_t)r->experts, (uint32_t)r->top_k, (uint32_t)r->n_groups, (uint32_t)(r->experts / r->n_groups), (uint32_t)r->top_groups,
+                     r->scoring == IXH_SCORE_SIGMOID, r->renormalize != 0, (double)r->scale};
+    const int rc = launch_route(logits, dtype, ld, (uint32_t)tokens, d, bias, ids, weights, (hipStream_t)stream);
+    if (rc == IXH_ELAUNCH) set_error("route: launch failed");
+    return rc;
+}
+
+static int to_matrix(const IxhExpertMatrix &p, int64_t experts, int64_t out_f, int64_t in_f, int64_t outputs, const char *name, ExMatrix *out) {
+    if (p.out_f != out_f || p.in_f != in_f) {
+        set_error("experts: %s is %lld x %lld, expected %lld x %lld", name, (long long)p.out_f, (long long)p.in_f, (long long)out_f, (long long)in_f);
+        return IXH_EINVAL;
+    }
+    const int64_t words = ixh_lanes_plane_words(out_f, in_f, p.bits);
+    if (words < 0) { set_error("experts: %s, %lld x %lld at %d bits, is no lane layout", name, (long long)out_f, (long long)in_f, p.bits); return IXH_EINVAL; }
+    if (!p.plane || ((uintptr_t)p.plane & 15u) || p.plane_words < (uint64_t)words * (uint64_t)experts) {
+        set_error("experts: %s needs planes of %lld words for each expert, 16-byte aligned", name, (long long)words);
+        return IXH_EINVAL;
+    }
+    if (!p.scale || !p.exc_off || !p.exc_pos || !p.exc_val || p.n_quads < 64 || p.n_quads % 64 || p.n_quads >= (1ull << 30)) {
+        set_error("experts: %s: scale, exc_off or the list is NULL, or the list holds no whole groups of 64 quads, or 2^30 quads", name);
+        return IXH_EINVAL;
+    }
+    *out = ExMatrix{p.plane, p.exc_off, p.exc_pos, p.exc_val, p.scale, p.bias, (uint64_t)words, (uint32_t)((out_f + 3) / 4),
+                    (uint32_t)((in_f + kLnCols - 1) / kLnCols), (uint32_t)in_f, (uint32_t)outputs, p.bits};
+    return IXH_OK;
+}
+
+static int to_experts(const IxhExperts *p, int64_t tokens, int32_t top_k, ExDev *out) {
+    if (!p) { set_error("experts is NULL"); return IXH_EINVAL; }
+    if (p->n_experts < 1 || p->n_experts > (int32_t)kExMostExperts) { set_error("experts: %d experts not in 1..%u", p->n_experts, kExMostExperts); return IXH_EINVAL; }
+    if (p->hidden < 1 || p->inner < 1 || p->hidden >= (1ll << 31) || p->inner >= (1ll << 29)) { set_error("experts: %lld x %lld", (long long)p->inner, (long long)p->hidden); return IXH_EINVAL; }
+    if (!ep_known(p->activation)) { set_error("experts: activation %d", p->activation); return IXH_EINVAL; }
+    if (top_k < 1 || tokens < 0 || tokens > (int64_t)kExMostSlots / top_k) {
+        set_error("experts: %lld tokens of %d experts each, not 2^20 places at most", (long long)tokens, top_k);
+        return IXH_EINVAL;
+    }
+    *out = ExDev{};
+    out->experts = (uint32_t)p->n_experts, out->hidden = (uint32_t)p->hidden, out->inner = (uint32_t)p->inner;
+    out->activation = p->activation, out->gated = p->gated != 0;
+    int rc = to_matrix(p->first, p->n_experts, out->gated ? (p->inner + 15) / 16 * 32 : p->inner, p->hidden, p->inner, "the first matrix", &out->first);
+    if (!rc) rc = to_matrix(p->second, p->n_experts, p->hidden, p->inner, p->hidden, "the second matrix", &out->second);
+    return rc;
+}
+
+size_t ixh_experts_workspace_bytes(const IxhExperts *experts, int64_t tokens, int32_t top_k) {
+    ExDev d;
+    if (to_experts(experts, tokens, top_k, &d)) return 0;
+    return experts_workspace_bytes(d, (uint32_t)tokens, (uint32_t)top_k);
+}
+
+int ixh_experts(const IxhExperts *experts, const uint16_t *x, int64_t ldx, int64_t tokens, const int32_t *ids, const float *weights,
+                int32_t top_k, const uint16_t *residual, int64_t ld_residual, uint16_t *y, int64_t ldy, void *workspace,
+                size_t workspace_bytes, ixh_stream_t stream) {
+    ExDev d;
+    int rc = to_experts(experts, tokens, top_k, &d);
+    if (rc) return rc;
+    if (tokens == 0) return IXH_OK;
+    if (!x || !ids || !weights || !y) { set_error("experts: x, ids, weights or y is NULL"); return IXH_EINVAL; }
+    if (tokens > 1 && (ldx < (int64_t)d.hidden || ldy < (int64_t)d.hidden || (residual && ld_residual < (int64_t)d.hidden))) {
+        set_error("experts: ldx, ldy or ld_residual shorter than a row");
+        return IXH_EINVAL;
+    }
+    const size_t need = experts_workspace_bytes(d, (uint32_t)tokens, (uint32_t)top_k);
+    if (!workspace || workspace_bytes < need) {
+        set_error("workspace of %zu bytes needed, %zu given", need, workspace ? workspace_bytes : (size_t)0);
+        return IXH_EWORKSPACE;
+    }
+    const ExCall call{x, ldx, (uint32_t)tokens, (uint32_t)top_k, ids, weights, residual, ld_residual, y, ldy};
+    rc = launch_experts(d, call, workspace, (hipStream_t)stream);
+    if (rc == IXH_ELAUNCH) set_error("experts: launch failed");
+    if (rc == IXH_EUNSUPPORTED) set_error("experts: rows of this length do not fit");
+    return rc;
 }
 
 static int encode_levels_ok(int32_t n_levels, const int32_t *level_bits) {

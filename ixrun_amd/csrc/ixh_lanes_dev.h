@@ -165,6 +165,22 @@ __device__ __forceinline__ void ln_wave_order() {  // LDS accesses of the wave's
     __builtin_amdgcn_wave_barrier();
 }
 
+typedef __bf16 lr_bf16x4 __attribute__((ext_vector_type(4)));
+
+// Where a column's activations are in LDS: rows of MT bf16, the columns of a cell in the order of the list's positions
+// (lane_offset), so that a position times MT is a byte offset. At 16 rows the halves of a row of 32 bytes and of a run of eight
+// rows change places with the column, so that both a random column's half and the sixteen pieces that a transposing read
+// takes from four groups of eight columns lie on all banks.
+template <int MT> __device__ __forceinline__ uint32_t lr_place(uint32_t bytes) {
+    return MT == 16 ? bytes ^ ((bytes >> 1) & 0x90u) : bytes;
+}
+
+// A transposing read: sixteen lanes name sixteen pieces of 8 bytes, four columns of a place each, and lane n of them gets
+// activation row n of the four columns.
+__device__ __forceinline__ lr_bf16x4 lr_turned(uint32_t at) {
+    return __builtin_bit_cast(lr_bf16x4, __builtin_amdgcn_ds_read_tr16_b64_v4i16((LN_LDS(ln_s16x4) *)(uintptr_t)at));
+}
+
 inline uint32_t ln_cus() {
     static const uint32_t n = [] {
         int dev = 0, v = 256;

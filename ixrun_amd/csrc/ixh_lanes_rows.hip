@@ -30,22 +30,6 @@ namespace ixh {
 // rows' pairs of columns a lane has in registers on the way to LDS: as many as 512 columns x 16 or 768 x 8 take of 16 waves
 template <int MT> constexpr uint32_t kLrXAhead = MT == 8 ? 3 : 2;
 
-typedef __bf16 lr_bf16x4 __attribute__((ext_vector_type(4)));
-
-// Where a column's activations are in LDS: rows of MT bf16, the columns of a cell in the order of the list's positions
-// (lane_offset), so that a position times MT is a byte offset. At 16 rows the halves of a row of 32 bytes and of a run of eight
-// rows change places with the column, so that both a random column's half and the sixteen pieces that a transposing read
-// takes from four groups of eight columns lie on all banks.
-template <int MT> __device__ __forceinline__ uint32_t lr_place(uint32_t bytes) {
-    return MT == 16 ? bytes ^ ((bytes >> 1) & 0x90u) : bytes;
-}
-
-// A transposing read: sixteen lanes name sixteen pieces of 8 bytes, four columns of a place each, and lane n of them gets
-// activation row n of the four columns.
-__device__ __forceinline__ lr_bf16x4 lr_turned(uint32_t at) {
-    return __builtin_bit_cast(lr_bf16x4, __builtin_amdgcn_ds_read_tr16_b64_v4i16((LN_LDS(ln_s16x4) *)(uintptr_t)at));
-}
-
 // (the order of a cell's columns is worked out on the address bits of 128 rows)
 template <int BITS, bool WIDE> constexpr uint32_t kLrXAt = (LnPairs<BITS, WIDE>::kLutBytes + 4095u) & ~4095u;
 

@@ -1,0 +1,286 @@
+"""Routing and the experts' products against their formulas in 64 bits (operator_reference.py has the bounds)."""
+import math
+
+import pytest
+import torch
+
+import operator_reference as ref
+from helpers import calibrated_weight, outlier_weight, student_t_weight
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module")
+def dev():
+    assert torch.cuda.is_available(), "these tests need the MI355X"
+    return torch.device("cuda:0")
+
+
+# ---- routing ----
+def _check_route(logits, top_k, dev, **options):
+    from ixrun_amd import route_experts
+
+    bias = options.get("bias")
+    on = dict(options, bias=bias.to(dev) if bias is not None else None)
+    ids, weights = route_experts(logits.to(dev), top_k, **on)
+    want_ids, want = ref.route(logits, top_k, **options)
+    assert ids.dtype == torch.int32 and weights.dtype == torch.float32 and ids.shape == want_ids.shape
+    assert torch.equal(ids.cpu(), want_ids)
+    got = weights.cpu().double()
+    assert torch.equal(got.isnan(), want.isnan())
+    # worked out in 64 bits and rounded once to fp32
+    assert bool(((got - want).abs() <= 1.001 * ref.U32 * want.abs() + 2.0 ** -149)[~want.isnan()].all())
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("tokens,experts,top_k", [(1, 1, 1), (1, 64, 6), (5, 7, 7), (3, 65, 1), (130, 128, 8), (33, 200, 16), (2, 1024, 64), (9, 500, 3)])
+def test_softmax_routing(dev, dtype, tokens, experts, top_k):
+    g = torch.Generator().manual_seed(tokens + experts)
+    _check_route((torch.randn(tokens, experts, generator=g) * 2).to(dtype), top_k, dev)
+
+
+@pytest.mark.parametrize("scoring", ["softmax", "sigmoid"])
+@pytest.mark.parametrize("renormalize,scale", [(True, 1.0), (False, 2.5)])
+@pytest.mark.parametrize("with_bias", [False, True])
+@pytest.mark.parametrize("experts,n_groups,top_groups,top_k", [(32, 1, 1, 5), (160, 8, 3, 6), (96, 4, 4, 8), (64, 64, 9, 9), (12, 6, 1, 2)])
+def test_routing_options(dev, scoring, renormalize, scale, with_bias, experts, n_groups, top_groups, top_k):
+    g = torch.Generator().manual_seed(experts)
+    logits = torch.randn(21, experts, generator=g)
+    bias = torch.randn(experts, generator=g) * 0.3 if with_bias else None
+    _check_route(logits, top_k, dev, scoring=scoring, bias=bias, n_groups=n_groups, top_groups=top_groups, renormalize=renormalize, scale=scale)
+
+
+@pytest.mark.parametrize("scoring", ["softmax", "sigmoid"])
+@pytest.mark.parametrize("with_bias", [False, True])
+@pytest.mark.parametrize("n_groups,top_groups", [(1, 1), (4, 2)])
+def test_routing_of_closed_equal_and_odd_logits(dev, scoring, with_bias, n_groups, top_groups):
+    """Rows with no open expert, with fewer than are chosen, with equal logits, the largest and smallest values, NaN and infinity."""
+    inf, nan, top = math.inf, math.nan, torch.finfo(torch.float32).max
+    logits = torch.zeros(12, 16)
+    logits[0] = -inf
+    logits[1] = -inf
+    logits[1, 9] = 0.5
+    logits[2, ::2] = 1.0
+    logits[3] = -top
+    logits[4] = torch.arange(16) % 3 - 1.0
+    logits[5, 4] = nan
+    logits[6, 3] = inf
+    logits[7] = torch.tensor([top, -top] * 8)
+    logits[8, 1:] = -0.0
+    logits[9, 5:] = -inf
+    logits[10] = 300.0 + torch.arange(16)
+    logits[11] = -200.0 - torch.arange(16)
+    bias = (torch.arange(16) % 5).float() / 8 if with_bias else None
+    if with_bias:
+        bias[11] = -inf
+    _check_route(logits, 4, dev, scoring=scoring, bias=bias, n_groups=n_groups, top_groups=top_groups)
+
+
+def test_routing_of_views(dev):
+    """Leading dimensions, rows at a stride, a transposed view, no tokens at all."""
+    from ixrun_amd import route_experts
+
+    g = torch.Generator().manual_seed(3)
+    wide = torch.randn(6, 5, 40, generator=g)
+    for view in (wide[..., :24], wide[:, 1, 8:30], wide.transpose(0, 1)[..., 1:], wide[2, 2], wide[:, :, :24].transpose(1, 2)):
+        on_gpu = wide.to(dev).as_strided(view.shape, view.stride(), view.storage_offset())
+        ids, weights = route_experts(on_gpu, 3)
+        want_ids, want = ref.route(view, 3)
+        assert torch.equal(ids.cpu(), want_ids) and torch.allclose(weights.cpu().double(), want, rtol=1.001 * ref.U32, atol=0)
+    ids, weights = route_experts(torch.empty(0, 24, device=dev), 3)
+    assert ids.shape == weights.shape == (0, 3)
+
+
+# ---- the experts' products ----
+RECIPES = {"t": student_t_weight, "outlier": outlier_weight, "real": lambda o, i, seed: calibrated_weight(o, i, seed, scale=0.0123046875 / 8)[0]}
+
+
+def _layer(dev, experts, hidden, inner, recipe="t", level_bits=(3, 5, 8), gated=True, bias=False, activation="silu", seed=0):
+    from ixrun_amd import StreamingExperts
+    from ixrun_amd.quantize import decode_to_weight, int8x_quantize
+
+    make, rows = RECIPES[recipe], 2 * inner if gated else inner
+    gate_up = [int8x_quantize(make(rows, hidden, seed=seed + 2 * e), level_bits) for e in range(experts)]
+    down = [int8x_quantize(make(hidden, inner, seed=seed + 2 * e + 1), level_bits) for e in range(experts)]
+    g = torch.Generator().manual_seed(seed)
+    b1 = (torch.randn(experts, rows, generator=g) * 0.1).bfloat16() if bias else None
+    b2 = (torch.randn(experts, hidden, generator=g) * 0.1).bfloat16() if bias else None
+    layer = StreamingExperts(gate_up, down, activation=activation, gated=gated, gate_up_bias=b1, down_bias=b2)
+    dense = dict(gate_up=torch.stack([decode_to_weight(p) for p in gate_up]).to(dev), down=torch.stack([decode_to_weight(p) for p in down]).to(dev),
+                 act=activation, gated=gated, gate_up_bias=b1.to(dev) if bias else None, down_bias=b2.to(dev) if bias else None)
+    return layer, dense
+
+
+def _call(dev, tokens, top_k, experts, hidden, seed=1, skew=0.0, residual=False):
+    g = torch.Generator().manual_seed(seed)
+    x = torch.randn(tokens, hidden, generator=g).bfloat16().to(dev)
+    logits = torch.randn(tokens, experts, generator=g) + skew * torch.arange(experts)
+    ids = logits.topk(top_k, 1)[1].to(torch.int32).to(dev)
+    weights = torch.rand(tokens, top_k, generator=g).to(dev)
+    return x, ids, weights, torch.randn(tokens, hidden, generator=g).bfloat16().to(dev) if residual else None
+
+
+def _close(y, want, bound):
+    off = (y.double() - want).abs()
+    assert y.dtype == torch.bfloat16 and y.shape == want.shape
+    assert bool((off <= bound).all()), f"{int((off > bound).sum())} of {off.numel()} elements, worst {float((off / bound).max()):.2f} bounds"
+
+
+@pytest.mark.parametrize("recipe,level_bits", [("t", (3, 5, 8)), ("real", (3, 5, 8)), ("outlier", (4, 8)), ("outlier", (3, 4, 5, 6, 8)), ("real", (6, 8))])
+@pytest.mark.parametrize("tokens", [1, 2, 7, 40, 150])
+def test_experts_by_scheme_and_tokens(dev, recipe, level_bits, tokens):
+    layer, dense = _layer(dev, 6, 1024, 320, recipe, level_bits)
+    x, ids, weights, residual = _call(dev, tokens, 3, 6, 1024, residual=True)
+    _close(layer(x, ids, weights, residual), *ref.experts(x, ids, weights, **dense, residual=residual))
+
+
+@pytest.mark.parametrize("hidden,inner", [(64, 16), (512, 1), (520, 33), (1, 5), (777, 250), (1400, 744), (96, 1300), (2049, 17), (6000, 40)])
+@pytest.mark.parametrize("tokens", [1, 21])
+@pytest.mark.parametrize("gated,bias,activation", [(True, True, "gelu_tanh"), (False, False, "relu2")])
+def test_experts_by_size(dev, hidden, inner, tokens, gated, bias, activation):
+    layer, dense = _layer(dev, 3, hidden, inner, "outlier", gated=gated, bias=bias, activation=activation)
+    x, ids, weights, _ = _call(dev, tokens, 2, 3, hidden)
+    _close(layer(x, ids, weights), *ref.experts(x, ids, weights, **dense))
+
+
+@pytest.mark.parametrize("activation", ["none", "silu", "gelu", "gelu_tanh", "relu", "relu2"])
+@pytest.mark.parametrize("gated", [True, False])
+def test_experts_by_activation(dev, activation, gated):
+    layer, dense = _layer(dev, 4, 256, 96, "outlier", gated=gated, activation=activation)
+    x, ids, weights, _ = _call(dev, 11, 2, 4, 256)
+    _close(layer(x, ids, weights), *ref.experts(x, ids, weights, **dense))
+
+
+@pytest.mark.parametrize("tokens", [3, 90])
+def test_experts_of_uneven_and_missing_places(dev, tokens):
+    """All tokens with one expert, experts without any token, places without an expert (whose weights may be anything), tokens of nothing else, an
+    expert twice."""
+    layer, dense = _layer(dev, 5, 512, 64, "t")
+    x, ids, weights, residual = _call(dev, tokens, 3, 5, 512, residual=True)
+    ids[:] = 2
+    _close(layer(x, ids, weights), *ref.experts(x, ids, weights, **dense))
+    x, ids, weights, residual = _call(dev, tokens, 3, 5, 512, skew=2.0, residual=True)
+    ids[::2, 1] = -1
+    ids[1] = -1
+    ids[-1, 0] = 5
+    ids[-1, 2] = 2 ** 31 - 1
+    clean = torch.where((ids >= 0) & (ids < 5), weights, 0)
+    weights = torch.where((ids >= 0) & (ids < 5), weights, math.nan)
+    y = layer(x, ids, weights, residual)
+    _close(y, *ref.experts(x, ids, clean, **dense, residual=residual))
+    assert torch.equal(y[1], residual[1])
+    assert torch.equal(layer(x, ids.long(), weights, residual), y)
+    far = torch.where(ids < 0, torch.full_like(ids, -1).long() * 2 ** 40, ids.long())
+    assert torch.equal(layer(x, far, weights, residual), y)
+
+
+def test_experts_rows_do_not_hang_on_each_other(dev):
+    """A row of infinities and NaN leaves the others as they are, and a token's result is the same wherever it stands."""
+    layer, dense = _layer(dev, 4, 512, 64, "real")
+    x, ids, weights, _ = _call(dev, 60, 2, 4, 512)
+    y = layer(x, ids, weights)
+    wild = x.clone()
+    wild[5] = math.inf
+    wild[17, 3] = math.nan
+    z = layer(wild, ids, weights)
+    same = torch.ones(60, dtype=torch.bool)
+    same[[5, 17]] = False
+    assert torch.equal(z[same], y[same]) and bool(z[17].isnan().all())
+    order = torch.randperm(60, generator=torch.Generator().manual_seed(2)).to(dev)
+    assert torch.equal(layer(x[order], ids[order], weights[order]), y[order])
+
+
+def test_experts_of_views(dev):
+    layer, _ = _layer(dev, 4, 264, 64, "t")
+    x, ids, weights, residual = _call(dev, 24, 2, 4, 264, residual=True)
+    want = layer(x, ids, weights, residual)
+    apart = torch.zeros(24, 400, dtype=torch.bfloat16, device=dev)
+    for start in (0, 1, 3):
+        view = apart[:, start:start + 264]
+        view.copy_(x)
+        assert torch.equal(layer(view, ids, weights, residual), want)
+        assert torch.equal(layer(x, ids, weights, view.copy_(residual)), want)
+    assert torch.equal(layer(x.t().contiguous().t(), ids.t().contiguous().t(), weights.t().contiguous().t(), residual), want)
+    deep = layer(x.view(2, 12, 264), ids.view(2, 12, 2), weights.view(2, 12, 2), residual.view(2, 12, 264))
+    assert deep.shape == (2, 12, 264) and torch.equal(deep.view(24, 264), want)
+    assert layer(x[:0], ids[:0], weights[:0]).shape == (0, 264)
+    # weights of another type are taken as they are
+    assert torch.equal(layer(x, ids, weights.bfloat16()), layer(x, ids, weights.bfloat16().float()))
+
+
+def test_experts_refusals(dev):
+    layer, _ = _layer(dev, 2, 64, 16)
+    x, ids, weights, residual = _call(dev, 3, 1, 2, 64, residual=True)
+    with pytest.raises(TypeError):
+        layer(x.float(), ids, weights)
+    with pytest.raises(TypeError):
+        layer(x, ids.short(), weights)
+    with pytest.raises(TypeError):
+        layer(x, ids, ids)
+    with pytest.raises(ValueError):
+        layer(x[:, :63], ids, weights)
+    with pytest.raises(ValueError):
+        layer(x, ids[:2], weights)
+    with pytest.raises(ValueError):
+        layer(x, ids, weights[:, :0])
+    with pytest.raises(ValueError):
+        layer(x, ids, weights, residual[:2])
+    with pytest.raises(RuntimeError):
+        layer(x.cpu(), ids, weights)
+    with pytest.raises(RuntimeError):
+        layer(x, ids.cpu(), weights)
+    with pytest.raises(RuntimeError, match="no gradient"):
+        layer(x.clone().requires_grad_(), ids, weights)
+    with pytest.raises(TypeError, match="cast"):
+        _layer(dev, 2, 64, 16)[0].float()
+
+
+def test_experts_state(dev):
+    """A state of the same sizes is loaded as a whole; parts of one and lists that do not fit are refused."""
+    layer, dense = _layer(dev, 3, 256, 48, "t")
+    other, _ = _layer(dev, 3, 256, 48, "t")
+    x, ids, weights, _ = _call(dev, 5, 2, 3, 256)
+    state = {k: v.clone() for k, v in layer.state_dict().items()}
+    for v in other.state_dict().values():
+        v.zero_()
+    other.load_state_dict(state)
+    assert torch.equal(other(x, ids, weights), layer(x, ids, weights))
+    other.load_state_dict({k: v.cpu().to(dev) for k, v in state.items()}, assign=True)
+    assert torch.equal(other(x, ids, weights), layer(x, ids, weights))
+    with pytest.raises(RuntimeError, match="a part of"):
+        other.load_state_dict({k: v for k, v in state.items() if k != "_first_pos"}, strict=False)
+    wrong = dict(state, _second_off=state["_second_off"] + 1 << 20)
+    with pytest.raises(RuntimeError, match="does not fit"):
+        other.load_state_dict(wrong)
+    assert torch.equal(other(x, ids, weights), layer(x, ids, weights))
+
+
+@pytest.mark.parametrize("tokens", [1, 33])
+def test_experts_from_a_graph_and_another_stream(dev, tokens):
+    from ixrun_amd import route_experts
+
+    layer, dense = _layer(dev, 8, 512, 128, "real")
+    x, _, _, residual = _call(dev, tokens, 2, 8, 512, residual=True)
+    router = torch.randn(8, 512, generator=torch.Generator().manual_seed(4)).to(dev) * 0.05
+
+    def block(x, residual):
+        ids, weights = route_experts(x.float() @ router.t(), 2)
+        return layer(x, ids, weights, residual=residual), ids, weights
+
+    want = block(x, residual)[0]
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        again = block(x, residual)[0]
+    torch.cuda.current_stream().wait_stream(side)
+    assert torch.equal(again, want)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        y, ids, weights = block(x, residual)
+    for seed in range(3):
+        x.copy_(torch.randn(x.shape, generator=torch.Generator().manual_seed(seed)).bfloat16())
+        graph.replay()
+        eager, eager_ids, _ = block(x, residual)
+        torch.cuda.synchronize()
+        assert torch.equal(y, eager) and torch.equal(ids, eager_ids)
+        _close(y, *ref.experts(x, ids, weights, **dense, residual=residual))
