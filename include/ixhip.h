@@ -273,6 +273,33 @@ int ixh_lanes_gemm(const IxhLanes *lanes, const uint16_t *x, int64_t ldx, const 
 size_t ixh_lanes_gemm_workspace_bytes(const IxhLanes *lanes, int32_t m);
 
 /*
+ * The product with what follows it, in one rounding:
+ *   y[j, r] = bf16( act( sum_k f32(x[j, k]) * f32(w[r, k]) + bias[r] ) * multiplier[j, r] + residual[j, r] ),  1 <= m <= 4096,
+ * fp32 throughout.  bias, multiplier and residual are bf16 and may be NULL (0, 1 and 0); the last two may be y itself, at y's stride.
+ * From 17 rows on IXH_EUNSUPPORTED for what ixh_lanes_gemm does not take.
+ */
+#define IXH_ACT_NONE 0
+#define IXH_ACT_SILU 1
+#define IXH_ACT_GELU 2      /* 0.5 v (1 + erf(v / sqrt 2)) */
+#define IXH_ACT_GELU_TANH 3 /* 0.5 v (1 + tanh(sqrt(2 / pi) (v + 0.044715 v^3))) */
+#define IXH_ACT_RELU 4
+#define IXH_ACT_RELU2 5     /* max(v, 0)^2 */
+typedef struct IxhEpilogue {
+    int32_t activation;
+    const uint16_t *multiplier;
+    int64_t ld_multiplier;
+    const uint16_t *residual;
+    int64_t ld_residual;
+} IxhEpilogue;
+int ixh_lanes_product(const IxhLanes *lanes, const uint16_t *x, int64_t ldx, const uint16_t *bias, int32_t m, const IxhEpilogue *epilogue,
+                      uint16_t *y, int64_t ldy, void *workspace, size_t workspace_bytes, ixh_stream_t stream);
+size_t ixh_lanes_product_workspace_bytes(const IxhLanes *lanes, int32_t m);
+
+/* The same of sums that are there already, in bf16 [m, ldv]: y = bf16( act(v) * multiplier + residual ), any m; y may be v. */
+int ixh_epilogue(const uint16_t *v, int64_t ldv, int64_t m, int64_t out_f, const IxhEpilogue *epilogue, uint16_t *y, int64_t ldy,
+                 ixh_stream_t stream);
+
+/*
  * Routing of tokens to experts.  Per row of `experts` logits (dtype IXH_F32, IXH_F16 or IXH_BF16, a row every `ld` elements) the top_k chosen
  * experts, best first, to ids [tokens, top_k] and their weights to weights [tokens, top_k].
  *   scores   p = softmax or sigmoid (IXH_SCORE_*) of the open experts' logits; an expert whose logit is -infinity is closed
@@ -308,12 +335,6 @@ int ixh_route(const IxhRouting *routing, const void *logits, int32_t dtype, int6
  * the last zero.  Its bias (bf16, may be NULL) is [n_experts, 2 * inner], the gate's first ([n_experts, inner] if not gated).  `second` is
  * hidden x inner, its bias [n_experts, hidden].
  */
-#define IXH_ACT_NONE 0
-#define IXH_ACT_SILU 1
-#define IXH_ACT_GELU 2      /* 0.5 v (1 + erf(v / sqrt 2)) */
-#define IXH_ACT_GELU_TANH 3 /* 0.5 v (1 + tanh(sqrt(2 / pi) (v + 0.044715 v^3))) */
-#define IXH_ACT_RELU 4
-#define IXH_ACT_RELU2 5     /* max(v, 0)^2 */
 typedef struct IxhExpertMatrix {
     int32_t bits;
     int64_t out_f;

@@ -65,6 +65,11 @@ IXH_SCORE_SOFTMAX, IXH_SCORE_SIGMOID = 0, 1
 ACTIVATIONS = {None: 0, "none": 0, "silu": 1, "gelu": 2, "gelu_tanh": 3, "relu": 4, "relu2": 5}  # IXH_ACT_*
 
 
+class IxhEpilogue(C.Structure):
+    _fields_ = [("activation", C.c_int32), ("multiplier", C.c_void_p), ("ld_multiplier", C.c_int64), ("residual", C.c_void_p),
+                ("ld_residual", C.c_int64)]
+
+
 class IxhRouting(C.Structure):
     _fields_ = [(name, C.c_int32) for name in ("experts", "top_k", "n_groups", "top_groups", "scoring", "renormalize")] + [("scale", C.c_float)]
 
@@ -132,7 +137,7 @@ EXPORTS = (
     "ixh_decode_unranked_ws",
     "ixh_lanes_plane_words", "ixh_lanes_cells", "ixh_lanes_pack", "ixh_lanes_list", "ixh_lanes_gemv",
     "ixh_lanes_gemv_workspace_bytes", "ixh_lanes_gemm", "ixh_lanes_gemm_workspace_bytes",
-    "ixh_route", "ixh_experts", "ixh_experts_workspace_bytes",
+    "ixh_lanes_product", "ixh_lanes_product_workspace_bytes", "ixh_epilogue", "ixh_route", "ixh_experts", "ixh_experts_workspace_bytes",
 )
 TEST_EXPORTS = ("ixh_set_option",)
 
@@ -221,6 +226,13 @@ def lib() -> C.CDLL:
         L.ixh_lanes_gemm.argtypes = L.ixh_lanes_gemv.argtypes
         L.ixh_lanes_gemm_workspace_bytes.restype = C.c_size_t
         L.ixh_lanes_gemm_workspace_bytes.argtypes = [C.POINTER(IxhLanes), C.c_int32]
+        L.ixh_lanes_product_workspace_bytes.restype = C.c_size_t
+        L.ixh_lanes_product_workspace_bytes.argtypes = [C.POINTER(IxhLanes), C.c_int32]
+        L.ixh_lanes_product.restype = C.c_int
+        L.ixh_lanes_product.argtypes = [C.POINTER(IxhLanes), C.c_void_p, C.c_int64, C.c_void_p, C.c_int32, C.POINTER(IxhEpilogue), C.c_void_p,
+                                        C.c_int64, C.c_void_p, C.c_size_t, C.c_void_p]
+        L.ixh_epilogue.restype = C.c_int
+        L.ixh_epilogue.argtypes = [C.c_void_p, C.c_int64, C.c_int64, C.c_int64, C.POINTER(IxhEpilogue), C.c_void_p, C.c_int64, C.c_void_p]
         L.ixh_route.restype = C.c_int
         L.ixh_route.argtypes = [C.POINTER(IxhRouting), C.c_void_p, C.c_int32, C.c_int64, C.c_int64, C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p]
         L.ixh_experts_workspace_bytes.restype = C.c_size_t

@@ -685,6 +685,55 @@ int ixh_lanes_gemm(const IxhLanes *lanes, const uint16_t *x, int64_t ldx, const 
     return lanes_status(launch_lanes_gemm(d, x, m, ldx, bias, true, y, ldy, ws, (hipStream_t)stream), ws, "lanes_gemm");
 }
 
+static int to_epilogue(const IxhEpilogue *p, int64_t m, int64_t out_f, Epilogue *out) {
+    if (!p) { set_error("epilogue is NULL"); return IXH_EINVAL; }
+    if (!ep_known(p->activation)) { set_error("epilogue: activation %d", p->activation); return IXH_EINVAL; }
+    if (m > 1 && ((p->multiplier && p->ld_multiplier < out_f) || (p->residual && p->ld_residual < out_f))) {
+        set_error("epilogue: ld_multiplier or ld_residual shorter than a row");
+        return IXH_EINVAL;
+    }
+    *out = Epilogue{p->multiplier, p->residual, p->ld_multiplier, p->ld_residual, p->activation};
+    return IXH_OK;
+}
+
+size_t ixh_lanes_product_workspace_bytes(const IxhLanes *lanes, int32_t m) {
+    return m <= 16 ? ixh_lanes_gemv_workspace_bytes(lanes, m) : ixh_lanes_gemm_workspace_bytes(lanes, m);
+}
+
+int ixh_lanes_product(const IxhLanes *lanes, const uint16_t *x, int64_t ldx, const uint16_t *bias, int32_t m, const IxhEpilogue *epilogue,
+                      uint16_t *y, int64_t ldy, void *workspace, size_t workspace_bytes, ixh_stream_t stream) {
+    LanesDev d;
+    Epilogue ep;
+    int rc = to_lanes(lanes, &d, true);
+    if (!rc) rc = to_epilogue(epilogue, m, lanes->out_f, &ep);
+    if (rc) return rc;
+    if (m < 1 || m > kLanesGemmMost) { set_error("m = %d not in 1..%d", m, kLanesGemmMost); return IXH_EINVAL; }
+    if (!x || !y) { set_error("x or y is NULL"); return IXH_EINVAL; }
+    if (m > 1 && (ldx < (int64_t)d.in_f || ldy < (int64_t)d.out_f)) { set_error("ldx or ldy shorter than a row"); return IXH_EINVAL; }
+    LnScratch ws{(float *)workspace, workspace_bytes, 0};
+    if (m <= 16) return lanes_status(launch_lanes_gemv(d, x, m, ldx, bias, y, ldy, ws, ep, (hipStream_t)stream), ws, "lanes_product");
+    if (!lanes_gemm_aligned(d, x, m, ldx)) {
+        set_error("lanes_product: x not 16-byte aligned, or rows of %u at a stride of %lld not whole 16-byte pieces within 4 GB",
+                  d.in_f, (long long)ldx);
+        return IXH_EUNSUPPORTED;
+    }
+    return lanes_status(launch_lanes_gemm(d, x, m, ldx, bias, true, y, ldy, ws, ep, (hipStream_t)stream), ws, "lanes_product");
+}
+
+int ixh_epilogue(const uint16_t *v, int64_t ldv, int64_t m, int64_t out_f, const IxhEpilogue *epilogue, uint16_t *y, int64_t ldy,
+                 ixh_stream_t stream) {
+    Epilogue ep;
+    const int rc = to_epilogue(epilogue, m, out_f, &ep);
+    if (rc) return rc;
+    if (m < 0 || m >= (1ll << 31) || out_f < 1 || out_f >= (1ll << 31)) { set_error("epilogue: %lld x %lld", (long long)m, (long long)out_f); return IXH_EINVAL; }
+    if (m == 0) return IXH_OK;
+    if (!v || !y) { set_error("epilogue: v or y is NULL"); return IXH_EINVAL; }
+    if (m > 1 && (ldv < out_f || ldy < out_f)) { set_error("epilogue: ldv or ldy shorter than a row"); return IXH_EINVAL; }
+    if (launch_epilogue(v, ldv, (uint32_t)m, (uint32_t)out_f, y, ldy, ep, (hipStream_t)stream) == IXH_OK) return IXH_OK;
+    set_error("epilogue: launch failed");
+    return IXH_ELAUNCH;
+}
+
 // ---- experts ----
 int ixh_route(const IxhRouting *r, const void *logits, int32_t dtype, int64_t ld, int64_t tokens, const float *bias, int32_t *ids,
               float *weights, ixh_stream_t stream) {

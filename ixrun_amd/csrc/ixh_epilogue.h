@@ -20,4 +20,32 @@ inline bool ep_known(int act) { return act >= IXH_ACT_NONE && act <= IXH_ACT_REL
 // round-to-nearest-even, NaN stays NaN whatever its bits
 __device__ __forceinline__ uint16_t ep_bf16(float v) { return __builtin_bit_cast(uint16_t, (__bf16)v); }
 
+// bf16(act(sum + bias) * multiplier + residual); multiplier and residual bf16 [rows, ld], or NULL.
+struct Epilogue {
+    const uint16_t *multiplier, *residual;
+    int64_t ld_multiplier, ld_residual;
+    int activation;
+    __device__ __forceinline__ uint16_t output(float sum, uint32_t r, uint32_t at) const {
+        float v = ep_activation(activation, sum);
+        if (multiplier) v *= bf16_bits_to_f32(multiplier[(int64_t)r * ld_multiplier + at]);
+        if (residual) v += bf16_bits_to_f32(residual[(int64_t)r * ld_residual + at]);
+        return ep_bf16(v);
+    }
+};
+
+int launch_epilogue(const uint16_t *v, int64_t ldv, uint32_t m, uint32_t out_f, uint16_t *y, int64_t ldy, Epilogue ep, hipStream_t s);
+
 }  // namespace ixh
+
+// The kernels of ixh_lanes*.hip exist twice: by themselves, and with an epilogue in place of their own output, from the same text, which
+// ixh_lanes*_ep.hip include with IXH_EP.  (As functions that both kernels call, the plain kernels came out with other schedules and, in
+// k_lanes_rows, up to 48 instructions more.)
+#ifdef IXH_EP
+#define EP(name) name##_ep
+#define EP_PARAM , Epilogue ep
+#define EP_ARG , ep
+#else
+#define EP(name) name
+#define EP_PARAM
+#define EP_ARG
+#endif

@@ -28,6 +28,7 @@
 //             32768 * (column / 32768) on.
 #pragma once
 #include "ixh_dev.h"
+#include "ixh_epilogue.h"
 #include "ixh_lanes_bounds.h"
 
 namespace ixh {
@@ -80,10 +81,14 @@ int launch_lanes_list(const uint16_t *w, const LanesDev &L, uint16_t *pos, int8_
 bool lanes_gemv_takes(const LanesDev &L, int m);
 int launch_lanes_gemv(const LanesDev &L, const uint16_t *x, int m, int64_t ldx, const uint16_t *bias, uint16_t *y,
                       int64_t ldy, LnScratch &ws, hipStream_t s);
+int launch_lanes_gemv(const LanesDev &L, const uint16_t *x, int m, int64_t ldx, const uint16_t *bias, uint16_t *y,
+                      int64_t ldy, LnScratch &ws, Epilogue ep, hipStream_t s);
 size_t lanes_rows_workspace_bytes(const LanesDev &L, int m);  // in k_lanes_rows
 size_t lanes_rows_workspace_most(const LanesDev &L);           // of any count from five to sixteen, whichever kernel takes it
 int launch_lanes_rows(const LanesDev &L, const uint16_t *x, int m, int64_t ldx, const uint16_t *bias, uint16_t *y, int64_t ldy,
                       LnScratch &ws, hipStream_t s);
+int launch_lanes_rows(const LanesDev &L, const uint16_t *x, int m, int64_t ldx, const uint16_t *bias, uint16_t *y, int64_t ldy,
+                      LnScratch &ws, Epilogue ep, hipStream_t s);
 // 17 and more rows (ixh_lanes_gemm.hip), the bias added before the one rounding (once) or after one, then rounded again;
 // IXH_EUNSUPPORTED unless lanes_gemm_aligned:
 // x 16-byte aligned, in_f and ldx multiples of 8, x within 4 GB
@@ -91,10 +96,14 @@ bool lanes_gemm_aligned(const LanesDev &L, const uint16_t *x, int m, int64_t ldx
 size_t lanes_gemm_workspace_bytes(const LanesDev &L, int m);
 int launch_lanes_gemm(const LanesDev &L, const uint16_t *x, int m, int64_t ldx, const uint16_t *bias, bool once, uint16_t *y,
                       int64_t ldy, LnScratch &ws, hipStream_t s);
+int launch_lanes_gemm(const LanesDev &L, const uint16_t *x, int m, int64_t ldx, const uint16_t *bias, bool once, uint16_t *y,
+                      int64_t ldy, LnScratch &ws, Epilogue ep, hipStream_t s);
 // of them, those of many rows and large layers (ixh_lanes_prompt.hip): x as above, the bias added once
 bool lanes_prompt_wins(const LanesDev &L, int m);
 size_t lanes_prompt_workspace_bytes(const LanesDev &L, int m);
 int launch_lanes_prompt(const LanesDev &L, const uint16_t *x, int m, int64_t ldx, const uint16_t *bias, uint16_t *y, int64_t ldy,
                         LnScratch &ws, hipStream_t s);
+int launch_lanes_prompt(const LanesDev &L, const uint16_t *x, int m, int64_t ldx, const uint16_t *bias, uint16_t *y, int64_t ldy,
+                        LnScratch &ws, Epilogue ep, hipStream_t s);
 
 }  // namespace ixh

@@ -82,7 +82,7 @@ constexpr uint32_t kLnXPad = 64;      // bytes behind a row of activations in LD
     const uint32_t *__restrict__ plane, const uint16_t *__restrict__ x, const uint32_t *__restrict__ exc_off,                            \
         const uint16_t *__restrict__ scale_at, uint32_t shape, uint32_t all_tiles, uint32_t tiles_per_wg, uint32_t in_f,                 \
         uint32_t inv_tiles, uint32_t list_groups, const uint16_t *__restrict__ exc_pos, const int8_t *__restrict__ exc_val, int64_t ldx, \
-        const uint16_t *__restrict__ bias, uint16_t *__restrict__ y, int64_t ldy, uint32_t out_f
+        const uint16_t *__restrict__ bias, uint16_t *__restrict__ y, int64_t ldy, uint32_t out_f EP_PARAM
 template <int BITS, int MT, bool WIDE, bool BY_WAVE> __device__ __forceinline__ void lv_gemv(LV_ARGUMENTS) {
     extern __shared__ __attribute__((aligned(16))) uint8_t ln_smem[];
     const uint32_t smem = (uint32_t)(uintptr_t)(LN_LDS(uint8_t) *)ln_smem;
@@ -353,19 +353,23 @@ template <int BITS, int MT, bool WIDE, bool BY_WAVE> __device__ __forceinline__ 
             for (uint32_t c = part; c < (BY_WAVE ? n_waves : C); c += 16u) sum += parts[(c * tiles_per_wg + t) * (MT * 4u) + (uint32_t)r * 4u + (lane & 3u)];
             sum = lv_row_sum(sum);
             if (lane < 4 && at < out_f && (uint32_t)r < m) {
+#ifdef IXH_EP
+                y[(int64_t)r * ldy + at] = ep.output(bias ? sum + bf16_bits_to_f32(bias[at]) : sum, (uint32_t)r, at);
+#else
                 uint32_t b = f32_to_bf16_bits(sum);
                 if (bias) b = f32_to_bf16_bits(bf16_bits_to_f32(b) + bf16_bits_to_f32(bias[at]));
                 y[(int64_t)r * ldy + at] = (uint16_t)b;
+#endif
             }
         }
     }
 }
 
-#define LV_PASSED plane, x, exc_off, scale_at, shape, all_tiles, tiles_per_wg, in_f, inv_tiles, list_groups, exc_pos, exc_val, ldx, bias, y, ldy, out_f
-template <int BITS, int MT, bool WIDE> __global__ void __launch_bounds__(1024) k_lanes_gemv(LV_ARGUMENTS) {
+#define LV_PASSED plane, x, exc_off, scale_at, shape, all_tiles, tiles_per_wg, in_f, inv_tiles, list_groups, exc_pos, exc_val, ldx, bias, y, ldy, out_f EP_ARG
+template <int BITS, int MT, bool WIDE> __global__ void __launch_bounds__(1024) EP(k_lanes_gemv)(LV_ARGUMENTS) {
     lv_gemv<BITS, MT, WIDE, false>(LV_PASSED);
 }
-template <int BITS, int MT, bool WIDE> __global__ void __launch_bounds__(1024) k_lanes_gemv_by_wave(LV_ARGUMENTS) {
+template <int BITS, int MT, bool WIDE> __global__ void __launch_bounds__(1024) EP(k_lanes_gemv_by_wave)(LV_ARGUMENTS) {
     lv_gemv<BITS, MT, WIDE, true>(LV_PASSED);
 }
 #undef LV_ARGUMENTS
@@ -383,10 +387,10 @@ template <int BITS, int MT, bool WIDE> __global__ void __launch_bounds__(1024) k
 // ---------------------------------------------------------------------------------------------------------------
 template <int BITS, int MT, int N>
 __global__ void __launch_bounds__(1024)
-k_lanes_gemv_few(const uint32_t *__restrict__ plane, const uint16_t *__restrict__ x, const uint32_t *__restrict__ exc_off,
+EP(k_lanes_gemv_few)(const uint32_t *__restrict__ plane, const uint16_t *__restrict__ x, const uint32_t *__restrict__ exc_off,
                  const uint16_t *__restrict__ scale_at, const uint16_t *__restrict__ bias, uint32_t shape, uint32_t inv_cells,
                  uint32_t out_f, uint32_t in_f, const uint16_t *__restrict__ exc_pos, const int8_t *__restrict__ exc_val,
-                 int64_t ldx, uint16_t *__restrict__ y, int64_t ldy) {
+                 int64_t ldx, uint16_t *__restrict__ y, int64_t ldy EP_PARAM) {
     extern __shared__ __attribute__((aligned(16))) uint8_t ln_smem[];
     using P = LnPairs<BITS, false>;
     const uint32_t smem = (uint32_t)(uintptr_t)(LN_LDS(uint8_t) *)ln_smem;
@@ -512,17 +516,21 @@ k_lanes_gemv_few(const uint32_t *__restrict__ plane, const uint16_t *__restrict_
         if (MT <= 2) sum += ln_dpp<0x128>(sum);
         sum = lv_sum_of_rows(sum);
         if (r < m && out_row < out_f) {
+#ifdef IXH_EP
+            y[(int64_t)r * ldy + out_row] = ep.output(bias ? sum + bf16_bits_to_f32(bias_raw[n]) : sum, r, out_row);
+#else
             uint32_t b = f32_to_bf16_bits(sum);
             if (bias) b = f32_to_bf16_bits(bf16_bits_to_f32(b) + bf16_bits_to_f32(bias_raw[n]));
             y[(int64_t)r * ldy + out_row] = (uint16_t)b;
+#endif
         }
     }
 }
 
 // outputs from the slices' sums, in slice order
 __global__ void __launch_bounds__(256)
-k_lanes_reduce(const float *__restrict__ ws, uint32_t slices, int m, uint32_t out_f, uint32_t ws_ld,
-               const uint16_t *__restrict__ bias, bool once, uint16_t *__restrict__ y, int64_t ldy) {
+EP(k_lanes_reduce)(const float *__restrict__ ws, uint32_t slices, int m, uint32_t out_f, uint32_t ws_ld,
+               const uint16_t *__restrict__ bias, bool once, uint16_t *__restrict__ y, int64_t ldy EP_PARAM) {
     const uint32_t row = blockIdx.x * 256u + threadIdx.x, r = blockIdx.y;
     if (row >= out_f) return;
     const float *p = ws + (size_t)r * ws_ld + row;
@@ -536,18 +544,23 @@ k_lanes_reduce(const float *__restrict__ ws, uint32_t slices, int m, uint32_t ou
         for (uint32_t k = 0; k < 8; ++k)
             if (g + k < slices) sum += v[k];
     }
+#ifdef IXH_EP
+    y[(int64_t)r * ldy + row] = ep.output(bias ? sum + bf16_bits_to_f32(bias[row]) : sum, r, row);
+#else
     uint32_t h = f32_to_bf16_bits(sum);
     if (bias) h = f32_to_bf16_bits((once ? sum : bf16_bits_to_f32(h)) + bf16_bits_to_f32(bias[row]));
     y[(int64_t)r * ldy + row] = (uint16_t)h;
+#endif
 }
 
 int launch_lanes_reduce(const float *ws, uint32_t slices, int m, uint32_t out_f, uint32_t ws_ld, const uint16_t *bias, bool once,
-                        uint16_t *y, int64_t ldy, hipStream_t s) {
-    IXH_LAUNCH(k_lanes_reduce, dim3((out_f + 255u) / 256u, m), dim3(256), 0, s, ws, slices, m, out_f, ws_ld, bias, once,
-                       y, ldy);
+                        uint16_t *y, int64_t ldy EP_PARAM, hipStream_t s) {
+    IXH_LAUNCH(EP(k_lanes_reduce), dim3((out_f + 255u) / 256u, m), dim3(256), 0, s, ws, slices, m, out_f, ws_ld, bias, once,
+                       y, ldy EP_ARG);
     return hipGetLastError() == hipSuccess ? IXH_OK : IXH_ELAUNCH;
 }
 
+#ifndef IXH_EP  // (as it is)
 // ---------------------------------------------------------------------------------------------------------------
 // Writing the layout from the decoded bf16 weights (deploy time): one wave per cell.  value = round(w / scale) gives
 // back the integer exactly (w is value * scale rounded to 8 significant bits, |value| <= 128).
@@ -664,6 +677,7 @@ int launch_lanes_list(const uint16_t *w, const LanesDev &L, uint16_t *pos, int8_
     }
     return hipGetLastError() == hipSuccess ? IXH_OK : IXH_ELAUNCH;
 }
+#endif
 
 // Workgroups of 16, 8 or 4 waves, one, two or four to a CU: the split whose last round of row quads is fullest.  No waves where LDS
 // holds none: its first pass, sixteen waves, decides that.
@@ -697,48 +711,48 @@ template <int BITS, int MT, bool WIDE, bool BY_WAVE = false> static LvSplit lv_s
 // row quads by `tiles` to a workgroup of `waves`, N cells a wave
 template <int BITS, int MT, int N>
 static int lanes_gemv_few_launch(const LanesDev &L, uint32_t tiles, uint32_t waves, const uint16_t *x, int m, int64_t ldx, const uint16_t *bias,
-                                 uint16_t *y, int64_t ldy, hipStream_t s) {
+                                 uint16_t *y, int64_t ldy EP_PARAM, hipStream_t s) {
     const size_t lds = LnPairs<BITS, false>::kLutBytes + MT * (L.n_cells * 1024u + kLnXPad) + tiles * L.n_cells * (MT * 16u);
-    static const bool raised = hipFuncSetAttribute(reinterpret_cast<const void *>(k_lanes_gemv_few<BITS, MT, N>),
+    static const bool raised = hipFuncSetAttribute(reinterpret_cast<const void *>(EP(k_lanes_gemv_few)<BITS, MT, N>),
                                                    hipFuncAttributeMaxDynamicSharedMemorySize, (int)kLnLds) == hipSuccess;
     if (!raised) return IXH_ELAUNCH;
     const bool aligned = ln_whole_pieces((uintptr_t)x, L.in_f, m, ldx);
     const uint32_t shape = L.n_cells | tiles << 8 | (uint32_t)__builtin_ctz(waves) << 16 | (uint32_t)aligned << 19 | (uint32_t)(m - 1) << 20;
     // (a cell / n_cells as a product with 2^16 / n_cells, rounded up: exact for the 32 cells that there are at most)
-    IXH_LAUNCH((k_lanes_gemv_few<BITS, MT, N>), dim3((L.n_tiles + tiles - 1u) / tiles), dim3(kWave * waves), lds, s, L.plane, x, L.exc_off,
-                       L.scale, bias, shape, 65536u / L.n_cells + 1u, L.out_f, L.in_f, L.exc_pos, L.exc_val, ldx, y, ldy);
+    IXH_LAUNCH((EP(k_lanes_gemv_few)<BITS, MT, N>), dim3((L.n_tiles + tiles - 1u) / tiles), dim3(kWave * waves), lds, s, L.plane, x, L.exc_off,
+                       L.scale, bias, shape, 65536u / L.n_cells + 1u, L.out_f, L.in_f, L.exc_pos, L.exc_val, ldx, y, ldy EP_ARG);
     return hipGetLastError() == hipSuccess ? IXH_OK : IXH_ELAUNCH;
 }
 
 template <int BITS, int MT, bool WIDE, bool BY_WAVE = false>
 static int lanes_gemv_launch(const LanesDev &L, const uint16_t *x, int m, int64_t ldx, const uint16_t *bias, uint16_t *y,
-                             int64_t ldy, hipStream_t s) {
+                             int64_t ldy EP_PARAM, hipStream_t s) {
     const auto [best_waves, best_tiles] = lv_split<BITS, MT, WIDE, BY_WAVE>(L);
     // A cell or two a wave: up to two cells a wave k_lanes_gemv is slower or even, see there.  (A thread takes one piece of a row of activations:
     // no more cells in a row than waves.)
     if (best_waves && L.n_cells <= best_waves && best_tiles * L.n_cells <= 2u * best_waves) {
         uint32_t waves = best_waves;
         while (waves / 2u >= best_tiles * L.n_cells) waves /= 2u;
-        if (best_tiles * L.n_cells <= waves) return lanes_gemv_few_launch<BITS, MT, 1>(L, best_tiles, waves, x, m, ldx, bias, y, ldy, s);
-        return lanes_gemv_few_launch<BITS, MT, 2>(L, best_tiles, waves, x, m, ldx, bias, y, ldy, s);
+        if (best_tiles * L.n_cells <= waves) return lanes_gemv_few_launch<BITS, MT, 1>(L, best_tiles, waves, x, m, ldx, bias, y, ldy EP_ARG, s);
+        return lanes_gemv_few_launch<BITS, MT, 2>(L, best_tiles, waves, x, m, ldx, bias, y, ldy EP_ARG, s);
     }
     // Sums by wave where there is no room for sums by cell, which save an LDS read a cell (us from graphs, k_lanes_rows or the smaller
     // pair table in their place / so: two rows 65536 x 20480 at 5 bits 227 / 203, 20480 x 30720 108 / 100, 16384 x 32768 at 3 bits 54.4 / 51.8, 4096 x 36864
     // 20.4 / 21.5; one row 20480 x 40960 at 5 bits 129.6 / 125.8).
     if constexpr (!BY_WAVE && MT <= 2)
         if (!best_waves && L.n_cells > 16u) {
-            const int rc = lanes_gemv_launch<BITS, MT, WIDE, true>(L, x, m, ldx, bias, y, ldy, s);
+            const int rc = lanes_gemv_launch<BITS, MT, WIDE, true>(L, x, m, ldx, bias, y, ldy EP_ARG, s);
             if (rc != IXH_EUNSUPPORTED) return rc;
         }
     // the smaller pair table where rows are too long beside the larger one
     if constexpr (!BY_WAVE && WIDE && (BITS == 4 || BITS == 5) && MT <= 2)
-        if (!best_waves) return lanes_gemv_launch<BITS, MT, false>(L, x, m, ldx, bias, y, ldy, s);
+        if (!best_waves) return lanes_gemv_launch<BITS, MT, false>(L, x, m, ldx, bias, y, ldy EP_ARG, s);
     if (!best_waves) return IXH_EUNSUPPORTED;
     uint32_t log_waves = 31u - (uint32_t)__builtin_clz(best_waves);
     while ((1u << log_waves) > best_tiles * L.n_cells) --log_waves;
     const auto kernel = [] {
-        if constexpr (BY_WAVE) return k_lanes_gemv_by_wave<BITS, MT, WIDE>;
-        else return k_lanes_gemv<BITS, MT, WIDE>;
+        if constexpr (BY_WAVE) return EP(k_lanes_gemv_by_wave)<BITS, MT, WIDE>;
+        else return EP(k_lanes_gemv)<BITS, MT, WIDE>;
     }();
     static const bool raised = hipFuncSetAttribute(reinterpret_cast<const void *>(kernel),
                                                    hipFuncAttributeMaxDynamicSharedMemorySize, (int)kLnLds) == hipSuccess;
@@ -751,20 +765,21 @@ static int lanes_gemv_launch(const LanesDev &L, const uint16_t *x, int m, int64_
     const uint32_t inv_tiles = best_tiles == 1 ? 0u : (uint32_t)(((1ull << 32) + best_tiles - 1u) / best_tiles);
     IXH_LAUNCH(kernel, dim3((L.n_tiles + best_tiles - 1) / best_tiles), dim3(kWave << log_waves),
                        (lv_lds<BITS, MT, WIDE, BY_WAVE>(L, best_tiles, 1u << log_waves)), s, L.plane, x, L.exc_off, L.scale, shape, L.n_tiles, best_tiles, L.in_f,
-                       inv_tiles, L.list_groups, L.exc_pos, L.exc_val, ldx, bias, y, ldy, L.out_f);
+                       inv_tiles, L.list_groups, L.exc_pos, L.exc_val, ldx, bias, y, ldy, L.out_f EP_ARG);
     return hipGetLastError() == hipSuccess ? IXH_OK : IXH_ELAUNCH;
 }
 
 template <int BITS>
 static int lanes_gemv_rows(const LanesDev &L, const uint16_t *x, int m, int64_t ldx, const uint16_t *bias, uint16_t *y,
-                           int64_t ldy, LnScratch &ws, hipStream_t s) {
+                           int64_t ldy, LnScratch &ws EP_PARAM, hipStream_t s) {
     int rc = IXH_EUNSUPPORTED;
-    if (m == 1) rc = lanes_gemv_launch<BITS, 1, true>(L, x, m, ldx, bias, y, ldy, s);
-    else if (m == 2) rc = lanes_gemv_launch<BITS, 2, true>(L, x, m, ldx, bias, y, ldy, s);
-    else if (m <= 4) rc = lanes_gemv_launch<BITS, 4, true>(L, x, m, ldx, bias, y, ldy, s);
-    return rc == IXH_EUNSUPPORTED ? launch_lanes_rows(L, x, m, ldx, bias, y, ldy, ws, s) : rc;
+    if (m == 1) rc = lanes_gemv_launch<BITS, 1, true>(L, x, m, ldx, bias, y, ldy EP_ARG, s);
+    else if (m == 2) rc = lanes_gemv_launch<BITS, 2, true>(L, x, m, ldx, bias, y, ldy EP_ARG, s);
+    else if (m <= 4) rc = lanes_gemv_launch<BITS, 4, true>(L, x, m, ldx, bias, y, ldy EP_ARG, s);
+    return rc == IXH_EUNSUPPORTED ? launch_lanes_rows(L, x, m, ldx, bias, y, ldy, ws EP_ARG, s) : rc;
 }
 
+#ifndef IXH_EP
 // whether lanes_gemv_launch finds a split
 template <int BITS> static bool lanes_gemv_fits(const LanesDev &L, int m) {
     constexpr bool SMALLER = BITS != 4 && BITS != 5;  // (a smaller table of pairs, up to two rows)
@@ -780,14 +795,15 @@ bool lanes_gemv_takes(const LanesDev &L, int m) {
         default: return lanes_gemv_fits<8>(L, m);
     }
 }
+#endif
 
 int launch_lanes_gemv(const LanesDev &L, const uint16_t *x, int m, int64_t ldx, const uint16_t *bias, uint16_t *y,
-                      int64_t ldy, LnScratch &ws, hipStream_t s) {
+                      int64_t ldy, LnScratch &ws EP_PARAM, hipStream_t s) {
     switch (L.bits) {
-        case 3: return lanes_gemv_rows<3>(L, x, m, ldx, bias, y, ldy, ws, s);
-        case 4: return lanes_gemv_rows<4>(L, x, m, ldx, bias, y, ldy, ws, s);
-        case 5: return lanes_gemv_rows<5>(L, x, m, ldx, bias, y, ldy, ws, s);
-        default: return lanes_gemv_rows<8>(L, x, m, ldx, bias, y, ldy, ws, s);
+        case 3: return lanes_gemv_rows<3>(L, x, m, ldx, bias, y, ldy, ws EP_ARG, s);
+        case 4: return lanes_gemv_rows<4>(L, x, m, ldx, bias, y, ldy, ws EP_ARG, s);
+        case 5: return lanes_gemv_rows<5>(L, x, m, ldx, bias, y, ldy, ws EP_ARG, s);
+        default: return lanes_gemv_rows<8>(L, x, m, ldx, bias, y, ldy, ws EP_ARG, s);
     }
 }
 

@@ -1,5 +1,6 @@
 // What the kernels that read the lane layout (ixh_lanes.h) share: a lane's codes to dequantised pairs.
 #pragma once
+#include "ixh_epilogue.h"
 #include "ixh_fast358.h"
 #include "ixh_lanes.h"
 
@@ -193,6 +194,6 @@ inline uint32_t ln_cus() {
 // outputs from `slices` sums each, [slice][activation row][ws_ld], added in slice order; the bias is added to the sum as it is
 // (rounded once) or rounded to bf16
 int launch_lanes_reduce(const float *ws, uint32_t slices, int m, uint32_t out_f, uint32_t ws_ld, const uint16_t *bias, bool once,
-                        uint16_t *y, int64_t ldy, hipStream_t s);
+                        uint16_t *y, int64_t ldy EP_PARAM, hipStream_t s);
 
 }  // namespace ixh

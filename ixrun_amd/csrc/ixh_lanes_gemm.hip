@@ -61,10 +61,10 @@ __device__ __forceinline__ void lg_decode5(const uint32_t (&w)[5], uint32_t lut_
 
 template <int BITS, int MB, int DEPTH>
 __global__ void __launch_bounds__(kLgBlocks *kWave)
-k_lanes_gemm(const uint32_t *__restrict__ plane, const uint16_t *__restrict__ x, const uint16_t *__restrict__ scale_at, uint32_t c_share,
+EP(k_lanes_gemm)(const uint32_t *__restrict__ plane, const uint16_t *__restrict__ x, const uint16_t *__restrict__ scale_at, uint32_t c_share,
              uint32_t c_more, uint32_t b_share, uint32_t b_more, uint32_t in_f, uint32_t ldx, uint32_t m_all, uint32_t most_at_once, uint32_t n_cells, uint32_t n_tiles,
              const uint32_t *__restrict__ exc_off, const uint16_t *__restrict__ exc_pos, const int8_t *__restrict__ exc_val, uint32_t out_f,
-             float *__restrict__ ws, bool ws_aligned, const uint16_t *__restrict__ bias, bool once, uint16_t *__restrict__ y, int64_t ldy) {
+             float *__restrict__ ws, bool ws_aligned, const uint16_t *__restrict__ bias, bool once, uint16_t *__restrict__ y, int64_t ldy EP_PARAM) {
     extern __shared__ __attribute__((aligned(16))) uint8_t lg_smem[];
     using P = LnPairs<BITS, kLgWide<BITS>>;
     constexpr uint32_t kTile = kLgTileBytes;
@@ -326,9 +326,13 @@ k_lanes_gemm(const uint32_t *__restrict__ plane, const uint16_t *__restrict__ x,
 #pragma unroll
                         for (uint32_t k = 0; k < 4; ++k) {
                             if (at + k >= out_f) continue;
+#ifdef IXH_EP
+                            y[(int64_t)r * ldy + at + k] = ep.output(bias ? acc[b][k] + bf16_bits_to_f32(bias[at + k]) : acc[b][k], r, at + k);
+#else
                             uint32_t h = f32_to_bf16_bits(acc[b][k]);
                             if (bias) h = f32_to_bf16_bits((once ? acc[b][k] : bf16_bits_to_f32(h)) + bf16_bits_to_f32(bias[at + k]));
                             y[(int64_t)r * ldy + at + k] = (uint16_t)h;
+#endif
                         }
                     }
                 }
@@ -349,31 +353,35 @@ static size_t lg_bytes(const LanesDev &L, const LgPlan &p, int m) {
     return p.slices > 1 ? (size_t)p.slices * (uint32_t)m * ((L.n_tiles + 3u) / 4u * 16u) * sizeof(float) : 0;
 }
 
+#ifndef IXH_EP
 size_t lanes_gemm_workspace_bytes(const LanesDev &L, int m) {
     return lanes_prompt_wins(L, m) ? lanes_prompt_workspace_bytes(L, m) : lg_bytes(L, lg_cut(L, m), m);
 }
+#endif
 
 template <int BITS, int MB, int DEPTH>
 static int gemm_launch(const LanesDev &L, const LgPlan &p, const uint16_t *x, int m, int64_t ldx, const uint16_t *bias, bool once,
-                       uint16_t *y, int64_t ldy, float *ws, hipStream_t s) {
+                       uint16_t *y, int64_t ldy, float *ws EP_PARAM, hipStream_t s) {
     constexpr size_t lds = LnPairs<BITS, kLgWide<BITS>>::kLutBytes + kLgBlocks * kLgTileBytes + 2u * MB * 4096u;
     static_assert(lds <= kLnLds, "LDS of a CU");
-    static const bool raised = hipFuncSetAttribute(reinterpret_cast<const void *>(k_lanes_gemm<BITS, MB, DEPTH>),
+    static const bool raised = hipFuncSetAttribute(reinterpret_cast<const void *>(EP(k_lanes_gemm)<BITS, MB, DEPTH>),
                                                    hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds) == hipSuccess;
     if (!raised) return IXH_ELAUNCH;
     const uint32_t blocks = (L.n_tiles + 3u) / 4u;
     const LgSplit c(L.n_cells, p.slices), b(blocks, p.groups);
-    IXH_LAUNCH((k_lanes_gemm<BITS, MB, DEPTH>), dim3(p.slices, p.groups, p.m_groups), dim3(kLgBlocks * kWave), lds, s, L.plane, x, L.scale,
+    IXH_LAUNCH((EP(k_lanes_gemm)<BITS, MB, DEPTH>), dim3(p.slices, p.groups, p.m_groups), dim3(kLgBlocks * kWave), lds, s, L.plane, x, L.scale,
                        c.share, c.more, b.share, b.more, L.in_f, (uint32_t)ldx, (uint32_t)m, lg_most_at_once(blocks, p.groups), L.n_cells,
-                       L.n_tiles, L.exc_off, L.exc_pos, L.exc_val, L.out_f, ws, ((uintptr_t)ws & 15u) == 0, bias, once, y, ldy);
+                       L.n_tiles, L.exc_off, L.exc_pos, L.exc_val, L.out_f, ws, ((uintptr_t)ws & 15u) == 0, bias, once, y, ldy EP_ARG);
     if (p.slices > 1)
-        return launch_lanes_reduce(ws, p.slices, m, L.out_f, (L.n_tiles + 3u) / 4u * 16u, bias, once, y, ldy, s);
+        return launch_lanes_reduce(ws, p.slices, m, L.out_f, (L.n_tiles + 3u) / 4u * 16u, bias, once, y, ldy EP_ARG, s);
     return hipGetLastError() == hipSuccess ? IXH_OK : IXH_ELAUNCH;
 }
 
+#ifndef IXH_EP
 bool lanes_gemm_aligned(const LanesDev &L, const uint16_t *x, int m, int64_t ldx) {
     return ((uintptr_t)x & 15u) == 0 && L.in_f % 8u == 0 && (m == 1 || (ldx % 8 == 0 && ldx < (1ll << 31) / m));
 }
+#endif
 
 template <int BITS, class... A>
 static int gemm_rows(const LanesDev &L, const LgPlan &p, A... a) {
@@ -390,17 +398,17 @@ static int gemm_rows(const LanesDev &L, const LgPlan &p, A... a) {
 }
 
 int launch_lanes_gemm(const LanesDev &L, const uint16_t *x, int m, int64_t ldx, const uint16_t *bias, bool once, uint16_t *y,
-                      int64_t ldy, LnScratch &ws, hipStream_t s) {
+                      int64_t ldy, LnScratch &ws EP_PARAM, hipStream_t s) {
     if (!lanes_gemm_aligned(L, x, m, ldx)) return IXH_EUNSUPPORTED;
-    if (lanes_prompt_wins(L, m)) return launch_lanes_prompt(L, x, m, ldx, bias, y, ldy, ws, s);
+    if (lanes_prompt_wins(L, m)) return launch_lanes_prompt(L, x, m, ldx, bias, y, ldy, ws EP_ARG, s);
     const LgPlan p = lg_cut(L, m);
     if (!ws.holds(lg_bytes(L, p, m))) return IXH_EWORKSPACE;
     if (m == 1) ldx = L.in_f;
     switch (L.bits) {
-        case 3: return gemm_rows<3>(L, p, x, m, ldx, bias, once, y, ldy, ws.at, s);
-        case 4: return gemm_rows<4>(L, p, x, m, ldx, bias, once, y, ldy, ws.at, s);
-        case 5: return gemm_rows<5>(L, p, x, m, ldx, bias, once, y, ldy, ws.at, s);
-        default: return gemm_rows<8>(L, p, x, m, ldx, bias, once, y, ldy, ws.at, s);
+        case 3: return gemm_rows<3>(L, p, x, m, ldx, bias, once, y, ldy, ws.at EP_ARG, s);
+        case 4: return gemm_rows<4>(L, p, x, m, ldx, bias, once, y, ldy, ws.at EP_ARG, s);
+        case 5: return gemm_rows<5>(L, p, x, m, ldx, bias, once, y, ldy, ws.at EP_ARG, s);
+        default: return gemm_rows<8>(L, p, x, m, ldx, bias, once, y, ldy, ws.at EP_ARG, s);
     }
 }
 

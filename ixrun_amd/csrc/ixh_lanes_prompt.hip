@@ -20,13 +20,18 @@ struct LpOut {
     uint32_t parts;           // lp_parts: of tiles, for each group of activation rows
 };
 // four weight rows' sums of activation row r: the bias is added before the one rounding
-__device__ __forceinline__ void lp_store(const LpOut &out, uint32_t r, uint32_t row, ln_f32x4 sum) {
+__device__ __forceinline__ void lp_store(const LpOut &out EP_PARAM, uint32_t r, uint32_t row, ln_f32x4 sum) {
     if (r >= out.m || row >= out.out_f) return;
     uint16_t *const to = out.y + (int64_t)r * out.ldy + row;
     uint16_t v[4];
 #pragma unroll
     for (uint32_t k = 0; k < 4; ++k)
+#ifdef IXH_EP
+        if (row + k < out.out_f) v[k] = ep.output(out.bias ? sum[k] + bf16_bits_to_f32(out.bias[row + k]) : sum[k], r, row + k);
+        else v[k] = 0;
+#else
         v[k] = (uint16_t)f32_to_bf16_bits(sum[k] + (out.bias && row + k < out.out_f ? bf16_bits_to_f32(out.bias[row + k]) : 0.0f));
+#endif
     if (out.wide && row + 4u <= out.out_f) {
         *reinterpret_cast<ln_u32x2 *>(to) = ln_u32x2{v[0] | (uint32_t)v[1] << 16, v[2] | (uint32_t)v[3] << 16};
     } else {
@@ -43,7 +48,7 @@ constexpr uint32_t kLpXBlocks = 2;  // row blocks of a workgroup of k_lanes_xtil
 // 8 (l / 16) .. + 7; zeros past the last row and column.  A workgroup writes four column blocks of two row blocks, so that
 // whole lines are read; rows past the last are the last one's (no result has part in them).
 __global__ void __launch_bounds__(256)
-k_lanes_xtile(const uint16_t *__restrict__ x, int64_t ldx, uint32_t m, uint32_t in_f, uint32_t n_kb, uint32_t n_mblk,
+EP(k_lanes_xtile)(const uint16_t *__restrict__ x, int64_t ldx, uint32_t m, uint32_t in_f, uint32_t n_kb, uint32_t n_mblk,
               ln_u32x4 *__restrict__ xt) {
     const uint32_t lane = threadIdx.x & 63u, kb = blockIdx.x * 4u + (threadIdx.x >> 6), col = kb * 32u + (lane >> 4) * 8u;
     const uint16_t *const from = x + min(col, in_f - 8u);
@@ -87,9 +92,9 @@ k_lanes_xtile(const uint16_t *__restrict__ x, int64_t ldx, uint32_t m, uint32_t 
 // ---------------------------------------------------------------------------------------------------------------
 template <int BITS, int MI, int NW>
 __global__ void __launch_bounds__(kLpThreads) __attribute__((amdgpu_waves_per_eu(2, 2)))
-k_lanes_prompt(const uint32_t *__restrict__ plane, const ln_u32x4 *__restrict__ xt, const uint32_t *__restrict__ exc_off,
+EP(k_lanes_prompt)(const uint32_t *__restrict__ plane, const ln_u32x4 *__restrict__ xt, const uint32_t *__restrict__ exc_off,
                const uint16_t *__restrict__ scale_at, uint32_t n_cells, uint32_t n_tiles, uint32_t n_mblk,
-               const uint16_t *__restrict__ exc_pos, const int8_t *__restrict__ exc_val, ln_f32x4 *__restrict__ ws, LpOut out) {
+               const uint16_t *__restrict__ exc_pos, const int8_t *__restrict__ exc_val, ln_f32x4 *__restrict__ ws, LpOut out EP_PARAM) {
     extern __shared__ __attribute__((aligned(16))) uint8_t lp_smem[];
     using P = LnPairs<BITS, true>;
     constexpr uint32_t NI = 8 / NW, MW = 8 / NW;  // weight blocks of a wave, waves along the activation rows
@@ -362,7 +367,7 @@ k_lanes_prompt(const uint32_t *__restrict__ plane, const ln_u32x4 *__restrict__ 
             for (uint32_t i = 0; i < MI; ++i)
 #pragma unroll
                 for (uint32_t b = 0; b < NI; ++b)
-                    lp_store(out, (mb0 + i) * 16u + n, tile * kLpRows + (nw * NI + b) * 16u + 4u * kg, acc[i][b]);
+                    lp_store(out EP_ARG, (mb0 + i) * 16u + n, tile * kLpRows + (nw * NI + b) * 16u + 4u * kg, acc[i][b]);
             continue;
         }
         const uint32_t part = mg * out.parts + lp_part(blockIdx.x, tile, begins, gridDim.x, lp_tiles(n_tiles));
@@ -379,7 +384,7 @@ k_lanes_prompt(const uint32_t *__restrict__ plane, const ln_u32x4 *__restrict__ 
 // in the mean (5120 x 17408, 3 bits, 256 / 512 rows 66.9 / 99.5 -> 65.7 / 98.1 us; two or four runs of 256 sums a workgroup gain less).
 template <int MI, int NW>
 __global__ void __launch_bounds__(256)
-k_lanes_prompt_reduce(const ln_f32x4 *__restrict__ ws, uint32_t groups, uint32_t per, uint32_t tiles, uint32_t n_cells, LpOut out) {
+EP(k_lanes_prompt_reduce)(const ln_f32x4 *__restrict__ ws, uint32_t groups, uint32_t per, uint32_t tiles, uint32_t n_cells, LpOut out EP_PARAM) {
     constexpr uint32_t NI = 8 / NW, MW = 8 / NW, SIZE = kLpWaves * MI * NI * 64u;
     const uint32_t at = blockIdx.x * 256u + threadIdx.x, tile = blockIdx.y, mg = blockIdx.z;
     const uint32_t lane = at & 63u, block = at >> 6, b = block % NI, i = block / NI % MI, wave = block / (NI * MI);
@@ -396,7 +401,7 @@ k_lanes_prompt_reduce(const ln_f32x4 *__restrict__ ws, uint32_t groups, uint32_t
     ln_f32x4 sum = from[(size_t)head * SIZE];
 #pragma unroll 4
     for (uint32_t g = g0 + 1u; g <= g1; ++g) sum += from[(size_t)g * SIZE];
-    lp_store(out, r, row, sum);
+    lp_store(out EP_ARG, r, row, sum);
 }
 
 struct LpPlan { uint32_t mi, nw, m_groups, groups, n_mblk; };
@@ -420,6 +425,7 @@ static LpPlan lp_plan(const LanesDev &L, int m) {
 static size_t lp_x_bytes(const LanesDev &L, const LpPlan &p) { return (size_t)L.n_cells * 16u * p.n_mblk * 1024u; }
 static uint32_t lp_part_size(const LpPlan &p) { return kLpWaves * p.mi * (8u / p.nw) * 64u; }  // 16-byte units
 
+#ifndef IXH_EP
 // Above 128 rows and 3 * 2^23 weights.  Fewer rows do not hide the decode behind their products, and fewer weights leave a workgroup a
 // few cells, which the pipeline's start and the sums' way through memory outweigh.  us, k_lanes_gemm against this: 5120 x 17408
 // (3 bits) 50 / 53 at 128 rows, 61 / 52 at 144, 138 / 97 at 512; 5120 x 5120 25 / 28, 27 / 29, 56 / 48; 5120 x 4096 25 / 28 at 144
@@ -431,54 +437,57 @@ bool lanes_prompt_wins(const LanesDev &L, int m) {
     return m > 128 && (uint64_t)L.out_f * L.in_f > 3u << 23 && (uint64_t)lp_tiles(L.n_tiles) * L.n_cells < 1u << 24 &&
            (uint64_t)L.n_cells * 16u * (((uint32_t)m + 15u) / 16u) * 1024u < 1ull << 31;
 }
+#endif
 
 // (15: to the next whole 16 bytes of whatever address is given)
 static size_t lp_bytes(const LanesDev &L, const LpPlan &p) {
     return 15u + lp_x_bytes(L, p) + (size_t)p.m_groups * lp_parts(p.groups, lp_tiles(L.n_tiles)) * lp_part_size(p) * 16u;
 }
+#ifndef IXH_EP
 size_t lanes_prompt_workspace_bytes(const LanesDev &L, int m) { return lp_bytes(L, lp_plan(L, m)); }
+#endif
 
 template <int BITS, int MI, int NW>
-static int prompt_launch(const LanesDev &L, const LpPlan &p, const ln_u32x4 *xt, ln_f32x4 *sums, const LpOut &out, hipStream_t s) {
+static int prompt_launch(const LanesDev &L, const LpPlan &p, const ln_u32x4 *xt, ln_f32x4 *sums, const LpOut &out EP_PARAM, hipStream_t s) {
     constexpr size_t lds = LnPairs<BITS, true>::kLutBytes + 2u * kLpTile + 16u * kLpRounds * kLpThreads + kWave * 4u;
     static_assert(lds <= kLnLds, "LDS of a CU");
-    static const bool raised = hipFuncSetAttribute(reinterpret_cast<const void *>(k_lanes_prompt<BITS, MI, NW>),
+    static const bool raised = hipFuncSetAttribute(reinterpret_cast<const void *>(EP(k_lanes_prompt)<BITS, MI, NW>),
                                                    hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds) == hipSuccess;
     if (!raised) return IXH_ELAUNCH;
     const dim3 grid(p.groups, p.m_groups);
-    hipLaunchKernelGGL((k_lanes_prompt<BITS, MI, NW>), grid, dim3(kLpThreads), lds, s, L.plane, xt, L.exc_off, L.scale, L.n_cells, L.n_tiles,
-                       p.n_mblk, L.exc_pos, L.exc_val, sums, out);
+    hipLaunchKernelGGL((EP(k_lanes_prompt)<BITS, MI, NW>), grid, dim3(kLpThreads), lds, s, L.plane, xt, L.exc_off, L.scale, L.n_cells, L.n_tiles,
+                       p.n_mblk, L.exc_pos, L.exc_val, sums, out EP_ARG);
     return IXH_OK;
 }
 
 template <int BITS>
-static int prompt_rows(const LanesDev &L, const LpPlan &p, const ln_u32x4 *xt, ln_f32x4 *sums, const LpOut &out, hipStream_t s) {
-    if (p.nw == 1) return p.mi == 3 ? prompt_launch<BITS, 3, 1>(L, p, xt, sums, out, s) : prompt_launch<BITS, 4, 1>(L, p, xt, sums, out, s);
-    return p.mi == 3 ? prompt_launch<BITS, 3, 2>(L, p, xt, sums, out, s) : prompt_launch<BITS, 4, 2>(L, p, xt, sums, out, s);
+static int prompt_rows(const LanesDev &L, const LpPlan &p, const ln_u32x4 *xt, ln_f32x4 *sums, const LpOut &out EP_PARAM, hipStream_t s) {
+    if (p.nw == 1) return p.mi == 3 ? prompt_launch<BITS, 3, 1>(L, p, xt, sums, out EP_ARG, s) : prompt_launch<BITS, 4, 1>(L, p, xt, sums, out EP_ARG, s);
+    return p.mi == 3 ? prompt_launch<BITS, 3, 2>(L, p, xt, sums, out EP_ARG, s) : prompt_launch<BITS, 4, 2>(L, p, xt, sums, out EP_ARG, s);
 }
 
 int launch_lanes_prompt(const LanesDev &L, const uint16_t *x, int m, int64_t ldx, const uint16_t *bias, uint16_t *y, int64_t ldy,
-                        LnScratch &ws, hipStream_t s) {
+                        LnScratch &ws EP_PARAM, hipStream_t s) {
     const LpPlan p = lp_plan(L, m);
     if (!ws.holds(lp_bytes(L, p))) return IXH_EWORKSPACE;
     ln_u32x4 *const xt = reinterpret_cast<ln_u32x4 *>(((uintptr_t)ws.at + 15u) & ~(uintptr_t)15u);
     ln_f32x4 *const sums = reinterpret_cast<ln_f32x4 *>(reinterpret_cast<uint8_t *>(xt) + lp_x_bytes(L, p));
     const uint32_t n_kb = L.n_cells * 16u, tiles = lp_tiles(L.n_tiles);
-    hipLaunchKernelGGL(k_lanes_xtile, dim3(n_kb / 4u, (p.n_mblk + kLpXBlocks - 1u) / kLpXBlocks), dim3(256), 0, s, x, ldx, (uint32_t)m, L.in_f, n_kb, p.n_mblk, xt);
+    hipLaunchKernelGGL(EP(k_lanes_xtile), dim3(n_kb / 4u, (p.n_mblk + kLpXBlocks - 1u) / kLpXBlocks), dim3(256), 0, s, x, ldx, (uint32_t)m, L.in_f, n_kb, p.n_mblk, xt);
     const LpOut out{bias, y, ldy, (uint32_t)m, L.out_f, ((uintptr_t)y & 7u) == 0 && ldy % 4 == 0, lp_parts(p.groups, tiles)};
     int rc;
     switch (L.bits) {
-        case 3: rc = prompt_rows<3>(L, p, xt, sums, out, s); break;
-        case 4: rc = prompt_rows<4>(L, p, xt, sums, out, s); break;
-        case 5: rc = prompt_rows<5>(L, p, xt, sums, out, s); break;
-        default: rc = prompt_rows<8>(L, p, xt, sums, out, s); break;
+        case 3: rc = prompt_rows<3>(L, p, xt, sums, out EP_ARG, s); break;
+        case 4: rc = prompt_rows<4>(L, p, xt, sums, out EP_ARG, s); break;
+        case 5: rc = prompt_rows<5>(L, p, xt, sums, out EP_ARG, s); break;
+        default: rc = prompt_rows<8>(L, p, xt, sums, out EP_ARG, s); break;
     }
     if (rc != IXH_OK) return rc;
     if (out.parts) {
-        const auto reduce = p.nw == 1 ? p.mi == 3 ? k_lanes_prompt_reduce<3, 1> : k_lanes_prompt_reduce<4, 1>
-                                      : p.mi == 3 ? k_lanes_prompt_reduce<3, 2> : k_lanes_prompt_reduce<4, 2>;
+        const auto reduce = p.nw == 1 ? p.mi == 3 ? EP(k_lanes_prompt_reduce)<3, 1> : EP(k_lanes_prompt_reduce)<4, 1>
+                                      : p.mi == 3 ? EP(k_lanes_prompt_reduce)<3, 2> : EP(k_lanes_prompt_reduce)<4, 2>;
         hipLaunchKernelGGL(reduce, dim3(lp_part_size(p) / 256u, tiles, p.m_groups), dim3(256), 0, s, sums, p.groups,
-                           p.groups % tiles == 0 ? p.groups / tiles : 0u, tiles, L.n_cells, out);
+                           p.groups % tiles == 0 ? p.groups / tiles : 0u, tiles, L.n_cells, out EP_ARG);
     }
     return hipGetLastError() == hipSuccess ? IXH_OK : IXH_ELAUNCH;
 }

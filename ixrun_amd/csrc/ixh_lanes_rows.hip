@@ -35,11 +35,11 @@ template <int BITS, bool WIDE> constexpr uint32_t kLrXAt = (LnPairs<BITS, WIDE>:
 
 template <int BITS, int MT, bool WIDE>
 __global__ void __launch_bounds__(1024)
-k_lanes_rows(const uint32_t *__restrict__ plane, const uint16_t *__restrict__ x, const uint32_t *__restrict__ exc_off,
+EP(k_lanes_rows)(const uint32_t *__restrict__ plane, const uint16_t *__restrict__ x, const uint32_t *__restrict__ exc_off,
              const uint16_t *__restrict__ scale_at, uint32_t n_cells, uint32_t n_tiles, uint32_t in_f, uint32_t shape,
              uint32_t cells_split, uint32_t blocks_split, const uint16_t *__restrict__ exc_pos, const int8_t *__restrict__ exc_val,
              int64_t ldx, uint32_t out_f, uint32_t x_rows, float *__restrict__ ws, const uint16_t *__restrict__ bias,
-             uint16_t *__restrict__ y, int64_t ldy) {
+             uint16_t *__restrict__ y, int64_t ldy EP_PARAM) {
     extern __shared__ __attribute__((aligned(16))) uint8_t lr_smem[];
     using P = LnPairs<BITS, WIDE>;
     const uint32_t smem = (uint32_t)(uintptr_t)(LN_LDS(uint8_t) *)lr_smem;
@@ -316,9 +316,13 @@ k_lanes_rows(const uint32_t *__restrict__ plane, const uint16_t *__restrict__ x,
             if (gridDim.x > 1u) {
                 if (at < 4u * n_tiles) ws[((size_t)slice * m + r) * (n_tiles * 4u) + at] = sum[j];
             } else if (at < out_f) {
+#ifdef IXH_EP
+                y[(int64_t)r * ldy + at] = ep.output(sum[j] + plus, r, at);
+#else
                 uint32_t h = f32_to_bf16_bits(sum[j]);
                 if (bias) h = f32_to_bf16_bits(bf16_bits_to_f32(h) + plus);
                 y[(int64_t)r * ldy + at] = (uint16_t)h;
+#endif
             }
         }
     }
@@ -426,6 +430,7 @@ static size_t lr_bytes(const LanesDev &L, const LrPlan &p, int m) {
     return p.slices > 1 ? (size_t)p.slices * (uint32_t)m * L.n_tiles * 4u * sizeof(float) : 0;
 }
 
+#ifndef IXH_EP
 size_t lanes_rows_workspace_bytes(const LanesDev &L, int m) { return lr_bytes(L, lr_plan_of(L, m), m); }
 
 // (k_lanes_gemm cuts the columns finer for fewer rows, and then takes more)
@@ -435,33 +440,34 @@ size_t lanes_rows_workspace_most(const LanesDev &L) {
         for (int m = 9; m <= 16; ++m) most = max(most, lanes_gemm_workspace_bytes(L, m));
     return most;
 }
+#endif
 
 template <int BITS, int MT, bool WIDE>
 static int rows_launch(const LanesDev &L, const uint16_t *x, int m, int64_t ldx, const uint16_t *bias, uint16_t *y, int64_t ldy,
-                       LnScratch &ws, hipStream_t s) {
+                       LnScratch &ws EP_PARAM, hipStream_t s) {
     const LrPlan p = lr_plan<BITS, MT, WIDE>(L);
     if (!ws.holds(lr_bytes(L, p, m))) return IXH_EWORKSPACE;
-    static const bool raised = hipFuncSetAttribute(reinterpret_cast<const void *>(k_lanes_rows<BITS, MT, WIDE>),
+    static const bool raised = hipFuncSetAttribute(reinterpret_cast<const void *>(EP(k_lanes_rows)<BITS, MT, WIDE>),
                                                    hipFuncAttributeMaxDynamicSharedMemorySize, (int)kLnLds) == hipSuccess;
     if (!raised) return IXH_ELAUNCH;
     const bool pairs = ((uintptr_t)x & 3u) == 0 && L.in_f % 2u == 0 && ldx % 2 == 0 && ldx < 1ll << 27;
     const uint32_t blocks = (L.n_tiles + 3u) / 4u, log_waves = 31u - (uint32_t)__builtin_clz(p.waves);
     const uint32_t shape = (uint32_t)m | log_waves << 5 | (uint32_t)pairs << 8;
-    IXH_LAUNCH((k_lanes_rows<BITS, MT, WIDE>), dim3(p.slices, p.groups), dim3(kWave * p.waves), p.lds, s, L.plane, x, L.exc_off,
+    IXH_LAUNCH((EP(k_lanes_rows)<BITS, MT, WIDE>), dim3(p.slices, p.groups), dim3(kWave * p.waves), p.lds, s, L.plane, x, L.exc_off,
                        L.scale, L.n_cells, L.n_tiles, L.in_f, shape, (L.n_cells / p.slices) << 20 | L.n_cells % p.slices,
-                       (blocks / p.groups) << 24 | blocks % p.groups, L.exc_pos, L.exc_val, ldx, L.out_f, p.x_rows, ws.at, bias, y, ldy);
-    if (p.slices > 1) return launch_lanes_reduce(ws.at, p.slices, m, L.out_f, L.n_tiles * 4u, bias, false, y, ldy, s);
+                       (blocks / p.groups) << 24 | blocks % p.groups, L.exc_pos, L.exc_val, ldx, L.out_f, p.x_rows, ws.at, bias, y, ldy EP_ARG);
+    if (p.slices > 1) return launch_lanes_reduce(ws.at, p.slices, m, L.out_f, L.n_tiles * 4u, bias, false, y, ldy EP_ARG, s);
     return hipGetLastError() == hipSuccess ? IXH_OK : IXH_ELAUNCH;
 }
 
 int launch_lanes_rows(const LanesDev &L, const uint16_t *x, int m, int64_t ldx, const uint16_t *bias, uint16_t *y, int64_t ldy,
-                      LnScratch &ws, hipStream_t s) {
-    if (lr_gemm_wins(L, m) && lanes_gemm_aligned(L, x, m, ldx)) return launch_lanes_gemm(L, x, m, ldx, bias, false, y, ldy, ws, s);
+                      LnScratch &ws EP_PARAM, hipStream_t s) {
+    if (lr_gemm_wins(L, m) && lanes_gemm_aligned(L, x, m, ldx)) return launch_lanes_gemm(L, x, m, ldx, bias, false, y, ldy, ws EP_ARG, s);
 #define LR_ROWS(B)                                                                                                              \
-    (lr_wide<B>(L, m) ? m <= 8 ? rows_launch<B, 8, (B == 4 || B == 5)>(L, x, m, ldx, bias, y, ldy, ws, s)                        \
-                               : rows_launch<B, 16, B == 4>(L, x, m, ldx, bias, y, ldy, ws, s)                                   \
-     : m <= 8         ? rows_launch<B, 8, false>(L, x, m, ldx, bias, y, ldy, ws, s)                                              \
-                      : rows_launch<B, 16, false>(L, x, m, ldx, bias, y, ldy, ws, s))
+    (lr_wide<B>(L, m) ? m <= 8 ? rows_launch<B, 8, (B == 4 || B == 5)>(L, x, m, ldx, bias, y, ldy, ws EP_ARG, s)                        \
+                               : rows_launch<B, 16, B == 4>(L, x, m, ldx, bias, y, ldy, ws EP_ARG, s)                                   \
+     : m <= 8         ? rows_launch<B, 8, false>(L, x, m, ldx, bias, y, ldy, ws EP_ARG, s)                                              \
+                      : rows_launch<B, 16, false>(L, x, m, ldx, bias, y, ldy, ws EP_ARG, s))
     switch (L.bits) {
         case 3: return LR_ROWS(3);
         case 4: return LR_ROWS(4);

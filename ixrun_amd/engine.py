@@ -13,6 +13,7 @@ _split_chunk, _use_fused, _w_buf``), which callers of ``fused_gemv`` read.
 """
 from __future__ import annotations
 
+import ctypes
 import gc
 import os
 
@@ -40,6 +41,7 @@ except AttributeError:  # pragma: no cover
     _current_device = torch.cuda.current_device
 
 LANE_BUFFERS = ("_lane_plane", "_lane_off", "_lane_pos", "_lane_val")
+MAX_PRODUCT_ROWS = 4096  # of one call of ixh_lanes_product
 MAX_FUSED_ROWS = 16  # activation rows served by the fused decode+GEMV kernel
 # With a decode buffer at hand, more rows than this go through decode + library GEMM.  Tensors that are almost all
 # level 1, MI355X: the pair takes 72-75 us on 17408 x 5120 and 5120 x 17408 at any M up to 32 and 34-50 us on
@@ -243,7 +245,6 @@ class StreamingLinear(nn.Module):
             self._scale.reshape(1),
         )
         # what every fused call passes unchanged (the table follows the module when it moves: see _apply)
-        import ctypes
         self._struct_ref = ctypes.byref(self._dp.struct)
         self._table_ptr = self._table.data_ptr() if hasattr(self, "_table") else None
         self._lanes = self._lane_ref = self._bias_ptr = None
@@ -455,6 +456,70 @@ class StreamingLinear(nn.Module):
                     y = y + self._bias.to(y.dtype)
                 return y
         return self._decode_and_multiply(x)
+
+    def product(self, x, activation=None, multiplier=None, residual=None):
+        """``activation(self(x)) * multiplier + residual``, the layer's product with what follows it in one rounding:
+        sum, bias, activation (``silu``, ``gelu``, ``gelu_tanh``, ``relu``, ``relu2`` or none), product and sum are fp32.
+
+        ``multiplier`` and ``residual`` are bf16 of the output's shape, or None: the gate of a gated block takes the other half's
+        output as its multiplier, a block's last projection the residual stream.  bf16 activations on the layer's device; no gradients.
+        From the lane layout it is one kernel's epilogue; without one, and for 17 and more rows that are no whole 16-byte pieces,
+        ``forward`` runs and the rest follows as a launch of its own, from the product rounded to bf16."""
+        for name, t in (("x", x), ("multiplier", multiplier), ("residual", residual)):
+            if t is None:
+                continue
+            if t.dtype is not torch.bfloat16:
+                raise TypeError(f"{name} must be bf16 (got {t.dtype})")
+            if t.device != self._scale.device:
+                raise RuntimeError(f"{name} must live on {self._scale.device} (got {t.device}); the HIP path has no CPU fallback")
+            if t.requires_grad and torch.is_grad_enabled():
+                raise RuntimeError("StreamingLinear.product has no gradient: call it under torch.no_grad(), or with tensors that need none")
+        if activation not in _lib.ACTIVATIONS:
+            raise ValueError(f"activation {activation!r} is none of {[a for a in _lib.ACTIVATIONS if a]}")
+        in_f, out_f, dev = self.in_features, self.out_features, x.device
+        if x.dim() < 1 or x.shape[-1] != in_f:
+            raise ValueError(f"x is {tuple(x.shape)}, expected [..., {in_f}]")
+        shape = x.shape[:-1] + (out_f,)
+
+        def rows_of(t, name, width, wanted):
+            if t.shape != wanted:
+                raise ValueError(f"{name} is {tuple(t.shape)}, expected {tuple(wanted)}")
+            t = t.reshape(-1, width) if t.dim() != 2 else t
+            return t if t.stride(1) == 1 and (t.shape[0] <= 1 or t.stride(0) >= width) else t.contiguous()
+
+        x2 = rows_of(x, "x", in_f, x.shape)
+        m2 = rows_of(multiplier, "multiplier", out_f, shape) if multiplier is not None else None
+        r2 = rows_of(residual, "residual", out_f, shape) if residual is not None else None
+        rows = x2.shape[0]
+        y = torch.empty(shape, dtype=torch.bfloat16, device=dev)
+        if rows == 0:
+            return y
+        act = _lib.ACTIVATIONS[activation]
+
+        def epilogue(at):
+            return _lib.IxhEpilogue(act, m2.data_ptr() + 2 * at * m2.stride(0) if m2 is not None else None, m2.stride(0) if m2 is not None else 0,
+                                    r2.data_ptr() + 2 * at * r2.stride(0) if r2 is not None else None, r2.stride(0) if r2 is not None else 0)
+
+        L = _lib.lib()
+        with _lib.on_device(dev):
+            stream = _raw_stream(dev.index if dev.index is not None else torch.cuda.current_device())
+            if (self._lanes is not None and self._use_fused and not self._gemv_flags and (self._bias is None or self._bias_ptr)
+                    and (rows <= MAX_FUSED_ROWS or (self._gemm_ok and in_f % 8 == 0))):
+                if rows > MAX_FUSED_ROWS and (x2.data_ptr() % 16 or x2.stride(0) % 8):
+                    x2 = x2.clone(memory_format=torch.contiguous_format)
+                step = min(MAX_PRODUCT_ROWS, max(((1 << 31) - 1) // x2.stride(0), MAX_FUSED_ROWS))
+                need = L.ixh_lanes_product_workspace_bytes(self._lane_ref, min(rows, step))
+                if rows > step and rows % step:  # (fewer rows may cut the columns finer)
+                    need = max(need, L.ixh_lanes_product_workspace_bytes(self._lane_ref, rows % step))
+                ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
+                for at in range(0, rows, step):
+                    _lib.check(L.ixh_lanes_product(self._lane_ref, x2.data_ptr() + 2 * at * x2.stride(0), x2.stride(0), self._bias_ptr,
+                                                   min(step, rows - at), ctypes.byref(epilogue(at)), y.data_ptr() + 2 * at * out_f, out_f,
+                                                   ws.data_ptr() if need else None, need, stream))
+                return y
+            v = self.forward(x2)
+            _lib.check(L.ixh_epilogue(v.data_ptr(), v.stride(0), rows, out_f, ctypes.byref(epilogue(0)), y.data_ptr(), out_f, stream))
+        return y
 
     def _decode_and_multiply(self, x):
         w = self._decode()

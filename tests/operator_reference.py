@@ -57,9 +57,13 @@ def rounded(v, off):
     return at, torch.maximum(high - at, at - low)
 
 
-def epilogue(x, w, bias=None, act=None, multiplier=None, residual=None):
-    """bf16(act(x w^T + bias) * multiplier + residual): value before its rounding, and bound with it."""
+def epilogue(x, w, bias=None, act=None, multiplier=None, residual=None, apart=False):
+    """bf16(act(x w^T + bias) * multiplier + residual): value before its rounding, and bound with it.
+
+    `apart`: the product is rounded to bf16 by itself, and its bias added in bf16 (two roundings of what is at most the sum of both)."""
     y, off = product(x, w, bias)
+    if apart:
+        off = off + 2 * U16 * (1 + U16) * (y.abs() + off + (bias.double().abs() if bias is not None else 0))
     y, off = activated(y, off, act)
     if multiplier is not None:
         m = multiplier.double()

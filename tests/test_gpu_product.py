@@ -1,0 +1,202 @@
+"""StreamingLinear.product against its formula in 64 bits (operator_reference.py has the bounds)."""
+import math
+
+import pytest
+import torch
+
+import operator_reference as ref
+from helpers import calibrated_weight, outlier_weight, packed_from_int8, int8_mix, student_t_weight
+
+pytestmark = pytest.mark.gpu
+
+PARTS = [(None, False, False), ("silu", True, False), ("none", False, True), ("gelu_tanh", True, True)]
+
+
+@pytest.fixture(scope="module")
+def dev():
+    assert torch.cuda.is_available(), "these tests need the MI355X"
+    return torch.device("cuda:0")
+
+
+def _layer(dev, out_f, in_f, recipe="t", level_bits=(3, 5, 8), bias=False, lanes=True, seed=0):
+    """A layer and its dequantised weight, on the GPU from the start where that is large."""
+    from ixrun_amd import StreamingLinear
+    from ixrun_amd.quantize import decode_to_weight, int8x_quantize, quantize_for_deploy
+
+    if recipe == "mix8":  # most of the weights above 15: a plane of 8 bits
+        packed = packed_from_int8(int8_mix("only_l3", out_f * in_f, seed), out_f, in_f, level_bits=level_bits)
+    elif out_f * in_f > 1 << 22:
+        g = torch.Generator(dev).manual_seed(seed)
+        w = torch.randn(out_f, in_f, generator=g, device=dev) * 0.02
+        w[0, 0] = {"t": 0.7, "real": 0.2}[recipe]
+        packed = quantize_for_deploy(w.bfloat16(), level_bits)
+    else:
+        make = {"t": student_t_weight, "outlier": outlier_weight, "real": lambda o, i, seed: calibrated_weight(o, i, seed, scale=0.0123046875 / 8)[0]}[recipe]
+        packed = int8x_quantize(make(out_f, in_f, seed=seed), level_bits)
+    b = (torch.randn(out_f, generator=torch.Generator().manual_seed(seed)) * 0.5).bfloat16() if bias else None
+    layer = StreamingLinear(packed, bias=b, lanes=lanes)
+    if out_f * in_f > 1 << 22:
+        flat = torch.empty(out_f * in_f, dtype=torch.bfloat16, device=dev)
+        layer._dp.decode(*layer._decode_table(), out_bf16=flat)
+        return layer, flat.view(out_f, in_f), b.to(dev) if bias else None
+    return layer, decode_to_weight(packed).to(dev), b.to(dev) if bias else None
+
+
+def _operands(dev, rows, out_f, in_f, multiplier, residual, seed=1):
+    g = torch.Generator(dev).manual_seed(seed)
+    make = lambda *s: torch.randn(*s, generator=g, device=dev).bfloat16()
+    return make(rows, in_f), make(rows, out_f) if multiplier else None, make(rows, out_f) if residual else None
+
+
+def _close(y, want, bound):
+    off = (y.double() - want).abs()
+    assert y.dtype == torch.bfloat16 and y.shape == want.shape
+    assert bool((off <= bound).all()), f"{int((off > bound).sum())} of {off.numel()} elements, worst {float((off / bound).max()):.2f} bounds"
+
+
+def _check(dev, layer, w, bias, rows, act, multiplier, residual, apart=False, seed=1):
+    x, m, r = _operands(dev, rows, *w.shape, multiplier, residual, seed)
+    _close(layer.product(x, act, m, r), *ref.epilogue(x, w, bias, act, m, r, apart=apart))
+
+
+@pytest.mark.parametrize("recipe,level_bits", [("t", (3, 5, 8)), ("outlier", (4, 8)), ("real", (3, 5, 8)), ("mix8", (3, 5, 8))])
+@pytest.mark.parametrize("out_f,in_f", [(256, 512), (640, 4608), (1001, 2056)])
+@pytest.mark.parametrize("rows", [1, 2, 4, 7, 8, 13, 16, 17, 50, 100, 200])
+def test_products_by_scheme_and_rows(dev, recipe, level_bits, out_f, in_f, rows):
+    """Planes of 3, 4, 5 and 8 bits; every kind of epilogue once."""
+    layer, w, bias = _layer(dev, out_f, in_f, recipe, level_bits, bias=rows % 2 == 0)
+    act, multiplier, residual = PARTS[(rows + out_f) % 4]
+    _check(dev, layer, w, bias, rows, act, multiplier, residual)
+
+
+@pytest.mark.parametrize("act", ["none", "silu", "gelu", "gelu_tanh", "relu", "relu2"])
+@pytest.mark.parametrize("rows", [1, 6, 40])
+def test_products_by_activation(dev, act, rows):
+    layer, w, bias = _layer(dev, 320, 1024, "outlier", bias=True)
+    for multiplier in (False, True):
+        for residual in (False, True):
+            _check(dev, layer, w, bias, rows, act, multiplier, residual)
+
+
+@pytest.mark.parametrize("out_f,in_f", [(1, 1), (3, 17), (5, 513), (64, 64), (33, 2047), (2000, 520)])
+@pytest.mark.parametrize("rows", [1, 3, 16])
+def test_products_of_odd_sizes(dev, out_f, in_f, rows):
+    layer, w, bias = _layer(dev, out_f, in_f, "outlier", bias=True)
+    _check(dev, layer, w, bias, rows, "silu", True, True, apart=layer._lanes is None)
+
+
+@pytest.mark.parametrize("out_f,in_f,rows", [
+    (17408, 5120, 1), (5120, 17408, 1), (5120, 17408, 12), (17408, 5120, 5), (40960, 2048, 3), (4096, 36864, 2), (5120, 17408, 300), (17408, 5120, 129),
+    (32768, 1024, 400), (12288, 6144, 530), (2048, 2048, 700),
+])
+def test_large_products(dev, out_f, in_f, rows):
+    """The kernels of large layers: sums by wave, several slices and one, whole tiles of a prompt and parts of them."""
+    layer, w, bias = _layer(dev, out_f, in_f, "t", bias=True)
+    _check(dev, layer, w, bias, rows, "gelu_tanh", True, True)
+
+
+def test_a_long_prompt_is_taken_in_parts(dev):
+    layer, w, bias = _layer(dev, 96, 256, "t", bias=True)
+    _check(dev, layer, w, bias, 4096 + 31, "silu", True, True)
+
+
+@pytest.mark.parametrize("rows", [1, 9, 33])
+@pytest.mark.parametrize("how", ["no lanes", "odd rows", "fp32 bias"])
+def test_products_whose_kernel_has_no_epilogue(dev, rows, how):
+    layer, w, bias = _layer(dev, 72, 1023 if how == "odd rows" else 1024, "outlier", bias=True, lanes=how != "no lanes")
+    layer._set_shared_buf(torch.empty(layer.N, dtype=torch.bfloat16, device=dev))
+    if how == "fp32 bias":
+        layer._bias = layer._bias.float()
+        layer._bind()
+    _check(dev, layer, w, bias, rows, "silu", True, True, apart=True)
+
+
+def test_a_product_without_an_epilogue_is_the_forward(dev):
+    layer, _, _ = _layer(dev, 640, 1536, "t")
+    for rows in (1, 4, 12, 40):
+        x = _operands(dev, rows, 640, 1536, False, False)[0]
+        assert torch.equal(layer.product(x), layer(x))
+
+
+def test_products_of_views(dev):
+    layer, _, _ = _layer(dev, 200, 264, "t")
+    for rows in (1, 6, 30):
+        x, m, r = _operands(dev, rows, 200, 264, True, True)
+        want = layer.product(x, "silu", m, r)
+        wide = torch.full((rows, 500), math.nan, dtype=torch.bfloat16, device=dev)
+        for start in (0, 1, 8):
+            view = wide[:, start:start + 264]
+            assert torch.equal(layer.product(view.copy_(x), "silu", m, r), want)
+            view = wide[:, start:start + 200]
+            assert torch.equal(layer.product(x, "silu", view.copy_(m), r), want)
+            assert torch.equal(layer.product(x, "silu", m, view.copy_(r)), want)
+        assert torch.equal(layer.product(x.t().contiguous().t(), "silu", m.t().contiguous().t(), r.t().contiguous().t()), want)
+        deep = layer.product(x.view(1, rows, 264), "silu", m.view(1, rows, 200), r.view(1, rows, 200))
+        assert deep.shape == (1, rows, 200) and torch.equal(deep[0], want)
+    assert torch.equal(layer.product(x[0], "silu", m[0], r[0]), layer.product(x[:1], "silu", m[:1], r[:1])[0])
+    assert layer.product(x[:0], "silu", m[:0], r[:0]).shape == (0, 200)
+
+
+def test_infinities_and_nan_stay_in_their_rows(dev):
+    layer, _, _ = _layer(dev, 128, 512, "t")
+    for rows in (3, 12, 60):
+        x, m, r = _operands(dev, rows, 128, 512, True, True)
+        y = layer.product(x, "silu", m, r)
+        x[1, 7], m[2, 5], r[2, 6] = math.nan, math.inf, -math.inf
+        z = layer.product(x, "silu", m, r)
+        assert bool(z[1].isnan().all()) and torch.equal(z[0], y[0]) and torch.equal(z[3:], y[3:])
+        assert z[2, 6] == -math.inf and not bool(z[2, 5].isfinite()) and torch.equal(z[2, 7:], y[2, 7:])
+
+
+def test_product_refusals(dev):
+    layer, _, _ = _layer(dev, 64, 128)
+    x, m, r = _operands(dev, 3, 64, 128, True, True)
+    with pytest.raises(TypeError):
+        layer.product(x.float())
+    with pytest.raises(TypeError):
+        layer.product(x, None, m.float())
+    with pytest.raises(ValueError):
+        layer.product(x[:, :100])
+    with pytest.raises(ValueError):
+        layer.product(x, None, m[:2])
+    with pytest.raises(ValueError):
+        layer.product(x, None, None, r[:, :5])
+    with pytest.raises(ValueError, match="activation"):
+        layer.product(x, "swish")
+    with pytest.raises(RuntimeError):
+        layer.product(x.cpu())
+    with pytest.raises(RuntimeError, match="no gradient"):
+        layer.product(x.clone().requires_grad_())
+
+
+@pytest.mark.parametrize("rows", [1, 10, 70])
+def test_a_gated_block_from_a_graph_and_another_stream(dev, rows):
+    """Three products in a row, as a block makes them."""
+    gate, w_gate, _ = _layer(dev, 768, 512, "t", seed=1)
+    up, w_up, _ = _layer(dev, 768, 512, "t", seed=2)
+    down, w_down, _ = _layer(dev, 512, 768, "t", seed=3)
+    x = _operands(dev, rows, 1, 512, False, False)[0]
+
+    def block(x):
+        return down.product(gate.product(x, "silu", up(x)), residual=x)
+
+    want = block(x)
+    _close(up(x), *ref.epilogue(x, w_up))
+    h = gate.product(x, "silu", up(x))
+    _close(h, *ref.epilogue(x, w_gate, act="silu", multiplier=up(x)))
+    _close(want, *ref.epilogue(h, w_down, residual=x))
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        again = block(x)
+    torch.cuda.current_stream().wait_stream(side)
+    assert torch.equal(again, want)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        y = block(x)
+    for seed in range(3):
+        x.copy_(_operands(dev, rows, 1, 512, False, False, seed=seed + 10)[0])
+        graph.replay()
+        eager = block(x)
+        torch.cuda.synchronize()
+        assert torch.equal(y, eager)
