@@ -50,6 +50,15 @@ struct ExCall {
     int64_t ldy;
 };
 
+// The slots by expert.  For k_experts_rows tiles of a few slots each, {expert, first place in `order`, how many}; for k_experts_prompt
+// an expert's places are filled up to whole blocks of 16 (with ~0), and the tiles are {expert, first block, blocks}, up to 32 of them.
+struct ExPlan {
+    uint32_t *n_tiles, *n_blocks, *tiles, *order;
+};
+// many tokens to an expert (ixh_experts_prompt.hip); row_tiles and blocks: how many there may be
+int launch_experts_prompt(const ExDev &X, const ExCall &call, const ExPlan &plan, uint32_t row_tiles, uint32_t blocks, void *xt, void *inner,
+                          float *per_slot, hipStream_t s);
+
 size_t experts_workspace_bytes(const ExDev &X, uint32_t tokens, uint32_t top_k);
 int launch_experts(const ExDev &X, const ExCall &call, void *workspace, hipStream_t s);
 

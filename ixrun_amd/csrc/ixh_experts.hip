@@ -16,11 +16,11 @@ namespace ixh {
 // ---------------------------------------------------------------------------------------------------------------
 constexpr uint32_t kExPlanThreads = 1024, kExPlanWaves = kExPlanThreads / kWave;
 
-struct ExPlan {
-    uint32_t *n_tiles;
-    uint32_t *tiles;  // {expert, first of its places in `order`, how many} each
-    uint32_t *order;  // slots
-};
+// Tiles of an expert with n slots: of up to `rows` of them; with rows = 0 of up to 32 blocks of 16, as even as whole eights of blocks
+// allow (what is left of an eighth is as long as the whole).
+__device__ __forceinline__ uint32_t ex_eights(uint32_t n) { return (n + 127u) / 128u; }
+__device__ __forceinline__ uint32_t ex_tiles(uint32_t n, uint32_t rows) { return rows ? (n + rows - 1u) / rows : (ex_eights(n) + 3u) / 4u; }
+__device__ __forceinline__ uint32_t ex_places(uint32_t n, uint32_t rows) { return rows ? n : (n + 15u) & ~15u; }
 
 __global__ void __launch_bounds__(kExPlanThreads)
 k_experts_plan(const int32_t *__restrict__ ids, uint32_t slots, uint32_t experts, uint32_t rows, ExPlan plan) {
@@ -40,18 +40,25 @@ k_experts_plan(const int32_t *__restrict__ ids, uint32_t slots, uint32_t experts
     if (lane == 0) of_wave[wave] = mine;
     __syncthreads();
     uint32_t before = 0, tiles_before = 0;
-    for (uint32_t i = tid; i < e; i += kExPlanThreads) before += hist[i], tiles_before += (hist[i] + rows - 1u) / rows;
+    for (uint32_t i = tid; i < e; i += kExPlanThreads) before += ex_places(hist[i], rows), tiles_before += ex_tiles(hist[i], rows);
     for (int by = 32; by; by >>= 1) before += __shfl_xor(before, by), tiles_before += __shfl_xor(tiles_before, by);
     if (lane == 0) sums[0][wave] = before, sums[1][wave] = tiles_before;
     __syncthreads();
     before = tiles_before = 0;
     for (uint32_t w = 0; w < kExPlanWaves; ++w) before += sums[0][w], tiles_before += sums[1][w];
-    const uint32_t n = hist[e], n_tiles = (n + rows - 1u) / rows;
+    const uint32_t n = hist[e], n_tiles = ex_tiles(n, rows), places = ex_places(n, rows);
     for (uint32_t i = tid; i < n_tiles; i += kExPlanThreads) {
         uint32_t *const t = plan.tiles + 3u * (tiles_before + i);
-        t[0] = e, t[1] = before + i * rows, t[2] = min(rows, n - i * rows);
+        t[0] = e;
+        if (rows) {
+            t[1] = before + i * rows, t[2] = min(rows, n - i * rows);
+        } else {
+            const uint32_t eights = ex_eights(n), b0 = eights * i / n_tiles * 8u, b1 = min(eights * (i + 1u) / n_tiles * 8u, places / 16u);
+            t[1] = before / 16u + b0, t[2] = b1 - b0;
+        }
     }
-    if (e + 1u == experts && tid == 0) *plan.n_tiles = tiles_before + n_tiles;
+    for (uint32_t i = n + tid; i < places; i += kExPlanThreads) plan.order[before + i] = ~0u;
+    if (e + 1u == experts && tid == 0) *plan.n_tiles = tiles_before + n_tiles, *plan.n_blocks = (before + places) / 16u;
     uint32_t at = before;
     for (uint32_t w = 0; w < wave; ++w) at += of_wave[w];
     for (uint32_t i0 = from; i0 < to; i0 += kWave) {
@@ -388,52 +395,78 @@ template <bool FIRST> static int ex_matrix(const ExMatrix &W, const ExRows &R, u
 #undef EX_ROWS
 }
 
-// A call's scratch: the plan, the intermediate (rows of whole 16 bytes) and what each slot's expert makes of it.
+// Many tokens to an expert: 16 and more in the mean.
+// (Rows of up to 2^20 columns: offsets within a tile's rows are 32 bits.)
+static bool ex_many(const ExDev &X, uint32_t slots) {
+    return slots >= 16u * X.experts && std::max(X.first.n_cells, X.second.n_cells) <= 2048u;
+}
+
+// A call's scratch: the plan, the intermediate, what each slot's expert makes of it, and in k_experts_prompt the gathered rows.
 struct ExScratch {
-    uint32_t rows, n_tiles;  // of a tile; tiles at most
-    size_t tiles, order, inner, per_slot, bytes;
+    bool many;
+    uint32_t rows, n_tiles, blocks;  // slots of a tile (0: see ExPlan); tiles and blocks at most
+    size_t tiles, order, x, inner, per_slot, bytes;
     int64_t ld_inner;
 };
 static ExScratch ex_scratch(const ExDev &X, uint32_t tokens, uint32_t top_k) {
     ExScratch w{};
     const uint32_t slots = tokens * top_k;
-    w.rows = slots <= 4u * X.experts ? 8u : 16u;
-    w.n_tiles = std::min(slots, X.experts + slots / w.rows);
+    w.many = ex_many(X, slots);
     size_t at = 256;
     auto take = [&](size_t n) { const size_t from = at; at += (n + 255u) & ~(size_t)255u; return from; };
-    w.tiles = take((size_t)w.n_tiles * 12u);
-    w.order = take((size_t)slots * 4u);
-    w.ld_inner = (int64_t)((X.inner + 7u) & ~7u);
-    w.inner = take((size_t)slots * (size_t)w.ld_inner * 2u);
+    if (w.many) {
+        w.n_tiles = std::min(slots, X.experts) + slots / 512u;
+        w.blocks = std::min(slots, X.experts) + slots / 16u;
+        w.tiles = take((size_t)w.n_tiles * 12u);
+        w.order = take((size_t)w.blocks * 64u);
+        w.x = take((size_t)w.blocks * X.first.n_cells * 16384u);
+        w.inner = take((size_t)w.blocks * X.second.n_cells * 16384u);
+    } else {
+        w.rows = slots <= 4u * X.experts ? 8u : 16u;
+        w.n_tiles = std::min(slots, X.experts + slots / 8u);
+        w.tiles = take((size_t)w.n_tiles * 12u);
+        w.order = take((size_t)slots * 4u);
+        w.ld_inner = (int64_t)((X.inner + 7u) & ~7u);  // rows of whole 16 bytes
+        w.inner = take((size_t)slots * (size_t)w.ld_inner * 2u);
+    }
     w.per_slot = take((size_t)slots * X.hidden * 4u);
     w.bytes = at + 255u;  // to the next whole 256 bytes of whatever address is given
     return w;
 }
 
-size_t experts_workspace_bytes(const ExDev &X, uint32_t tokens, uint32_t top_k) { return tokens ? ex_scratch(X, tokens, top_k).bytes : 0; }
+// Callers may hold a scratch of a larger call: enough for any count of tokens up to this one.
+size_t experts_workspace_bytes(const ExDev &X, uint32_t tokens, uint32_t top_k) {
+    if (!tokens) return 0;
+    const uint32_t few = std::min(tokens, (16u * X.experts - 1u) / top_k);  // the most that are not many
+    return std::max(ex_scratch(X, tokens, top_k).bytes, few ? ex_scratch(X, few, top_k).bytes : 0u);
+}
 
 int launch_experts(const ExDev &X, const ExCall &call, void *workspace, hipStream_t s) {
     const uint32_t slots = call.tokens * call.top_k;
     const ExScratch w = ex_scratch(X, call.tokens, call.top_k);
     uint8_t *const ws = reinterpret_cast<uint8_t *>(((uintptr_t)workspace + 255u) & ~(uintptr_t)255u);
-    const bool planned = slots > X.experts / 4u && call.tokens > 1u;
+    const bool planned = w.many || (slots > X.experts / 4u && call.tokens > 1u);
     const uint32_t n_tiles = planned ? w.n_tiles : slots;
-    ExRows R{};
-    R.x = call.x, R.ldx = call.ldx, R.ids = call.ids, R.experts = X.experts, R.top_k = call.top_k;
-    if (planned) {
-        const ExPlan plan{reinterpret_cast<uint32_t *>(ws), reinterpret_cast<uint32_t *>(ws + w.tiles), reinterpret_cast<uint32_t *>(ws + w.order)};
-        IXH_LAUNCH(k_experts_plan, dim3(X.experts), dim3(kExPlanThreads), 0, s, call.ids, slots, X.experts, w.rows, plan);
-        R.n_tiles = plan.n_tiles, R.tiles = plan.tiles, R.order = plan.order;
+    uint32_t *const counts = reinterpret_cast<uint32_t *>(ws);
+    const ExPlan plan{counts, counts + 1, reinterpret_cast<uint32_t *>(ws + w.tiles), reinterpret_cast<uint32_t *>(ws + w.order)};
+    float *const per_slot = reinterpret_cast<float *>(ws + w.per_slot);
+    if (planned) IXH_LAUNCH(k_experts_plan, dim3(X.experts), dim3(kExPlanThreads), 0, s, call.ids, slots, X.experts, w.rows, plan);
+    int rc;
+    if (w.many) {
+        rc = launch_experts_prompt(X, call, plan, n_tiles, w.blocks, ws + w.x, ws + w.inner, per_slot, s);
+    } else {
+        ExRows R{};
+        R.x = call.x, R.ldx = call.ldx, R.ids = call.ids, R.experts = X.experts, R.top_k = call.top_k;
+        if (planned) R.n_tiles = plan.n_tiles, R.tiles = plan.tiles, R.order = plan.order;
+        R.out = ws + w.inner, R.ld_out = w.ld_inner, R.activation = X.activation, R.gated = X.gated;
+        rc = ex_matrix<true>(X.first, R, planned ? w.rows : 1u, n_tiles, s);
+        if (rc != IXH_OK) return rc;
+        R.x = reinterpret_cast<const uint16_t *>(ws + w.inner), R.ldx = w.ld_inner;
+        R.out = per_slot, R.ld_out = X.hidden;
+        rc = ex_matrix<false>(X.second, R, planned ? w.rows : 1u, n_tiles, s);
     }
-    R.out = ws + w.inner, R.ld_out = w.ld_inner, R.activation = X.activation, R.gated = X.gated;
-    int rc = ex_matrix<true>(X.first, R, planned ? w.rows : 1u, n_tiles, s);
     if (rc != IXH_OK) return rc;
-    R.x = reinterpret_cast<const uint16_t *>(ws + w.inner), R.ldx = w.ld_inner;
-    R.out = ws + w.per_slot, R.ld_out = X.hidden;
-    rc = ex_matrix<false>(X.second, R, planned ? w.rows : 1u, n_tiles, s);
-    if (rc != IXH_OK) return rc;
-    IXH_LAUNCH(k_experts_join, dim3(call.tokens, (X.hidden + 255u) / 256u), dim3(256), 0, s,
-               reinterpret_cast<const float *>(ws + w.per_slot), call, X.experts, X.hidden);
+    IXH_LAUNCH(k_experts_join, dim3(call.tokens, (X.hidden + 255u) / 256u), dim3(256), 0, s, per_slot, call, X.experts, X.hidden);
     return hipGetLastError() == hipSuccess ? IXH_OK : IXH_ELAUNCH;
 }
 

@@ -127,7 +127,7 @@ def _close(y, want, bound):
 
 
 @pytest.mark.parametrize("recipe,level_bits", [("t", (3, 5, 8)), ("real", (3, 5, 8)), ("outlier", (4, 8)), ("outlier", (3, 4, 5, 6, 8)), ("real", (6, 8))])
-@pytest.mark.parametrize("tokens", [1, 2, 7, 40, 150])
+@pytest.mark.parametrize("tokens", [1, 2, 7, 40, 150, 700])
 def test_experts_by_scheme_and_tokens(dev, recipe, level_bits, tokens):
     layer, dense = _layer(dev, 6, 1024, 320, recipe, level_bits)
     x, ids, weights, residual = _call(dev, tokens, 3, 6, 1024, residual=True)
@@ -135,7 +135,7 @@ def test_experts_by_scheme_and_tokens(dev, recipe, level_bits, tokens):
 
 
 @pytest.mark.parametrize("hidden,inner", [(64, 16), (512, 1), (520, 33), (1, 5), (777, 250), (1400, 744), (96, 1300), (2049, 17), (6000, 40)])
-@pytest.mark.parametrize("tokens", [1, 21])
+@pytest.mark.parametrize("tokens", [1, 21, 75])
 @pytest.mark.parametrize("gated,bias,activation", [(True, True, "gelu_tanh"), (False, False, "relu2")])
 def test_experts_by_size(dev, hidden, inner, tokens, gated, bias, activation):
     layer, dense = _layer(dev, 3, hidden, inner, "outlier", gated=gated, bias=bias, activation=activation)
@@ -147,11 +147,23 @@ def test_experts_by_size(dev, hidden, inner, tokens, gated, bias, activation):
 @pytest.mark.parametrize("gated", [True, False])
 def test_experts_by_activation(dev, activation, gated):
     layer, dense = _layer(dev, 4, 256, 96, "outlier", gated=gated, activation=activation)
-    x, ids, weights, _ = _call(dev, 11, 2, 4, 256)
-    _close(layer(x, ids, weights), *ref.experts(x, ids, weights, **dense))
+    for tokens in (11, 70):
+        x, ids, weights, _ = _call(dev, tokens, 2, 4, 256)
+        _close(layer(x, ids, weights), *ref.experts(x, ids, weights, **dense))
 
 
-@pytest.mark.parametrize("tokens", [3, 90])
+@pytest.mark.parametrize("tokens", [100, 250, 390, 512, 513, 700, 1000, 1100])
+@pytest.mark.parametrize("level_bits", [(3, 5, 8), (4, 8), (6, 8)])
+def test_experts_of_many_tokens(dev, tokens, level_bits):
+    """One expert with all of the tokens: tiles of one to 32 blocks of rows, several of them, the last one odd."""
+    layer, dense = _layer(dev, 2, 1100, 200, "outlier", level_bits, bias=True)
+    x, ids, weights, residual = _call(dev, tokens, 1, 2, 1100, residual=True)
+    ids[:] = 1
+    ids[-3:] = 0
+    _close(layer(x, ids, weights, residual), *ref.experts(x, ids, weights, **dense, residual=residual))
+
+
+@pytest.mark.parametrize("tokens", [3, 20, 90])
 def test_experts_of_uneven_and_missing_places(dev, tokens):
     """All tokens with one expert, experts without any token, places without an expert (whose weights may be anything), tokens of nothing else, an
     expert twice."""
@@ -177,32 +189,34 @@ def test_experts_of_uneven_and_missing_places(dev, tokens):
 def test_experts_rows_do_not_hang_on_each_other(dev):
     """A row of infinities and NaN leaves the others as they are, and a token's result is the same wherever it stands."""
     layer, dense = _layer(dev, 4, 512, 64, "real")
-    x, ids, weights, _ = _call(dev, 60, 2, 4, 512)
-    y = layer(x, ids, weights)
-    wild = x.clone()
-    wild[5] = math.inf
-    wild[17, 3] = math.nan
-    z = layer(wild, ids, weights)
-    same = torch.ones(60, dtype=torch.bool)
-    same[[5, 17]] = False
-    assert torch.equal(z[same], y[same]) and bool(z[17].isnan().all())
-    order = torch.randperm(60, generator=torch.Generator().manual_seed(2)).to(dev)
-    assert torch.equal(layer(x[order], ids[order], weights[order]), y[order])
+    for tokens in (20, 60):
+        x, ids, weights, _ = _call(dev, tokens, 2, 4, 512)
+        y = layer(x, ids, weights)
+        wild = x.clone()
+        wild[5] = math.inf
+        wild[17, 3] = math.nan
+        z = layer(wild, ids, weights)
+        same = torch.ones(tokens, dtype=torch.bool)
+        same[[5, 17]] = False
+        assert torch.equal(z[same], y[same]) and bool(z[17].isnan().all())
+        order = torch.randperm(tokens, generator=torch.Generator().manual_seed(2)).to(dev)
+        assert torch.equal(layer(x[order], ids[order], weights[order]), y[order])
 
 
-def test_experts_of_views(dev):
+@pytest.mark.parametrize("tokens", [24, 64])
+def test_experts_of_views(dev, tokens):
     layer, _ = _layer(dev, 4, 264, 64, "t")
-    x, ids, weights, residual = _call(dev, 24, 2, 4, 264, residual=True)
+    x, ids, weights, residual = _call(dev, tokens, 2, 4, 264, residual=True)
     want = layer(x, ids, weights, residual)
-    apart = torch.zeros(24, 400, dtype=torch.bfloat16, device=dev)
+    apart = torch.zeros(tokens, 400, dtype=torch.bfloat16, device=dev)
     for start in (0, 1, 3):
         view = apart[:, start:start + 264]
         view.copy_(x)
         assert torch.equal(layer(view, ids, weights, residual), want)
         assert torch.equal(layer(x, ids, weights, view.copy_(residual)), want)
     assert torch.equal(layer(x.t().contiguous().t(), ids.t().contiguous().t(), weights.t().contiguous().t(), residual), want)
-    deep = layer(x.view(2, 12, 264), ids.view(2, 12, 2), weights.view(2, 12, 2), residual.view(2, 12, 264))
-    assert deep.shape == (2, 12, 264) and torch.equal(deep.view(24, 264), want)
+    deep = layer(x.view(2, -1, 264), ids.view(2, -1, 2), weights.view(2, -1, 2), residual.view(2, -1, 264))
+    assert deep.shape == (2, tokens // 2, 264) and torch.equal(deep.view(tokens, 264), want)
     assert layer(x[:0], ids[:0], weights[:0]).shape == (0, 264)
     # weights of another type are taken as they are
     assert torch.equal(layer(x, ids, weights.bfloat16()), layer(x, ids, weights.bfloat16().float()))
@@ -255,7 +269,7 @@ def test_experts_state(dev):
     assert torch.equal(other(x, ids, weights), layer(x, ids, weights))
 
 
-@pytest.mark.parametrize("tokens", [1, 33])
+@pytest.mark.parametrize("tokens", [1, 33, 200])
 def test_experts_from_a_graph_and_another_stream(dev, tokens):
     from ixrun_amd import route_experts
 
