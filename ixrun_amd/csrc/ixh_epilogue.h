@@ -4,12 +4,19 @@
 
 namespace ixh {
 
+// e^v, within 2 |v| + 2 steps of fp32, and a quotient within 2: they stand in a factor between 0 and 1 of what is rounded to 8 bits.
+// (expf and the division of IEEE 754 take 40 instructions an activation against 6: half of the time that k_experts_prompt spent behind its
+// products.)
+__device__ __forceinline__ float ep_exp(float v) { return __builtin_amdgcn_exp2f(v * 1.44269504088896341f); }
+__device__ __forceinline__ float ep_ratio(float a, float b) { return a * __builtin_amdgcn_rcpf(b); }
+
 // The sum's activation.  Where exp overflows the quotient is the limit, 0 (of -infinity itself NaN, as infinity times 0 is).
+// 0.5 (1 + tanh(t)) is 1 / (1 + e^(-2 t)).
 __device__ __forceinline__ float ep_activation(int act, float v) {
     switch (act) {
-        case IXH_ACT_SILU: return v / (1.0f + expf(-v));
+        case IXH_ACT_SILU: return ep_ratio(v, 1.0f + ep_exp(-v));
         case IXH_ACT_GELU: return 0.5f * v * (1.0f + erff(v * 0.70710678118654752f));
-        case IXH_ACT_GELU_TANH: return 0.5f * v * (1.0f + tanhf(0.79788456080286536f * (v + 0.044715f * v * v * v)));
+        case IXH_ACT_GELU_TANH: return ep_ratio(v, 1.0f + ep_exp(-1.5957691216057308f * (v + 0.044715f * v * v * v)));
         case IXH_ACT_RELU: return v < 0.0f ? 0.0f : v;
         case IXH_ACT_RELU2: v = v < 0.0f ? 0.0f : v; return v * v;
         default: return v;

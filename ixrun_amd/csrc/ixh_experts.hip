@@ -20,11 +20,26 @@ constexpr uint32_t kExPlanThreads = 1024, kExPlanWaves = kExPlanThreads / kWave;
 // allow (what is left of an eighth is as long as the whole).
 __device__ __forceinline__ uint32_t ex_eights(uint32_t n) { return (n + 127u) / 128u; }
 __device__ __forceinline__ uint32_t ex_tiles(uint32_t n, uint32_t rows) { return rows ? (n + rows - 1u) / rows : (ex_eights(n) + 3u) / 4u; }
+// How many of these are of 4, 3, 2 and 1 eights of blocks: the order of the tiles, so that the last ones to be taken are short.  (Tiles of
+// `rows` slots are in the order of the experts.)
+constexpr uint32_t kExSizes = 4;
+struct ExSizes { uint32_t n[kExSizes]; };
+__device__ __forceinline__ ExSizes ex_sizes(uint32_t n, uint32_t rows) {
+    ExSizes of{};
+    if (rows) {
+        of.n[0] = ex_tiles(n, rows);
+    } else if (n) {
+        const uint32_t tiles = ex_tiles(n, 0), each = ex_eights(n) / tiles, longer = ex_eights(n) - each * tiles;
+#pragma unroll
+        for (uint32_t k = 0; k < kExSizes; ++k) of.n[k] = each == 4u - k ? tiles - longer : each + 1u == 4u - k ? longer : 0u;
+    }
+    return of;
+}
 __device__ __forceinline__ uint32_t ex_places(uint32_t n, uint32_t rows) { return rows ? n : (n + 15u) & ~15u; }
 
 __global__ void __launch_bounds__(kExPlanThreads)
 k_experts_plan(const int32_t *__restrict__ ids, uint32_t slots, uint32_t experts, uint32_t rows, ExPlan plan) {
-    __shared__ uint32_t hist[kExMostExperts], of_wave[kExPlanWaves], sums[2][kExPlanWaves];
+    __shared__ uint32_t hist[kExMostExperts], of_wave[kExPlanWaves], sums[1u + kExSizes][kExPlanWaves];
     const uint32_t tid = threadIdx.x, lane = tid & 63u, wave = tid >> 6, e = blockIdx.x;
     for (uint32_t i = tid; i < experts; i += kExPlanThreads) hist[i] = 0;
     __syncthreads();
@@ -39,26 +54,51 @@ k_experts_plan(const int32_t *__restrict__ ids, uint32_t slots, uint32_t experts
     for (int by = 32; by; by >>= 1) mine += __shfl_xor(mine, by);
     if (lane == 0) of_wave[wave] = mine;
     __syncthreads();
-    uint32_t before = 0, tiles_before = 0;
-    for (uint32_t i = tid; i < e; i += kExPlanThreads) before += ex_places(hist[i], rows), tiles_before += ex_tiles(hist[i], rows);
-    for (int by = 32; by; by >>= 1) before += __shfl_xor(before, by), tiles_before += __shfl_xor(tiles_before, by);
-    if (lane == 0) sums[0][wave] = before, sums[1][wave] = tiles_before;
+    // in front of this expert: places, and, of each size, tiles; with them all tiles of larger sizes
+    uint32_t sum[1u + kExSizes] = {};
+    for (uint32_t i = tid; i < experts; i += kExPlanThreads) {
+        const ExSizes of = ex_sizes(hist[i], rows);
+        if (i < e) sum[0] += ex_places(hist[i], rows);
+#pragma unroll
+        for (uint32_t k = 0; k < kExSizes; ++k) {
+            uint32_t larger = 0;
+#pragma unroll
+            for (uint32_t l = 0; l < k; ++l) larger += of.n[l];
+            sum[1u + k] += larger + (i < e ? of.n[k] : 0u);
+        }
+    }
+#pragma unroll
+    for (uint32_t k = 0; k <= kExSizes; ++k) {
+        for (int by = 32; by; by >>= 1) sum[k] += __shfl_xor(sum[k], by);
+        if (lane == 0) sums[k][wave] = sum[k];
+    }
     __syncthreads();
-    before = tiles_before = 0;
-    for (uint32_t w = 0; w < kExPlanWaves; ++w) before += sums[0][w], tiles_before += sums[1][w];
-    const uint32_t n = hist[e], n_tiles = ex_tiles(n, rows), places = ex_places(n, rows);
+#pragma unroll
+    for (uint32_t k = 0; k <= kExSizes; ++k) {
+        sum[k] = 0;
+        for (uint32_t w = 0; w < kExPlanWaves; ++w) sum[k] += sums[k][w];
+    }
+    const uint32_t before = sum[0], n = hist[e], n_tiles = ex_tiles(n, rows), places = ex_places(n, rows);
+    const ExSizes own_sizes = ex_sizes(n, rows);
     for (uint32_t i = tid; i < n_tiles; i += kExPlanThreads) {
-        uint32_t *const t = plan.tiles + 3u * (tiles_before + i);
-        t[0] = e;
         if (rows) {
-            t[1] = before + i * rows, t[2] = min(rows, n - i * rows);
-        } else {
-            const uint32_t eights = ex_eights(n), b0 = eights * i / n_tiles * 8u, b1 = min(eights * (i + 1u) / n_tiles * 8u, places / 16u);
-            t[1] = before / 16u + b0, t[2] = b1 - b0;
+            uint32_t *const t = plan.tiles + 3u * (sum[1] + i);
+            t[0] = e, t[1] = before + i * rows, t[2] = min(rows, n - i * rows);
+        } else {  // the longer ones of an expert's tiles come first
+            const uint32_t eights = ex_eights(n), each = eights / n_tiles, longer = eights - each * n_tiles;
+            const uint32_t b0 = (i * each + min(i, longer)) * 8u, size = each + (i < longer);
+            uint32_t at = i < longer ? i : i - longer;
+#pragma unroll
+            for (uint32_t k = 0; k < kExSizes; ++k) at += size == 4u - k ? sum[1u + k] : 0u;
+            uint32_t *const t = plan.tiles + 3u * at;
+            t[0] = e, t[1] = before / 16u + b0, t[2] = min(size * 8u, places / 16u - b0);
         }
     }
     for (uint32_t i = n + tid; i < places; i += kExPlanThreads) plan.order[before + i] = ~0u;
-    if (e + 1u == experts && tid == 0) *plan.n_tiles = tiles_before + n_tiles, *plan.n_blocks = (before + places) / 16u;
+    if (e + 1u == experts && tid == 0) {
+        *plan.n_tiles = rows ? sum[1] + n_tiles : sum[kExSizes] + own_sizes.n[kExSizes - 1u];  // (in front of this one: all larger ones, and all others')
+        *plan.n_blocks = (before + places) / 16u;
+    }
     uint32_t at = before;
     for (uint32_t w = 0; w < wave; ++w) at += of_wave[w];
     for (uint32_t i0 = from; i0 < to; i0 += kWave) {

@@ -37,7 +37,7 @@ __device__ __forceinline__ void ep_tile(const ExMatrix &W, const EpCall &R, uint
                                         uint8_t *ep_smem) {
     using P = LnPairs<BITS, true>;
     constexpr uint32_t NI = 8;
-    constexpr uint32_t AHEAD = 2;  // steps of 32 columns that the activations' operands are asked for ahead
+    constexpr uint32_t AHEAD = MI == 2 ? 8 : MI == 3 ? 4 : 2;  // steps of 32 columns that the activations' operands are asked for ahead
     constexpr uint32_t CODES = MI == 4 ? 1 : 2;  // stages that the codes are asked for ahead of their decode
     constexpr bool FLOAT = MI != 4;
     const uint32_t smem = (uint32_t)(uintptr_t)(LN_LDS(uint8_t) *)ep_smem;
@@ -345,9 +345,17 @@ __device__ __forceinline__ void ep_tile(const ExMatrix &W, const EpCall &R, uint
 #pragma unroll
             for (uint32_t b = 0; b < NI; ++b) {
                 const uint32_t col = (tile * NI + b) * 16u + 4u * kg;
+                ln_f32x4 v = acc[i][b];
+                if (bias)
 #pragma unroll
-                for (uint32_t k = 0; k < 4; ++k)
-                    if (col + k < W.outputs) to[col + k] = acc[i][b][k] + (bias ? bf16_bits_to_f32(bias[col + k]) : 0.0f);
+                    for (uint32_t k = 0; k < 4; ++k) v[k] += bf16_bits_to_f32(bias[min(col + k, W.outputs - 1u)]);
+                if (W.outputs % 4u == 0) {  // (rows of whole 16 bytes)
+                    if (col < W.outputs) *reinterpret_cast<ln_f32x4 *>(to + col) = v;
+                } else {
+#pragma unroll
+                    for (uint32_t k = 0; k < 4; ++k)
+                        if (col + k < W.outputs) to[col + k] = v[k];
+                }
             }
         }
     }
