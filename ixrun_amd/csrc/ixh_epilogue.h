@@ -22,6 +22,21 @@ __device__ __forceinline__ float ep_activation(int act, float v) {
         default: return v;
     }
 }
+// four sums', one way for all
+template <class V> __device__ __forceinline__ void ep_activations(int act, V &v) {
+    switch (act) {
+#define EP_EACH(A)                                            \
+    case A:                                                   \
+        for (int k = 0; k < 4; ++k) v[k] = ep_activation(A, v[k]); \
+        break;
+        EP_EACH(IXH_ACT_SILU)
+        EP_EACH(IXH_ACT_GELU)
+        EP_EACH(IXH_ACT_GELU_TANH)
+        EP_EACH(IXH_ACT_RELU)
+        EP_EACH(IXH_ACT_RELU2)
+#undef EP_EACH
+    }
+}
 inline bool ep_known(int act) { return act >= IXH_ACT_NONE && act <= IXH_ACT_RELU2; }
 
 // round-to-nearest-even, NaN stays NaN whatever its bits

@@ -45,11 +45,18 @@ k_experts_plan(const int32_t *__restrict__ ids, uint32_t slots, uint32_t experts
     __syncthreads();
     // a wave has whole 64 slots one after another
     const uint32_t share = ((slots + kExPlanThreads - 1u) / kExPlanThreads) * kWave, from = min(wave * share, slots), to = min(from + share, slots);
+    constexpr uint32_t N = 8;  // ids of a lane in flight
     uint32_t mine = 0;
-    for (uint32_t i = from + lane; i < to; i += kWave) {
-        const uint32_t id = (uint32_t)ids[i];
-        if (id < experts) atomicAdd(hist + id, 1u);
-        mine += id == e;
+    for (uint32_t i0 = from; i0 < to; i0 += N * kWave) {
+        uint32_t id[N];
+#pragma unroll
+        for (uint32_t k = 0; k < N; ++k) id[k] = (uint32_t)ids[min(i0 + k * kWave + lane, to - 1u)];
+#pragma unroll
+        for (uint32_t k = 0; k < N; ++k) {
+            if (i0 + k * kWave + lane >= to) id[k] = ~0u;
+            if (id[k] < experts) atomicAdd(hist + id[k], 1u);
+            mine += id[k] == e;
+        }
     }
     for (int by = 32; by; by >>= 1) mine += __shfl_xor(mine, by);
     if (lane == 0) of_wave[wave] = mine;
@@ -101,12 +108,18 @@ k_experts_plan(const int32_t *__restrict__ ids, uint32_t slots, uint32_t experts
     }
     uint32_t at = before;
     for (uint32_t w = 0; w < wave; ++w) at += of_wave[w];
-    for (uint32_t i0 = from; i0 < to; i0 += kWave) {
-        const uint32_t i = i0 + lane;
-        const bool own = i < to && (uint32_t)ids[i] == e;
-        const uint64_t all = __ballot(own);
-        if (own) plan.order[at + lanes_below(all)] = i;
-        at += (uint32_t)__popcll(all);
+    for (uint32_t i0 = from; i0 < to; i0 += N * kWave) {
+        uint32_t id[N];
+#pragma unroll
+        for (uint32_t k = 0; k < N; ++k) id[k] = (uint32_t)ids[min(i0 + k * kWave + lane, to - 1u)];
+#pragma unroll
+        for (uint32_t k = 0; k < N; ++k) {
+            const uint32_t i = i0 + k * kWave + lane;
+            const bool own = i < to && id[k] == e;
+            const uint64_t all = __ballot(own);
+            if (own) plan.order[at + lanes_below(all)] = i;
+            at += (uint32_t)__popcll(all);
+        }
     }
 }
 
@@ -367,18 +380,33 @@ k_experts_rows(ExMatrix W, ExRows R) {
     }
 }
 
-// y[t] = residual[t] + sum_j weights[t, j] * (what its expert made of it), in the order of j
+// y[t] = residual[t] + sum_j weights[t, j] * (what its expert made of it), in the order of j.  Bound: memory.  N columns a thread.
+template <int N>
 __global__ void __launch_bounds__(256)
 k_experts_join(const float *__restrict__ per_slot, ExCall call, uint32_t experts, uint32_t hidden) {
-    const uint32_t t = blockIdx.x, at = blockIdx.y * 256u + threadIdx.x;
+    const uint32_t t = blockIdx.x, at = (blockIdx.y * 256u + threadIdx.x) * N;
     if (at >= hidden) return;
-    float v = 0.0f;
+    typedef float Sums __attribute__((ext_vector_type(4)));
+    float v[N] = {};
+    const int32_t *const ids = call.ids + (size_t)t * call.top_k;
+    const float *const weights = call.weights + (size_t)t * call.top_k;
+    const float *const from = per_slot + (size_t)t * call.top_k * hidden + at;
+#pragma unroll 4
     for (uint32_t j = 0; j < call.top_k; ++j) {
-        const size_t slot = (size_t)t * call.top_k + j;
-        if ((uint32_t)call.ids[slot] < experts) v = __fmaf_rn(call.weights[slot], per_slot[slot * hidden + at], v);
+        if ((uint32_t)ids[j] >= experts) continue;
+        const float w = weights[j];
+        if constexpr (N == 4) {
+            const Sums p = *reinterpret_cast<const Sums *>(from + (size_t)j * hidden);
+#pragma unroll
+            for (int k = 0; k < 4; ++k) v[k] = __fmaf_rn(w, p[k], v[k]);
+        } else {
+            v[0] = __fmaf_rn(w, from[(size_t)j * hidden], v[0]);
+        }
     }
-    if (call.residual) v += bf16_bits_to_f32(call.residual[(int64_t)t * call.ld_residual + at]);
-    call.y[(int64_t)t * call.ldy + at] = ep_bf16(v);
+    uint16_t *const y = call.y + (int64_t)t * call.ldy + at;
+    const uint16_t *const residual = call.residual + (int64_t)t * call.ld_residual + at;
+#pragma unroll
+    for (int k = 0; k < N; ++k) y[k] = ep_bf16(call.residual ? v[k] + bf16_bits_to_f32(residual[k]) : v[k]);
 }
 
 // ---- host ----
@@ -506,7 +534,10 @@ int launch_experts(const ExDev &X, const ExCall &call, void *workspace, hipStrea
         rc = ex_matrix<false>(X.second, R, planned ? w.rows : 1u, n_tiles, s);
     }
     if (rc != IXH_OK) return rc;
-    IXH_LAUNCH(k_experts_join, dim3(call.tokens, (X.hidden + 255u) / 256u), dim3(256), 0, s, per_slot, call, X.experts, X.hidden);
+    if (X.hidden % 4u == 0)
+        IXH_LAUNCH(k_experts_join<4>, dim3(call.tokens, (X.hidden / 4u + 255u) / 256u), dim3(256), 0, s, per_slot, call, X.experts, X.hidden);
+    else
+        IXH_LAUNCH(k_experts_join<1>, dim3(call.tokens, (X.hidden + 255u) / 256u), dim3(256), 0, s, per_slot, call, X.experts, X.hidden);
     return hipGetLastError() == hipSuccess ? IXH_OK : IXH_ELAUNCH;
 }
 
