@@ -124,15 +124,19 @@ k_experts_plan(const int32_t *__restrict__ ids, uint32_t slots, uint32_t experts
 }
 
 // ---------------------------------------------------------------------------------------------------------------
-// k_experts_rows<BITS, MT, FIRST>: a tile of up to MT slots of one expert by a run of blocks of 16 weight rows.
+// k_experts_rows<BITS, MT, WIDE, FIRST>: tiles of up to MT slots of one expert.
 //
 // As in k_lanes_rows a lane's decoded weights are its operand of v_mfma_f32_16x16x32_bf16 as they are, the activations of the tile lie in
 // LDS a column's rows together (transposing reads make them the other operand), and listed elements are multiplied in fp32 by the lane of
-// their row.  A wave has whole cells of 512 columns of a block, and with a cell its list.  Rows longer than LDS holds are taken in
-// chunks of cells; the sums stay in LDS over them.  FIRST: the rows are gathered from the tokens, and the epilogue is the bias, the
-// activation and, gated, the product of the two halves; else they are those of the intermediate and the sums go out in fp32.
+// their row.  FIRST: the rows are gathered from the tokens, and the epilogue is the bias, the activation and, gated, the product of the two
+// halves; else they are those of the intermediate and the sums go out in fp32.
+//
+// How many tiles there are is known on the device only.  All of them are one list of items (16 weight rows of a tile, or a pair of blocks),
+// of which each workgroup, one a CU, has an equal run: its parts of one tile after another.  Of such a part the cells (16 rows x 512
+// columns) are dealt to the waves in equal runs as well; what a wave has of a block goes to LDS, and the epilogue adds the waves' parts in
+// the columns' order.  Rows longer than LDS holds are taken in chunks of cells, whose sums are added there.
 // ---------------------------------------------------------------------------------------------------------------
-constexpr uint32_t kExWaves = 8, kExThreads = kExWaves * kWave;
+constexpr uint32_t kExWaves = 16, kExThreads = kExWaves * kWave;
 
 struct ExRows {
     const uint16_t *x;
@@ -141,241 +145,307 @@ struct ExRows {
     const uint32_t *n_tiles, *tiles, *order;  // n_tiles NULL: a tile is a slot
     void *out;
     int64_t ld_out;
-    uint32_t experts, top_k, n_blocks, all_blocks, waves_along, chunk_cells;  // waves along the columns
+    uint32_t experts, top_k, slots;
+    uint32_t per_tile, most_blocks, chunk_cells;  // items of a tile; blocks that LDS has room for; cells of a chunk
+    uint32_t of_tile;                             // workgroups of each tile, or 0: of all of them
     int activation;
     bool gated, pairs;
 };
 
-template <int BITS> constexpr uint32_t kExXAt = (LnPairs<BITS, BITS == 4>::kLutBytes + 4095u) & ~4095u;
+template <int BITS, bool WIDE> constexpr uint32_t kExXAt = (LnPairs<BITS, WIDE>::kLutBytes + 4095u) & ~4095u;
 
-template <int BITS, int MT, bool FIRST>
-__global__ void __launch_bounds__(kExThreads) __attribute__((amdgpu_waves_per_eu(4)))
+template <int BITS, int MT, bool WIDE, bool FIRST>
+__global__ void __launch_bounds__(kExThreads)
 k_experts_rows(ExMatrix W, ExRows R) {
     extern __shared__ __attribute__((aligned(16))) uint8_t ex_smem[];
-    using P = LnPairs<BITS, BITS == 4>;
-    constexpr bool WIDE = BITS == 4;
-    constexpr uint32_t ROW = 2u * MT;
+    using P = LnPairs<BITS, WIDE>;
+    constexpr uint32_t ROW = 2u * MT, PART = 16u * MT;
+    constexpr uint32_t kZeros = MT == 1 ? 64u : 256u;  // bytes behind the activations
     const uint32_t smem = (uint32_t)(uintptr_t)(LN_LDS(uint8_t) *)ex_smem;
     const uint32_t tid = threadIdx.x, lane = tid & 63u, n = lane & 15u, kg = lane >> 4;
     const uint32_t wave = (uint32_t)__builtin_amdgcn_readfirstlane((int)(tid >> 6));
-
-    // ---- the tile ----
-    uint32_t e, first = blockIdx.x, count = 1;
-    if (R.n_tiles) {
-        const uint32_t *const t = R.tiles + 3u * blockIdx.x;
-        e = t[0], first = t[1], count = t[2];
-        if (blockIdx.x >= *R.n_tiles) return;
-    } else {
-        e = (uint32_t)R.ids[blockIdx.x];
-        if (e >= R.experts) return;
-    }
-    const uint32_t slot = R.n_tiles ? R.order[first + min(lane, count - 1u)] : first;  // of the tile's row `lane`
-    const int64_t x_row = (int64_t)(FIRST ? slot / R.top_k : first + min(lane, count - 1u)) * R.ldx;
-    const uint32_t b0 = blockIdx.y * R.n_blocks, n_blocks = min(R.n_blocks, R.all_blocks - b0);
-
-    const uint32_t C = W.n_cells;
-    const uint8_t *const plane = reinterpret_cast<const uint8_t *>(W.plane + (size_t)e * W.plane_words);
-    const uint32_t *const exc_off = W.exc_off + (size_t)e * (W.n_tiles * C + 1u);
-    const float scale = bf16_bits_to_f32(W.scale[e]);
-    const uint32_t x_at = smem + kExXAt<BITS>, x_none = R.chunk_cells * kLnCols * ROW;
-    float *const parts = reinterpret_cast<float *>(ex_smem + kExXAt<BITS> + x_none + 16u * ROW);  // [wave along][block][16][MT]
-    constexpr uint32_t PART = 16u * MT;
-
-    ln_build_lut<BITS, WIDE>(smem, scale, tid, kExThreads);
-    for (uint32_t i = tid; i < R.waves_along * R.n_blocks * PART; i += kExThreads) parts[i] = 0.0f;
-    if (tid < 16u) *reinterpret_cast<LN_LDS(ln_u32x4) *>((uintptr_t)(x_at + x_none + tid * 16u)) = ln_u32x4{0, 0, 0, 0};
-
+    const uint32_t C = W.n_cells, per = FIRST && R.gated ? 2u : 1u;  // blocks of an item
+    const uint32_t x_at = smem + kExXAt<BITS, WIDE>, x_none = R.chunk_cells * kLnCols * ROW;
+    float *const parts = reinterpret_cast<float *>(ex_smem + kExXAt<BITS, WIDE> + x_none + kZeros);  // [wave + block][16][MT]
+    float *const totals = parts + (kExWaves + R.most_blocks) * PART;  // [block][16][MT], with several chunks
     const uint32_t lut_lane = smem + ((lane & ((1u << P::kCopies) - 1u)) << 2);
+    // Where the lane's operands begin in the activations: of sixteen lanes pieces of four columns (of all rows), at 16 rows in a place of
+    // their own for the second four; of one row the lane's eight columns.  The blocks of 32 columns are added as constants.
     const uint32_t piece = MT == 16 ? n & 3u : n & 1u;
-    const uint32_t x_mine = (x_at + lr_place<MT>((8u * kg + (n >> 2)) * ROW)) ^ (piece * 8u);
-    const uint32_t scale_bits = __float_as_uint(scale) & 0x7FFFFFFFu;
-    const uint32_t wc = wave % R.waves_along, wb = wave / R.waves_along, waves_across = kExWaves / R.waves_along;
-    const uint32_t my_blocks = n_blocks > wb ? (n_blocks - wb + waves_across - 1u) / waves_across : 0u;
+    const uint32_t x_mine = MT == 1 ? x_at + kg * 16u : (x_at + lr_place<MT>((8u * kg + (n >> 2)) * ROW)) ^ (piece * 8u);
+    const uint32_t x_other = MT == 16 ? x_mine ^ (4u * ROW) : x_mine + 4u * ROW;
 
-    for (uint32_t c0 = 0; c0 < C; c0 += R.chunk_cells) {
-        const uint32_t cells = min(R.chunk_cells, C - c0);
-        if (c0) __syncthreads();  // the last chunk's activations are in use until here
-        // ---- activations: a pair of columns a lane, all rows ----
-        for (uint32_t task = wave; task < 4u * cells; task += kExWaves) {
-            const uint32_t col = c0 * kLnCols + task * 128u + 2u * lane;
-            uint32_t v[MT];
-#pragma unroll
-            for (uint32_t k = 0; k < MT; ++k) {
-                v[k] = 0;
-                if (k < count) {
-                    const uint16_t *const row = R.x + (((int64_t)__builtin_amdgcn_readlane((int)(x_row >> 32), (int)k) << 32) |
-                                                       (uint32_t)__builtin_amdgcn_readlane((int)x_row, (int)k));
-                    if (R.pairs) {
-                        if (col < W.in_f) v[k] = *reinterpret_cast<const uint32_t *>(row + col);
-                    } else {
-                        if (col < W.in_f) v[k] = row[col];
-                        if (col + 1u < W.in_f) v[k] |= (uint32_t)row[col + 1u] << 16;
-                    }
-                }
-            }
-            const uint32_t to = lane_offset(task * 128u + 2u * lane) * MT;
-#pragma unroll
-            for (uint32_t j = 0; j < 2; ++j)
-#pragma unroll
-                for (uint32_t h = 0; h < MT / 8u; ++h) {
-                    ln_u32x4 o;
-#pragma unroll
-                    for (uint32_t k = 0; k < 4; ++k)
-                        o[k] = __builtin_amdgcn_perm(v[8 * h + 2 * k + 1], v[8 * h + 2 * k], j ? 0x07060302u : 0x05040100u);
-                    *reinterpret_cast<LN_LDS(ln_u32x4) *>((uintptr_t)(x_at + (lr_place<MT>(to + j * ROW) ^ (h * 16u)))) = o;
-                }
+    // (below 2^30 items: fewer than 16 slots an expert)
+    const uint32_t all_items = (R.n_tiles ? *R.n_tiles : R.slots) * R.per_tile;
+    uint32_t item, item_end;
+    if (R.of_tile) {
+        const uint32_t tile = blockIdx.x / R.of_tile, part = blockIdx.x - tile * R.of_tile;
+        item = tile * R.per_tile + part * R.per_tile / R.of_tile, item_end = min(tile * R.per_tile + (part + 1u) * R.per_tile / R.of_tile, all_items);
+    } else {
+        const uint32_t share = all_items / gridDim.x, more = all_items - share * gridDim.x;
+        item = blockIdx.x * share + min(blockIdx.x, more), item_end = item + share + (blockIdx.x < more);
+    }
+    uint32_t staged = ~0u, e_table = ~0u;  // the tile whose activations are in LDS, the expert whose pairs are
+    for (uint32_t blocks; item < item_end; item += blocks / per) {
+        const uint32_t tile = item / R.per_tile, b0 = (item - tile * R.per_tile) * per;
+        blocks = min(min(R.per_tile * per - b0, R.most_blocks), (item_end - item) * per);
+        // ---- the tile ----
+        uint32_t e, first = tile, count = 1;
+        if (R.n_tiles) {
+            const uint32_t *const t = R.tiles + 3u * tile;
+            e = t[0], first = t[1], count = t[2];
+        } else {
+            e = (uint32_t)R.ids[tile];
+            if (e >= R.experts) continue;
         }
-        __syncthreads();
+        const uint32_t slot = R.n_tiles ? R.order[first + min(lane, count - 1u)] : first;  // of the tile's row `lane`
+        const int64_t x_row = (int64_t)(FIRST ? slot / R.top_k : first + min(lane, count - 1u)) * R.ldx;
+        const __amdgpu_buffer_rsrc_t codes_rs = __builtin_amdgcn_make_buffer_rsrc((void *)(W.plane + (size_t)e * W.plane_words), 0, -1, 0x00020000);
+        const uint32_t *const exc_off = W.exc_off + (size_t)e * (W.n_tiles * C + 1u);
+        const uint32_t scale_raw = W.scale[e];
 
-        // ---- this wave's cells: those of its share of the chunk, block after block ----
-        const uint32_t c_lo = cells * wc / R.waves_along, c_n = cells * (wc + 1u) / R.waves_along - c_lo;
-        const uint32_t units = my_blocks * c_n;
-        if (units == 0) continue;
-        struct Cursor { uint32_t j, c; };  // its j-th block, cell c of its share
-        auto after = [&](const Cursor &k) { return k.c + 1u < c_n ? Cursor{k.j, k.c + 1u} : k.j + 1u < my_blocks ? Cursor{k.j + 1u, 0u} : k; };
-        auto quad = [&](const Cursor &k, uint32_t q) { return 4u * (b0 + wb + k.j * waves_across) + q; };
-        uint32_t w[2][BITS];
-        auto load = [&](const Cursor &k, uint32_t half) {
-            const uint32_t t = min(quad(k, n >> 2), W.n_tiles - 1u);
-            const uint8_t *const cell = plane + (size_t)(t * C + c0 + c_lo + k.c) * (256u * BITS);
+        for (uint32_t c0 = 0; c0 < C; c0 += R.chunk_cells) {
+            const uint32_t cells = min(R.chunk_cells, C - c0), units = blocks * cells;
+            const uint32_t u0 = wave * units / kExWaves, u1 = (wave + 1u) * units / kExWaves;
+            // ---- what depends on nothing that LDS holds is asked for ----
+            // (requests past the last cell of the share are for that one again)
+            struct Cursor { uint32_t b, c; };  // a block of the part, a cell of the chunk
+            const uint32_t last_unit = u1 ? u1 - 1u : 0u, b_last = last_unit / cells, c_last = last_unit - b_last * cells;
+            auto after = [&](const Cursor &k) {
+                if (k.b == b_last && k.c == c_last) return k;
+                return k.c + 1u < cells ? Cursor{k.b, k.c + 1u} : Cursor{k.b + 1u, 0u};
+            };
+            // bytes of the lane's codes, and places of its quad's cell, of a block in front of its cells (below 2^31)
+            constexpr uint32_t kCell = 256u * BITS, kLane = BITS == 3 ? 12u : 16u;
+            const uint32_t in_cell = 4u * kg + (n & 3u);
+            auto codes_of = [&](uint32_t block) { return (min(4u * (b0 + block) + (n >> 2), W.n_tiles - 1u) * C + c0) * kCell + in_cell * kLane; };
+            auto cells_of = [&](uint32_t block) { return min(4u * (b0 + block) + kg, W.n_tiles - 1u) * C + c0; };
+            uint32_t w[2][2][BITS];  // the halves of a cell: each is asked for again, for the next cell, as soon as it is decoded
+            auto load = [&](uint32_t codes, uint32_t c, uint32_t half) {
 #pragma unroll
-            for (uint32_t j = 0; j < 2; ++j)
-                ln_load_lane<BITS>(reinterpret_cast<const uint32_t *>(cell), 32u * half + 16u * j + 4u * kg + (n & 3u), w[j]);
-        };
-        struct Extent { uint32_t first, end; };
-        auto extent = [&](const Cursor &k) {
-            const uint32_t t = quad(k, kg), cell = min(t, W.n_tiles - 1u) * C + c0 + c_lo + k.c;
-            const uint32_t a = exc_off[cell], b = exc_off[cell + 1u];
-            return Extent{a, t < W.n_tiles ? b : a};
-        };
-        struct Group { ln_u32x2 pos; uint32_t val; };
-        auto quad_of = [&](const Extent &x, uint32_t i) { return (x.first & ~3u) + 16u * i + (n & ~3u); };
-        auto g_load = [&](const Extent &x, uint32_t i) {
-            const uint32_t q = quad_of(x, i), at = q < x.end ? lane_listed(q, n & 3u) : 0u;
-            return Group{*reinterpret_cast<const ln_u32x2 *>(W.exc_pos + at), *reinterpret_cast<const uint32_t *>(W.exc_val + at)};
-        };
-        auto groups_of = [&](const Extent &x) {  // of the row quad that has most
-            const int g = (int)(x.end > x.first ? (x.end - (x.first & ~3u) + 15u) / 16u : 0u);
-            return (uint32_t)max(max(__builtin_amdgcn_readlane(g, 0), __builtin_amdgcn_readlane(g, 16)),
-                                 max(__builtin_amdgcn_readlane(g, 32), __builtin_amdgcn_readlane(g, 48)));
-        };
-        Cursor now{0u, 0u}, next = after(now);
-        load(now, 0);
-        Extent e_now = extent(now), e_next = extent(next);
-        Group list[2];
-#pragma unroll
-        for (uint32_t i = 0; i < 2; ++i) list[i] = g_load(e_now, i);
-        ln_f32x4 acc = {0, 0, 0, 0};
-        float ex[MT];
-#pragma unroll
-        for (int r = 0; r < MT; ++r) ex[r] = 0.0f;
-        const uint32_t c_seg = c0 * 1024u;
-        auto listed = [&](const Group &g, const Extent &x, uint32_t i) {
-            const uint32_t q = quad_of(x, i);
-            uint32_t at[4];
-#pragma unroll
-            for (uint32_t k = 0; k < 4; ++k) {
-                const uint32_t p = ((g.pos[k >> 1] >> (16 * (k & 1))) - c_seg) & 0xFFFFu;
-                const bool is = q + k >= x.first && q + k < x.end && ((g.val >> (8 * k)) & 255u);
-                at[k] = is ? min(p * MT, x_none) : x_none;
-            }
-            const uint32_t w01 = ln_pack((float)(int)(int8_t)g.val * scale, (float)(int)(int8_t)(g.val >> 8) * scale);
-            const uint32_t w23 = ln_pack((float)(int)(int8_t)(g.val >> 16) * scale, (float)((int)g.val >> 24) * scale);
-#pragma unroll
-            for (uint32_t k = 0; k < 4; ++k) {
-                const uint32_t wk = k & 2 ? w23 : w01, wbits = k & 1 ? wk & 0xFFFF0000u : wk << 16;
-                const float wv = __uint_as_float(wbits) - __uint_as_float((wbits & 0x80000000u) | scale_bits);  // (no element: times 0)
-#pragma unroll
-                for (uint32_t h = 0; h < MT / 8u; ++h) {
-                    const ln_u32x4 v = *reinterpret_cast<const LN_LDS(ln_u32x4) *>((uintptr_t)(x_at + (lr_place<MT>(at[k]) ^ (h * 16u))));
-#pragma unroll
-                    for (uint32_t j = 0; j < 4; ++j) {
-                        ex[8 * h + 2 * j] = __fmaf_rn(wv, __uint_as_float(v[j] << 16), ex[8 * h + 2 * j]);
-                        ex[8 * h + 2 * j + 1] = __fmaf_rn(wv, __uint_as_float(v[j] & 0xFFFF0000u), ex[8 * h + 2 * j + 1]);
+                for (uint32_t j = 0; j < 2; ++j) {
+                    const uint32_t q = 2u * half + j, at = c * kCell;
+                    uint32_t(&d)[BITS] = w[half][j];
+                    if constexpr (BITS == 3) {
+                        const ln_u32x3 v = __builtin_bit_cast(ln_u32x3, __builtin_amdgcn_raw_buffer_load_b96(codes_rs, (int)(codes + q * 192u), (int)at, 0));
+                        d[0] = v[0]; d[1] = v[1]; d[2] = v[2];
+                    } else {
+                        const ln_u32x4 v = __builtin_bit_cast(ln_u32x4, __builtin_amdgcn_raw_buffer_load_b128(codes_rs, (int)(codes + q * 256u), (int)at, 0));
+                        d[0] = v[0]; d[1] = v[1]; d[2] = v[2]; d[3] = v[3];
+                        if constexpr (BITS == 5)
+                            d[4] = __builtin_amdgcn_raw_buffer_load_b32(codes_rs, (int)(codes - 12u * in_cell + (1024u + q * 64u)), (int)at, 0);
+                        if constexpr (BITS == 8) {
+                            const ln_u32x4 u = __builtin_bit_cast(ln_u32x4, __builtin_amdgcn_raw_buffer_load_b128(codes_rs, (int)(codes + (1024u + q * 256u)), (int)at, 0));
+                            d[4] = u[0]; d[5] = u[1]; d[6] = u[2]; d[7] = u[3];
+                        }
                     }
                 }
-            }
-        };
-#pragma unroll 1
-        for (uint32_t u = 0; u < units; ++u) {
-            const uint32_t x_cell = x_mine + (c_lo + now.c) * (512u * ROW);
+            };
+            struct Extent { uint32_t first, end; };
+            auto extent = [&](uint32_t from, const Cursor &k) {  // (behind the last row quad: the last one's, of which nothing is taken)
+                const uint32_t a = exc_off[from + k.c], b = exc_off[from + k.c + 1u];
+                return Extent{a, 4u * (b0 + k.b) + kg < W.n_tiles ? b : a};
+            };
+            struct Group { ln_u32x2 pos; uint32_t val; };
+            auto quad_of = [&](const Extent &x, uint32_t i) { return (x.first & ~3u) + 16u * i + (n & ~3u); };
+            auto g_load = [&](const Extent &x, uint32_t i) {
+                const uint32_t q = quad_of(x, i), at = q < x.end ? lane_listed(q, n & 3u) : 0u;
+                return Group{*reinterpret_cast<const ln_u32x2 *>(W.exc_pos + at), *reinterpret_cast<const uint32_t *>(W.exc_val + at)};
+            };
+            const uint32_t b_first = min(u0 / cells, blocks - 1u);  // (an empty share at the end)
+            Cursor now{b_first, min(u0 - b_first * cells, cells - 1u)}, next = after(now);
+            uint32_t codes = codes_of(now.b), places = cells_of(now.b);
+            load(codes, now.c, 0);
+            load(codes, now.c, 1);
+            Extent e_now = extent(places, now);
+            if (next.b != now.b) codes = codes_of(next.b), places = cells_of(next.b);  // of the cell that is asked for next
+            Extent e_next = extent(places, next);
+            const float scale = bf16_bits_to_f32(scale_raw);
+            const uint32_t scale_bits = __float_as_uint(scale) & 0x7FFFFFFFu;
+
+            if (staged != tile || cells != C) {
+                // ---- activations: a pair of columns a lane, all rows ----
+                for (uint32_t task = wave; task < 4u * cells; task += kExWaves) {
+                    const uint32_t col = c0 * kLnCols + task * 128u + 2u * lane;
+                    uint32_t v[MT];
 #pragma unroll
-            for (uint32_t half = 0; half < 2; ++half) {
-                uint32_t o[2][16];
-                ln_decode<BITS, WIDE>(w[0], lut_lane, scale, o[0]);
-                ln_decode<BITS, WIDE>(w[1], lut_lane, scale, o[1]);
-                load(half ? next : now, half ^ 1u);
-                // (columns 128 q + 32 i of a cell lie at 128 q + 32 (i ^ q))
-#pragma unroll
-                for (uint32_t j = 0; j < 2; ++j)
-#pragma unroll
-                    for (uint32_t i = 0; i < 4; ++i) {
-                        const uint32_t q = 2u * half + j, a = (x_cell + q * (128u * ROW)) ^ ((q ^ i) * (32u * ROW));
-                        const lr_bf16x4 lo = lr_turned(a), hi = lr_turned(MT == 16 ? a ^ (4u * ROW) : a + 4u * ROW);
-                        acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
-                            __builtin_bit_cast(ln_bf16x8, ln_u32x4{o[j][4 * i], o[j][4 * i + 1], o[j][4 * i + 2], o[j][4 * i + 3]}),
-                            __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7), acc, 0, 0, 0);
+                    for (uint32_t k = 0; k < MT; ++k) {
+                        v[k] = 0;
+                        if (k < count) {
+                            const uint16_t *const row = R.x + (((int64_t)__builtin_amdgcn_readlane((int)(x_row >> 32), (int)k) << 32) |
+                                                               (uint32_t)__builtin_amdgcn_readlane((int)x_row, (int)k));
+                            if (R.pairs) {
+                                if (col < W.in_f) v[k] = *reinterpret_cast<const uint32_t *>(row + col);
+                            } else {
+                                if (col < W.in_f) v[k] = row[col];
+                                if (col + 1u < W.in_f) v[k] |= (uint32_t)row[col + 1u] << 16;
+                            }
+                        }
                     }
-            }
-            const uint32_t groups = groups_of(e_now);
-            if (groups) listed(list[0], e_now, 0);
-            if (groups > 1u) listed(list[1], e_now, 1);
-#pragma unroll 1
-            for (uint32_t i = 2; i < groups; ++i) listed(g_load(e_now, i), e_now, i);
-            if (next.j != now.j || u + 1u == units) {
-                // the block's sums: of listed elements over the four lanes of a row, of the plane as they are
-                float *const part = parts + (wc * R.n_blocks + wb + now.j * waves_across) * PART;
+                    const uint32_t to = lane_offset(task * 128u + 2u * lane) * MT;
+                    if constexpr (MT == 1) {
+                        *reinterpret_cast<LN_LDS(uint32_t) *>((uintptr_t)(x_at + to)) = v[0];
+                        continue;
+                    }
 #pragma unroll
-                for (int r = 0; r < MT; ++r) {
-                    ex[r] += ln_dpp<0x124>(ex[r]);
-                    ex[r] += ln_dpp<0x128>(ex[r]);
+                    for (uint32_t j = 0; j < 2; ++j)
+#pragma unroll
+                        for (uint32_t h = 0; h < MT / 8u; ++h) {
+                            ln_u32x4 o;
+#pragma unroll
+                            for (uint32_t k = 0; k < 4; ++k)
+                                o[k] = __builtin_amdgcn_perm(v[8 * h + 2 * k + 1], v[8 * h + 2 * k], j ? 0x07060302u : 0x05040100u);
+                            *reinterpret_cast<LN_LDS(ln_u32x4) *>((uintptr_t)(x_at + (lr_place<MT>(to + j * ROW) ^ (h * 16u)))) = o;
+                        }
                 }
-                if (n < 4u)
-#pragma unroll
-                    for (uint32_t r = 0; r < MT; ++r) part[(4u * kg + n) * MT + r] += ex[r];
-                ln_wave_order();
-                if (n < MT)
-#pragma unroll
-                    for (uint32_t k = 0; k < 4; ++k) part[(4u * kg + k) * MT + n] += acc[k];
-                ln_wave_order();
-                acc = ln_f32x4{0, 0, 0, 0};
-#pragma unroll
-                for (int r = 0; r < MT; ++r) ex[r] = 0.0f;
+                if (tid < kZeros / 16u) *reinterpret_cast<LN_LDS(ln_u32x4) *>((uintptr_t)(x_at + x_none + tid * 16u)) = ln_u32x4{0, 0, 0, 0};
+                staged = tile;
             }
-            now = next;
-            next = after(now);
-            e_now = e_next;
+            if (e_table != e) {
+                ln_build_lut<BITS, WIDE>(smem, scale, tid, kExThreads);
+                e_table = e;
+            }
+            Group list[2];
 #pragma unroll
             for (uint32_t i = 0; i < 2; ++i) list[i] = g_load(e_now, i);
-            e_next = extent(next);
-        }
-    }
-    __syncthreads();
+            asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
 
-    // ---- outputs: the waves' parts, in column order ----
-    auto sum_of = [&](uint32_t block, uint32_t row, uint32_t r) {
-        float v = 0.0f;
-        for (uint32_t k = 0; k < R.waves_along; ++k) v += parts[(k * R.n_blocks + block) * PART + row * MT + r];
-        return v;
-    };
-    const uint32_t per = FIRST && R.gated ? 2u : 1u, n_out = n_blocks / per * 16u, at0 = b0 / per * 16u;
-    const uint16_t *const bias = W.bias ? W.bias + (size_t)e * (per * W.outputs) : nullptr;
-    for (uint32_t i = tid; i < n_out * count; i += kExThreads) {
-        const uint32_t r = i / n_out, at = i - r * n_out, block = (at >> 4) * per, row = at & 15u, out = at0 + at;
-        if (out >= W.outputs) continue;
-        float v = sum_of(block, row, r);
-        if (bias) v += bf16_bits_to_f32(bias[out]);
-        if constexpr (FIRST) {
-            v = ep_activation(R.activation, v);
-            if (R.gated) {
-                float u = sum_of(block + 1u, row, r);
-                if (bias) u += bf16_bits_to_f32(bias[W.outputs + out]);
-                v *= u;
+            // ---- this wave's cells ----
+            ln_f32x4 acc = {0, 0, 0, 0};
+            float ex[MT];
+#pragma unroll
+            for (int r = 0; r < MT; ++r) ex[r] = 0.0f;
+            const uint32_t c_seg = c0 * 1024u;
+            auto listed = [&](const Group &g, const Extent &x, uint32_t i) {
+                const uint32_t q = quad_of(x, i);
+                const uint32_t w01 = ln_pack((float)(int)(int8_t)g.val * scale, (float)(int)(int8_t)(g.val >> 8) * scale);
+                const uint32_t w23 = ln_pack((float)(int)(int8_t)(g.val >> 16) * scale, (float)((int)g.val >> 24) * scale);
+#pragma unroll
+                for (uint32_t k = 0; k < 4; ++k) {
+                    const uint32_t p = ((g.pos[k >> 1] >> (16 * (k & 1))) - c_seg) & 0xFFFFu;
+                    const bool is = q + k >= x.first && q + k < x.end && ((g.val >> (8 * k)) & 255u);
+                    if (!__any(is)) continue;  // (a cell of few listed elements has them in the first quads of the first lanes)
+                    const uint32_t at = is ? min(p * MT, x_none) : x_none;
+                    const uint32_t wk = k & 2 ? w23 : w01, wbits = k & 1 ? wk & 0xFFFF0000u : wk << 16;
+                    const float wv = __uint_as_float(wbits) - __uint_as_float((wbits & 0x80000000u) | scale_bits);  // (no element: times 0)
+                    if constexpr (MT == 1) {
+                        const uint32_t h = *reinterpret_cast<const LN_LDS(uint16_t) *>((uintptr_t)(x_at + at));
+                        ex[0] = __fmaf_rn(wv, __uint_as_float(h << 16), ex[0]);
+                    }
+#pragma unroll
+                    for (uint32_t h = 0; h < MT / 8u; ++h) {
+                        const ln_u32x4 v = *reinterpret_cast<const LN_LDS(ln_u32x4) *>((uintptr_t)(x_at + (lr_place<MT>(at) ^ (h * 16u))));
+#pragma unroll
+                        for (uint32_t j = 0; j < 4; ++j) {
+                            ex[8 * h + 2 * j] = __fmaf_rn(wv, __uint_as_float(v[j] << 16), ex[8 * h + 2 * j]);
+                            ex[8 * h + 2 * j + 1] = __fmaf_rn(wv, __uint_as_float(v[j] & 0xFFFF0000u), ex[8 * h + 2 * j + 1]);
+                        }
+                    }
+                }
+            };
+#pragma unroll 1
+            for (uint32_t u = u0; u < u1; ++u) {
+                const uint32_t x_cell = x_mine + now.c * (512u * ROW), x_second = x_other + now.c * (512u * ROW);
+#pragma unroll
+                for (uint32_t half = 0; half < 2; ++half) {
+                    uint32_t o[2][16];
+                    ln_decode<BITS, WIDE>(w[half][0], lut_lane, scale, o[0]);
+                    ln_decode<BITS, WIDE>(w[half][1], lut_lane, scale, o[1]);
+                    load(codes, next.c, half);
+                    // (columns 128 q + 32 i of a cell lie at 128 q + 32 (i ^ q))
+#pragma unroll
+                    for (uint32_t j = 0; j < 2; ++j)
+#pragma unroll
+                        for (uint32_t i = 0; i < 4; ++i) {
+                            const uint32_t q = 2u * half + j, at = (q * 128u + (q ^ i) * 32u) * ROW;
+                            ln_bf16x8 x;
+                            if constexpr (MT == 1) {  // (one row in all sixteen columns of the product)
+                                x = __builtin_bit_cast(ln_bf16x8, *reinterpret_cast<const LN_LDS(ln_u32x4) *>((uintptr_t)(x_cell + at)));
+                            } else {
+                                const lr_bf16x4 lo = lr_turned(x_cell + at), hi = lr_turned(x_second + at);
+                                x = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+                            }
+                            acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
+                                __builtin_bit_cast(ln_bf16x8, ln_u32x4{o[j][4 * i], o[j][4 * i + 1], o[j][4 * i + 2], o[j][4 * i + 3]}), x, acc, 0, 0, 0);
+                        }
+                }
+                const uint32_t g = e_now.end > e_now.first ? (e_now.end - (e_now.first & ~3u) + 15u) / 16u : 0u;
+                if (__any(g > 0u)) listed(list[0], e_now, 0);
+                if (__any(g > 1u)) listed(list[1], e_now, 1);
+#pragma unroll 1
+                for (uint32_t i = 2; __any(g > i); ++i) listed(g_load(e_now, i), e_now, i);
+                if (next.b != now.b || u + 1u == u1) {
+                    // the block's sums: of listed elements over the four lanes of a row, of the plane as they are
+                    float *const part = parts + (wave + now.b) * PART;
+#pragma unroll
+                    for (int r = 0; r < MT; ++r) {
+                        ex[r] += ln_dpp<0x124>(ex[r]);
+                        ex[r] += ln_dpp<0x128>(ex[r]);
+                    }
+                    if constexpr (MT == 1) {
+                        if (n < 4u) part[4u * kg + n] = ex[0];
+                    } else if (n < 4u)
+#pragma unroll
+                        for (uint32_t r = 0; r < MT; r += 4)
+                            *reinterpret_cast<ln_f32x4 *>(part + (4u * kg + n) * MT + r) = ln_f32x4{ex[r], ex[r + 1], ex[r + 2], ex[r + 3]};
+                    ln_wave_order();
+                    if (n < MT)
+#pragma unroll
+                        for (uint32_t k = 0; k < 4; ++k) part[(4u * kg + k) * MT + n] += acc[k];
+                    acc = ln_f32x4{0, 0, 0, 0};
+#pragma unroll
+                    for (int r = 0; r < MT; ++r) ex[r] = 0.0f;
+                }
+                now = next;
+                next = after(now);
+                e_now = e_next;
+#pragma unroll
+                for (uint32_t i = 0; i < 2; ++i) list[i] = g_load(e_now, i);
+                if (next.b != now.b) codes = codes_of(next.b), places = cells_of(next.b);
+                e_next = extent(places, next);
             }
-            static_cast<uint16_t *>(R.out)[(int64_t)(first + r) * R.ld_out + out] = ep_bf16(v);
-        } else {
-            const uint32_t to = R.n_tiles ? R.order[first + r] : first;
-            static_cast<float *>(R.out)[(int64_t)to * R.ld_out + out] = v;
+            __syncthreads();
+
+            // ---- the waves' parts of a block, in column order ----
+            auto sum_of = [&](uint32_t block, uint32_t at) {
+                const uint32_t wa = ((block * cells + 1u) * kExWaves - 1u) / units, wb = ((block + 1u) * cells * kExWaves - 1u) / units;
+                float v = 0.0f;
+                for (uint32_t k = wa; k <= wb; ++k)  // (waves without a cell left no part)
+                    if (k * units / kExWaves != (k + 1u) * units / kExWaves) v += parts[(k + block) * PART + at];
+                return v;
+            };
+            const bool last = c0 + cells == C;
+            if (cells != C) {  // chunks: their sums are added up
+                for (uint32_t i = tid; i < blocks * PART; i += kExThreads) {
+                    const float v = sum_of(i / PART, i % PART);
+                    totals[i] = c0 ? totals[i] + v : v;
+                }
+                __syncthreads();
+                if (!last) continue;
+            }
+            auto value = [&](uint32_t block, uint32_t at) { return cells != C ? totals[block * PART + at] : sum_of(block, at); };
+            // ---- outputs ----
+            const uint32_t n_out = blocks / per * 16u, at0 = b0 / per * 16u;
+            const uint16_t *const bias = W.bias ? W.bias + (size_t)e * (per * W.outputs) : nullptr;
+            for (uint32_t i = tid; i < n_out * count; i += kExThreads) {
+                const uint32_t r = i / n_out, at = i - r * n_out, block = (at >> 4) * per, in_part = (at & 15u) * MT + r, out = at0 + at;
+                if (out >= W.outputs) continue;
+                float v = value(block, in_part);
+                if (bias) v += bf16_bits_to_f32(bias[out]);
+                if constexpr (FIRST) {
+                    v = ep_activation(R.activation, v);
+                    if (R.gated) {
+                        float u = value(block + 1u, in_part);
+                        if (bias) u += bf16_bits_to_f32(bias[W.outputs + out]);
+                        v *= u;
+                    }
+                    static_cast<uint16_t *>(R.out)[(int64_t)(first + r) * R.ld_out + out] = ep_bf16(v);
+                } else {
+                    const uint32_t to = R.n_tiles ? R.order[first + r] : first;
+                    static_cast<float *>(R.out)[(int64_t)to * R.ld_out + out] = v;
+                }
+            }
+            __syncthreads();
         }
     }
 }
@@ -410,57 +480,55 @@ k_experts_join(const float *__restrict__ per_slot, ExCall call, uint32_t experts
 }
 
 // ---- host ----
-struct ExShape { uint32_t rows, n_blocks, waves_along, chunk_cells; size_t lds; };
-
-template <int BITS>
-static size_t ex_lds(uint32_t rows, uint32_t cells, uint32_t waves_along, uint32_t n_blocks) {
-    return kExXAt<BITS> + (size_t)(cells * kLnCols + 16u) * 2u * rows + (size_t)waves_along * n_blocks * 16u * rows * sizeof(float);
+template <int BITS, int MT, bool WIDE> static size_t ex_lds(uint32_t cells, uint32_t blocks, bool chunks) {
+    return kExXAt<BITS, WIDE> + (size_t)cells * kLnCols * 2u * MT + 256u + (size_t)(kExWaves + blocks * (chunks ? 2u : 1u)) * 16u * MT * sizeof(float);
 }
 
-// How a matrix is cut: blocks of a workgroup, waves along the columns, cells of a chunk.
-template <int BITS>
-static ExShape ex_shape(const ExMatrix &W, uint32_t rows, uint32_t n_tiles, uint32_t step) {
-    const uint32_t all = (W.n_tiles + 3u) / 4u;
-    ExShape p{};
-    p.rows = rows;
-    // as many blocks to a workgroup as leave two workgroups to a CU
-    const uint32_t wanted = std::max(2u * ln_cus() / std::max(n_tiles, 1u), 1u);
-    p.n_blocks = std::min(std::max((all + wanted - 1u) / wanted, step), 16u);
-    p.n_blocks = (p.n_blocks + step - 1u) / step * step;
-    p.waves_along = 1;
-    while (p.waves_along < kExWaves && p.n_blocks * p.waves_along < kExWaves && 2u * p.waves_along <= W.n_cells) p.waves_along *= 2u;
+template <int BITS, int MT, bool WIDE, bool FIRST>
+static int ex_launch(const ExMatrix &W, ExRows R, uint32_t n_tiles, hipStream_t s) {
+    const uint32_t per = FIRST && R.gated ? 2u : 1u, all = (W.n_tiles + 3u) / 4u;
+    R.per_tile = all / per;
+    // as few chunks as leave room for the sums of eight blocks, and as many blocks of a part as then fit, up to those that a workgroup has at all
+    // Few tiles: as many workgroups to each, so that none begins a second one (which takes as long as some ten cells).
+    const uint64_t items = (uint64_t)n_tiles * R.per_tile;
+    R.of_tile = R.n_tiles || n_tiles > ln_cus() ? 0u : std::min(ln_cus() / n_tiles, R.per_tile);
+    const uint32_t groups = R.of_tile ? n_tiles * R.of_tile : (uint32_t)std::min<uint64_t>(items, ln_cus());
+    const uint32_t share = (uint32_t)std::min<uint64_t>((items + groups - 1u) / groups, R.per_tile) * per;
     for (uint32_t chunks = 1;; ++chunks) {
-        p.chunk_cells = (W.n_cells + chunks - 1u) / chunks;
-        if (p.chunk_cells == 1u) break;
-        if (p.chunk_cells <= kLnSegCells && ex_lds<BITS>(rows, p.chunk_cells, p.waves_along, p.n_blocks) <= kLnLds / 2u) break;
+        R.chunk_cells = (W.n_cells + chunks - 1u) / chunks;
+        if (R.chunk_cells <= kLnSegCells && ex_lds<BITS, MT, WIDE>(R.chunk_cells, 8u, chunks > 1u) <= kLnLds) break;
+        if (R.chunk_cells == 1u) return IXH_EUNSUPPORTED;
     }
-    p.lds = ex_lds<BITS>(rows, p.chunk_cells, p.waves_along, p.n_blocks);
-    return p;
-}
-
-template <int BITS, int MT, bool FIRST>
-static int ex_rows(const ExMatrix &W, ExRows R, uint32_t n_tiles, hipStream_t s) {
-    const uint32_t step = FIRST && R.gated ? 2u : 1u;
-    const ExShape p = ex_shape<BITS>(W, MT, n_tiles, step);
-    if (p.lds > kLnLds) return IXH_EUNSUPPORTED;
-    static const bool raised = hipFuncSetAttribute(reinterpret_cast<const void *>(k_experts_rows<BITS, MT, FIRST>),
+    const bool chunks = R.chunk_cells < W.n_cells;
+    R.most_blocks = std::max(share, per);
+    while (R.most_blocks > 8u && ex_lds<BITS, MT, WIDE>(R.chunk_cells, R.most_blocks, chunks) > kLnLds) R.most_blocks -= per;
+    const size_t lds = ex_lds<BITS, MT, WIDE>(R.chunk_cells, R.most_blocks, chunks);
+    static const bool raised = hipFuncSetAttribute(reinterpret_cast<const void *>(k_experts_rows<BITS, MT, WIDE, FIRST>),
                                                    hipFuncAttributeMaxDynamicSharedMemorySize, (int)kLnLds) == hipSuccess;
     if (!raised) return IXH_ELAUNCH;
-    R.n_blocks = p.n_blocks, R.all_blocks = (W.n_tiles + 3u) / 4u, R.waves_along = p.waves_along, R.chunk_cells = p.chunk_cells;
     R.pairs = ((uintptr_t)R.x & 3u) == 0 && W.in_f % 2u == 0 && R.ldx % 2 == 0;
-    IXH_LAUNCH((k_experts_rows<BITS, MT, FIRST>), dim3(n_tiles, (R.all_blocks + p.n_blocks - 1u) / p.n_blocks), dim3(kExThreads), p.lds, s, W, R);
+    IXH_LAUNCH((k_experts_rows<BITS, MT, WIDE, FIRST>), dim3(groups), dim3(kExThreads), lds, s, W, R);
     return hipGetLastError() == hipSuccess ? IXH_OK : IXH_ELAUNCH;
 }
 
-template <bool FIRST> static int ex_matrix(const ExMatrix &W, const ExRows &R, uint32_t rows, uint32_t n_tiles, hipStream_t s) {
-#define EX_ROWS(B) (rows <= 8 ? ex_rows<B, 8, FIRST>(W, R, n_tiles, s) : ex_rows<B, 16, FIRST>(W, R, n_tiles, s))
-    switch (W.bits) {
-        case 3: return EX_ROWS(3);
-        case 4: return EX_ROWS(4);
-        case 5: return EX_ROWS(5);
-        default: return EX_ROWS(8);
+template <int BITS, bool FIRST> static int ex_rows(const ExMatrix &W, const ExRows &R, uint32_t rows, uint32_t n_tiles, hipStream_t s) {
+    // The larger pair table where a CU has cells enough to repay its writing, and LDS the room beside the activations.
+    if constexpr (BITS == 5) {
+        const bool fits = ex_lds<5, 16, true>(W.n_cells, 8u, false) <= kLnLds;
+        if (rows > 1u && fits && (uint64_t)n_tiles * W.n_tiles * W.n_cells > 128ull * ln_cus())
+            return rows <= 8 ? ex_launch<5, 8, true, FIRST>(W, R, n_tiles, s) : ex_launch<5, 16, true, FIRST>(W, R, n_tiles, s);
     }
-#undef EX_ROWS
+    constexpr bool WIDE = BITS == 4;
+    if (rows == 1u) return ex_launch<BITS, 1, WIDE, FIRST>(W, R, n_tiles, s);
+    return rows <= 8 ? ex_launch<BITS, 8, WIDE, FIRST>(W, R, n_tiles, s) : ex_launch<BITS, 16, WIDE, FIRST>(W, R, n_tiles, s);
+}
+template <bool FIRST> static int ex_matrix(const ExMatrix &W, const ExRows &R, uint32_t rows, uint32_t n_tiles, hipStream_t s) {
+    switch (W.bits) {
+        case 3: return ex_rows<3, FIRST>(W, R, rows, n_tiles, s);
+        case 4: return ex_rows<4, FIRST>(W, R, rows, n_tiles, s);
+        case 5: return ex_rows<5, FIRST>(W, R, rows, n_tiles, s);
+        default: return ex_rows<8, FIRST>(W, R, rows, n_tiles, s);
+    }
 }
 
 // Many tokens to an expert: 16 and more in the mean.
@@ -524,7 +592,7 @@ int launch_experts(const ExDev &X, const ExCall &call, void *workspace, hipStrea
         rc = launch_experts_prompt(X, call, plan, n_tiles, w.blocks, ws + w.x, ws + w.inner, per_slot, s);
     } else {
         ExRows R{};
-        R.x = call.x, R.ldx = call.ldx, R.ids = call.ids, R.experts = X.experts, R.top_k = call.top_k;
+        R.x = call.x, R.ldx = call.ldx, R.ids = call.ids, R.experts = X.experts, R.top_k = call.top_k, R.slots = slots;
         if (planned) R.n_tiles = plan.n_tiles, R.tiles = plan.tiles, R.order = plan.order;
         R.out = ws + w.inner, R.ld_out = w.ld_inner, R.activation = X.activation, R.gated = X.gated;
         rc = ex_matrix<true>(X.first, R, planned ? w.rows : 1u, n_tiles, s);
