@@ -106,7 +106,8 @@ def host():
         _host.bind(*(C.cast(f, C.c_void_p).value for f in (
             L.ixh_prefix_entries, L.ixh_prefix_workspace_bytes, L.ixh_prefix_build_ws, L.ixh_decode, L.ixh_decode_gs,
             L.ixh_decode_unranked_takes, L.ixh_decode_unranked_workspace_bytes, L.ixh_decode_unranked_ws, L.ixh_encode_workspace_bytes,
-            L.ixh_encode_scan_counts, L.ixh_encode_wait, L.ixh_encode_pack)), check)
+            L.ixh_encode_scan_counts, L.ixh_encode_wait, L.ixh_encode_pack, L.ixh_lanes_product, L.ixh_lanes_product_workspace_bytes, L.ixh_route,
+            L.ixh_experts, L.ixh_experts_workspace_bytes)), check)
         _native = _host
     return _native
 

@@ -512,10 +512,14 @@ static int ex_launch(const ExMatrix &W, ExRows R, uint32_t n_tiles, hipStream_t 
 }
 
 template <int BITS, bool FIRST> static int ex_rows(const ExMatrix &W, const ExRows &R, uint32_t rows, uint32_t n_tiles, hipStream_t s) {
-    // The larger pair table where a CU has cells enough to repay its writing, and LDS the room beside the activations.
+    // The larger pair table where a CU has cells enough to repay its writing, and LDS room for it beside the activations and the sums of all
+    // that a workgroup has of a tile (us, smaller / larger: 64 tokens by 6 of 64 experts, 17 blocks of two cells a workgroup 39 / 34.4; 35 of
+    // four, which the larger one takes in three parts, 55.6 / 59).
     if constexpr (BITS == 5) {
-        const bool fits = ex_lds<5, 16, true>(W.n_cells, 8u, false) <= kLnLds;
-        if (rows > 1u && fits && (uint64_t)n_tiles * W.n_tiles * W.n_cells > 128ull * ln_cus())
+        const uint32_t per = FIRST && R.gated ? 2u : 1u, blocks = (W.n_tiles + 3u) / 4u;
+        const uint32_t share = std::min((uint32_t)(((uint64_t)n_tiles * blocks / per + ln_cus() - 1u) / ln_cus()) * per, blocks);
+        if (rows > 1u && (uint64_t)n_tiles * W.n_tiles * W.n_cells > 128ull * ln_cus() && W.n_cells <= kLnSegCells &&
+            (rows <= 8 ? ex_lds<5, 8, true>(W.n_cells, share, false) : ex_lds<5, 16, true>(W.n_cells, share, false)) <= kLnLds)
             return rows <= 8 ? ex_launch<5, 8, true, FIRST>(W, R, n_tiles, s) : ex_launch<5, 16, true, FIRST>(W, R, n_tiles, s);
     }
     constexpr bool WIDE = BITS == 4;

@@ -242,6 +242,11 @@ struct Library {
     decltype(&ixh_encode_scan_counts) encode_scan;
     decltype(&ixh_encode_wait) encode_wait;
     decltype(&ixh_encode_pack) encode_pack;
+    decltype(&ixh_lanes_product) lanes_product;
+    decltype(&ixh_lanes_product_workspace_bytes) lanes_product_workspace_bytes;
+    decltype(&ixh_route) route;
+    decltype(&ixh_experts) experts;
+    decltype(&ixh_experts_workspace_bytes) experts_workspace_bytes;
     PyObject *check;
 } library;
 
@@ -259,10 +264,13 @@ bool checked(int rc) {
 }
 
 // bind(prefix_entries, prefix_workspace_bytes, prefix_build_ws, decode, decode_gs, decode_unranked_takes, decode_unranked_workspace_bytes,
-// decode_unranked_ws, encode_workspace_bytes, encode_scan_counts, encode_wait, encode_pack, check): addresses, and what raises for a negative code
+// decode_unranked_ws, encode_workspace_bytes, encode_scan_counts, encode_wait, encode_pack, lanes_product, lanes_product_workspace_bytes, route,
+// experts, experts_workspace_bytes, check): addresses, and what raises for a negative code
 PyObject *bind(PyObject *, PyObject *args) {
-    PyObject *f[12], *check;
-    if (!PyArg_ParseTuple(args, "OOOOOOOOOOOOO", &f[0], &f[1], &f[2], &f[3], &f[4], &f[5], &f[6], &f[7], &f[8], &f[9], &f[10], &f[11], &check)) return nullptr;
+    PyObject *f[17], *check;
+    if (!PyArg_ParseTuple(args, "OOOOOOOOOOOOOOOOOO", &f[0], &f[1], &f[2], &f[3], &f[4], &f[5], &f[6], &f[7], &f[8], &f[9], &f[10], &f[11], &f[12],
+                          &f[13], &f[14], &f[15], &f[16], &check))
+        return nullptr;
     entry(library.prefix_entries, f[0]);
     entry(library.prefix_workspace_bytes, f[1]);
     entry(library.prefix_build, f[2]);
@@ -275,6 +283,11 @@ PyObject *bind(PyObject *, PyObject *args) {
     entry(library.encode_scan, f[9]);
     entry(library.encode_wait, f[10]);
     entry(library.encode_pack, f[11]);
+    entry(library.lanes_product, f[12]);
+    entry(library.lanes_product_workspace_bytes, f[13]);
+    entry(library.route, f[14]);
+    entry(library.experts, f[15]);
+    entry(library.experts_workspace_bytes, f[16]);
     if (PyErr_Occurred()) return nullptr;
     Py_INCREF(check);
     Py_XSETREF(library.check, check);
@@ -493,10 +506,156 @@ PyObject *encode(PyObject *, PyObject *const *args, Py_ssize_t n_args) {
     END_HANDLE_TH_ERRORS
 }
 
+// A contiguous tensor of this type on the current device that asks for no gradient; null for anything else.
+const at::Tensor *given(PyObject *o, at::ScalarType type, int64_t device) {
+    const at::Tensor *t = plain(o, type, device);
+    return t && !(t->requires_grad() && c10::GradMode::is_enabled()) ? t : nullptr;
+}
+bool alike(const at::Tensor &a, const at::Tensor &b, int64_t last) {  // the same leading dimensions, and `last`
+    return a.dim() == b.dim() && a.size(-1) == last && a.sizes().slice(0, a.dim() - 1) == b.sizes().slice(0, b.dim() - 1);
+}
+
+// route(logits, bias, top_k, n_groups, top_groups, scoring, renormalize, scale): (ids, weights), or None.
+// One token: 6.2 us a call (12.5 from Python).
+PyObject *route(PyObject *, PyObject *const *args, Py_ssize_t n_args) {
+    HANDLE_TH_ERRORS
+    if (n_args != 8 || !library.check) {
+        PyErr_SetString(PyExc_TypeError, "route: eight arguments, after bind");
+        return nullptr;
+    }
+    if (!THPVariable_CheckExact(args[0]) || !watching().empty()) Py_RETURN_NONE;
+    const at::Tensor &l = THPVariable_Unpack(args[0]);
+    if (!l.is_cuda()) Py_RETURN_NONE;
+    const at::ScalarType type = l.scalar_type();
+    const int32_t dtype = type == at::kFloat ? IXH_F32 : type == at::kHalf ? IXH_F16 : type == at::kBFloat16 ? IXH_BF16 : -1;
+    const int64_t device = c10::hip::current_device();
+    if (dtype < 0 || !given(args[0], type, device) || l.dim() < 1 || l.numel() < 1) Py_RETURN_NONE;
+    const int64_t experts = l.size(-1), tokens = l.numel() / experts;
+    const at::Tensor *bias = nullptr;
+    if (args[1] != Py_None) {
+        bias = given(args[1], at::kFloat, device);
+        if (!bias || bias->numel() != experts) Py_RETURN_NONE;
+    }
+    long v[5];
+    for (int i = 0; i < 5; ++i) v[i] = PyLong_AsLong(args[2 + i]);
+    const double scale = PyFloat_AsDouble(args[7]);
+    if (PyErr_Occurred()) {
+        PyErr_Clear();
+        Py_RETURN_NONE;
+    }
+    if (v[0] < 1 || v[0] > experts || experts > 1024) Py_RETURN_NONE;  // (what has to raise)
+    const IxhRouting routing{(int32_t)experts, (int32_t)v[0], (int32_t)v[1], (int32_t)v[2], (int32_t)v[3], (int32_t)v[4], (float)scale};
+    c10::SmallVector<int64_t, 4> shape(l.sizes().begin(), l.sizes().end());
+    shape.back() = v[0];
+    at::Tensor ids, weights;
+    int rc;
+    {
+        pybind11::gil_scoped_release without_gil;
+        ids = fresh(shape, at::kInt, device);
+        weights = fresh(shape, at::kFloat, device);
+        rc = library.route(&routing, l.const_data_ptr(), dtype, experts, tokens, bias ? static_cast<const float *>(bias->const_data_ptr()) : nullptr,
+                           static_cast<int32_t *>(ids.data_ptr()), static_cast<float *>(weights.data_ptr()),
+                           c10::hip::getCurrentHIPStream((c10::DeviceIndex)device).stream());
+    }
+    if (!checked(rc)) return nullptr;
+    PyObject *a = THPVariable_Wrap(std::move(ids)), *b = THPVariable_Wrap(std::move(weights));
+    PyObject *both = a && b ? PyTuple_Pack(2, a, b) : nullptr;
+    Py_XDECREF(a);
+    Py_XDECREF(b);
+    return both;
+    END_HANDLE_TH_ERRORS
+}
+
+// product(address of the IxhLanes, address of the bias, device, x, activation, multiplier, residual): the product with its epilogue in one
+// call of the library, or None.  The scratch is allocated for the call.
+PyObject *product(PyObject *, PyObject *const *args, Py_ssize_t n_args) {
+    HANDLE_TH_ERRORS
+    if (n_args != 7 || !library.check) {
+        PyErr_SetString(PyExc_TypeError, "product: seven arguments, after bind");
+        return nullptr;
+    }
+    const IxhLanes *lanes = reinterpret_cast<const IxhLanes *>(PyLong_AsUnsignedLongLong(args[0]));
+    const uint16_t *bias = reinterpret_cast<const uint16_t *>(PyLong_AsUnsignedLongLong(args[1]));
+    const long long device = PyLong_AsLongLong(args[2]), activation = PyLong_AsLongLong(args[4]);
+    if (PyErr_Occurred()) return nullptr;
+    if (!THPVariable_CheckExact(args[3]) || !watching().empty() || !THPVariable_Unpack(args[3]).is_cuda() || c10::hip::current_device() != device)
+        Py_RETURN_NONE;
+    const at::Tensor *x = given(args[3], at::kBFloat16, device);
+    if (!x || x->dim() < 1 || x->size(-1) != lanes->in_f) Py_RETURN_NONE;
+    const int64_t rows = x->numel() / lanes->in_f;
+    if (rows < 1 || rows > 4096 || (rows > kMaxRows && ((reinterpret_cast<uintptr_t>(x->const_data_ptr()) & 15u) || lanes->in_f % 8 || rows * lanes->in_f >= 1ll << 31)))
+        Py_RETURN_NONE;
+    IxhEpilogue ep{(int32_t)activation, nullptr, lanes->out_f, nullptr, lanes->out_f};
+    for (int i = 0; i < 2; ++i) {
+        if (args[5 + i] == Py_None) continue;
+        const at::Tensor *t = given(args[5 + i], at::kBFloat16, device);
+        if (!t || !alike(*t, *x, lanes->out_f)) Py_RETURN_NONE;
+        (i ? ep.residual : ep.multiplier) = static_cast<const uint16_t *>(t->const_data_ptr());
+    }
+    c10::SmallVector<int64_t, 4> shape(x->sizes().begin(), x->sizes().end());
+    shape.back() = lanes->out_f;
+    at::Tensor y, sums;
+    int rc;
+    {
+        pybind11::gil_scoped_release without_gil;
+        y = fresh(shape, at::kBFloat16, device);
+        const size_t need = library.lanes_product_workspace_bytes(lanes, (int32_t)rows);
+        if (need) sums = fresh({(int64_t)need}, at::kByte, device);
+        rc = library.lanes_product(lanes, static_cast<const uint16_t *>(x->const_data_ptr()), lanes->in_f, bias, (int32_t)rows, &ep,
+                                   static_cast<uint16_t *>(y.data_ptr()), lanes->out_f, need ? sums.data_ptr() : nullptr, need,
+                                   c10::hip::getCurrentHIPStream((c10::DeviceIndex)device).stream());
+    }
+    if (!checked(rc)) return nullptr;
+    return THPVariable_Wrap(std::move(y));
+    END_HANDLE_TH_ERRORS
+}
+
+// experts(address of the IxhExperts, device, most places of a call, x, ids, weights, residual): y, or None.
+PyObject *experts(PyObject *, PyObject *const *args, Py_ssize_t n_args) {
+    HANDLE_TH_ERRORS
+    if (n_args != 7 || !library.check) {
+        PyErr_SetString(PyExc_TypeError, "experts: seven arguments, after bind");
+        return nullptr;
+    }
+    const IxhExperts *of = reinterpret_cast<const IxhExperts *>(PyLong_AsUnsignedLongLong(args[0]));
+    const long long device = PyLong_AsLongLong(args[1]), most = PyLong_AsLongLong(args[2]);
+    if (PyErr_Occurred()) return nullptr;
+    if (!THPVariable_CheckExact(args[3]) || !watching().empty() || !THPVariable_Unpack(args[3]).is_cuda() || c10::hip::current_device() != device)
+        Py_RETURN_NONE;
+    const at::Tensor *x = given(args[3], at::kBFloat16, device), *ids = given(args[4], at::kInt, device), *weights = given(args[5], at::kFloat, device);
+    if (!x || !ids || !weights || x->dim() < 1 || x->size(-1) != of->hidden || x->numel() == 0 || ids->sizes() != weights->sizes()) Py_RETURN_NONE;
+    const int64_t tokens = x->numel() / of->hidden, top_k = ids->dim() ? ids->size(-1) : 0;
+    if (top_k < 1 || !alike(*ids, *x, top_k) || tokens > most / top_k) Py_RETURN_NONE;
+    const at::Tensor *residual = nullptr;
+    if (args[6] != Py_None) {
+        residual = given(args[6], at::kBFloat16, device);
+        if (!residual || residual->sizes() != x->sizes()) Py_RETURN_NONE;
+    }
+    at::Tensor y, scratch;
+    int rc;
+    {
+        pybind11::gil_scoped_release without_gil;
+        y = fresh(x->sizes(), at::kBFloat16, device);
+        const size_t need = library.experts_workspace_bytes(of, tokens, (int32_t)top_k);
+        scratch = fresh({(int64_t)need}, at::kByte, device);
+        rc = library.experts(of, static_cast<const uint16_t *>(x->const_data_ptr()), of->hidden, tokens, static_cast<const int32_t *>(ids->const_data_ptr()),
+                             static_cast<const float *>(weights->const_data_ptr()), (int32_t)top_k,
+                             residual ? static_cast<const uint16_t *>(residual->const_data_ptr()) : nullptr, of->hidden,
+                             static_cast<uint16_t *>(y.data_ptr()), of->hidden, scratch.data_ptr(), need,
+                             c10::hip::getCurrentHIPStream((c10::DeviceIndex)device).stream());
+    }
+    if (!checked(rc)) return nullptr;
+    return THPVariable_Wrap(std::move(y));
+    END_HANDLE_TH_ERRORS
+}
+
 PyMethodDef methods[] = {
     {"bind", bind, METH_VARARGS, "The library's entry points."},
     {"decode", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(decode)), METH_FASTCALL, "The bf16 weight of packed tensors, or None."},
     {"describe", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(describe_at)), METH_FASTCALL, "Fills an IxhPacked."},
+    {"route", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(route)), METH_FASTCALL, "Experts of each token and their weights, or None."},
+    {"product", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(product)), METH_FASTCALL, "A product with its epilogue, or None."},
+    {"experts", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(experts)), METH_FASTCALL, "The experts' products, or None."},
     {"encode", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(encode)), METH_FASTCALL, "Packed tensors of a bf16 weight, or None."},
     {nullptr, nullptr, 0, nullptr},
 };

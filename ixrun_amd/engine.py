@@ -251,7 +251,7 @@ class StreamingLinear(nn.Module):
         if getattr(self, LANE_BUFFERS[0], None) is not None:
             self._lanes = _lib.LanePacked(self.out_features, self.in_features, [getattr(self, b) for b in LANE_BUFFERS],
                                           self._scale)
-            self._lane_ref = ctypes.byref(self._lanes.struct)
+            self._lane_ref, self._lanes_at = ctypes.byref(self._lanes.struct), ctypes.addressof(self._lanes.struct)
             bias = self._bias
             if bias is not None and bias.dtype is torch.bfloat16 and bias.is_cuda and bias.is_contiguous():
                 self._bias_ptr = bias.data_ptr()  # added by the kernel
@@ -465,6 +465,11 @@ class StreamingLinear(nn.Module):
         output as its multiplier, a block's last projection the residual stream.  bf16 activations on the layer's device; no gradients.
         From the lane layout it is one kernel's epilogue; without one, and for 17 and more rows that are no whole 16-byte pieces,
         ``forward`` runs and the rest follows as a launch of its own, from the product rounded to bf16."""
+        act = _lib.ACTIVATIONS.get(activation)
+        if self._native is not None and self._use_fused and self._gemm_ok and not self._gemv_flags and act is not None:
+            y = _lib.host().product(self._lanes_at, self._bias_ptr or 0, self._scale.device.index, x, act, multiplier, residual)
+            if y is not None:
+                return y
         for name, t in (("x", x), ("multiplier", multiplier), ("residual", residual)):
             if t is None:
                 continue
@@ -494,7 +499,6 @@ class StreamingLinear(nn.Module):
         y = torch.empty(shape, dtype=torch.bfloat16, device=dev)
         if rows == 0:
             return y
-        act = _lib.ACTIVATIONS[activation]
 
         def epilogue(at):
             return _lib.IxhEpilogue(act, m2.data_ptr() + 2 * at * m2.stride(0) if m2 is not None else None, m2.stride(0) if m2 is not None else 0,

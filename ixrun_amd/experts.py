@@ -40,6 +40,10 @@ def route_experts(logits, top_k: int, *, scoring: str = "softmax", bias=None, n_
 
     A logit of -infinity closes its expert for the token (all of them for a token of padding); a place that finds no open expert has id -1
     and weight 0, which ``StreamingExperts`` passes over.  A NaN is chosen first and reaches the weights."""
+    top_groups = n_groups if top_groups is None else top_groups
+    done = _lib.host().route(logits, bias, top_k, n_groups, top_groups, SCORINGS.get(scoring), renormalize, scale)
+    if done is not None:
+        return done
     _inference_only("route_experts", logits, bias)
     if not logits.is_cuda:
         raise RuntimeError(f"logits must live on the GPU (got {logits.device}); the HIP path has no CPU fallback")
@@ -57,7 +61,6 @@ def route_experts(logits, top_k: int, *, scoring: str = "softmax", bias=None, n_
         if bias.device != dev or bias.numel() != experts:
             raise ValueError(f"bias must hold {experts} elements on {dev}")
         bias = bias.to(torch.float32).contiguous()
-    top_groups = n_groups if top_groups is None else top_groups
     routing = _lib.IxhRouting(experts, top_k, n_groups, top_groups, SCORINGS[scoring], bool(renormalize), scale)
     shape = logits.shape[:-1] + (max(top_k, 0),)
     ids = torch.empty(shape, dtype=torch.int32, device=dev)
@@ -177,7 +180,7 @@ class StreamingExperts(nn.Module):
         rows = -(-self.inner // 16) * 32 if self.gated else self.inner
         self._struct = _lib.IxhExperts(self.n_experts, self.gated, _lib.ACTIVATIONS[self.activation], self.hidden, self.inner,
                                        self._matrix("first", rows, self.hidden), self._matrix("second", self.hidden, self.inner))
-        self._struct_ref = C.byref(self._struct)
+        self._struct_ref, self._struct_at, self._device_index = C.byref(self._struct), C.addressof(self._struct), self._first_plane.device.index
 
     def _apply(self, fn, recurse=True):
         # .to() may move the buffers: point the arguments at the new storage.  (Their types are the layout's and stay.)
@@ -187,6 +190,7 @@ class StreamingExperts(nn.Module):
             t = getattr(self, name)
             if t.dtype != dtype:
                 raise TypeError(f"an experts' layer cannot be cast: {name} is {dtype}")
+        self._struct_at = 0
         if self._first_plane.is_cuda:
             self._bind()
         return out
@@ -226,6 +230,10 @@ class StreamingExperts(nn.Module):
         """``x`` bf16 [..., hidden]; ``ids`` (int32 or int64) and ``weights`` [..., top_k] as ``route_experts`` gives them; ``residual`` like ``x``.
 
         A place whose id is no expert's adds nothing."""
+        if self._struct_at:
+            y = _lib.host().experts(self._struct_at, self._device_index, MOST_PLACES, x, ids, weights, residual)
+            if y is not None:
+                return y
         _inference_only("StreamingExperts", x, weights, residual)
         dev = self._first_plane.device
         if x.dim() < 1 or x.shape[-1] != self.hidden:
