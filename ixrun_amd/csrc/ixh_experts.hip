@@ -124,7 +124,7 @@ k_experts_plan(const int32_t *__restrict__ ids, uint32_t slots, uint32_t experts
 }
 
 // ---------------------------------------------------------------------------------------------------------------
-// k_experts_rows<BITS, MT, WIDE, FIRST>: tiles of up to MT slots of one expert.
+// k_experts_rows<BITS, MT, WIDE, FIRST>: tiles of up to MT slots of one expert, MT = 1 or 8.
 //
 // As in k_lanes_rows a lane's decoded weights are its operand of v_mfma_f32_16x16x32_bf16 as they are, the activations of the tile lie in
 // LDS a column's rows together (transposing reads make them the other operand), and listed elements are multiplied in fp32 by the lane of
@@ -136,6 +136,9 @@ k_experts_plan(const int32_t *__restrict__ ids, uint32_t slots, uint32_t experts
 // columns) are dealt to the waves in equal runs as well; what a wave has of a block goes to LDS, and the epilogue adds the waves' parts in
 // the columns' order.  Rows longer than LDS holds are taken in chunks of cells, whose sums are added there.
 // ---------------------------------------------------------------------------------------------------------------
+// (Tiles of 16, which halve the decoding of an expert with more than eight, take longer: their listed elements cost twice as much, and 24 registers
+// go to memory.  us of a call, 8 / 16, 64 experts of 2048 x 1024 with 2, 8 and 16 tokens each: 68 / 91, 101 / 124, 149 / 156.)
+constexpr uint32_t kExTileRows = 8;
 constexpr uint32_t kExWaves = 16, kExThreads = kExWaves * kWave;
 
 struct ExRows {
@@ -159,6 +162,7 @@ __global__ void __launch_bounds__(kExThreads)
 k_experts_rows(ExMatrix W, ExRows R) {
     extern __shared__ __attribute__((aligned(16))) uint8_t ex_smem[];
     using P = LnPairs<BITS, WIDE>;
+    static_assert(MT == 1 || MT == 8, "rows of a tile");
     constexpr uint32_t ROW = 2u * MT, PART = 16u * MT;
     constexpr uint32_t kZeros = MT == 1 ? 64u : 256u;  // bytes behind the activations
     const uint32_t smem = (uint32_t)(uintptr_t)(LN_LDS(uint8_t) *)ex_smem;
@@ -169,11 +173,9 @@ k_experts_rows(ExMatrix W, ExRows R) {
     float *const parts = reinterpret_cast<float *>(ex_smem + kExXAt<BITS, WIDE> + x_none + kZeros);  // [wave + block][16][MT]
     float *const totals = parts + (kExWaves + R.most_blocks) * PART;  // [block][16][MT], with several chunks
     const uint32_t lut_lane = smem + ((lane & ((1u << P::kCopies) - 1u)) << 2);
-    // Where the lane's operands begin in the activations: of sixteen lanes pieces of four columns (of all rows), at 16 rows in a place of
-    // their own for the second four; of one row the lane's eight columns.  The blocks of 32 columns are added as constants.
-    const uint32_t piece = MT == 16 ? n & 3u : n & 1u;
-    const uint32_t x_mine = MT == 1 ? x_at + kg * 16u : (x_at + lr_place<MT>((8u * kg + (n >> 2)) * ROW)) ^ (piece * 8u);
-    const uint32_t x_other = MT == 16 ? x_mine ^ (4u * ROW) : x_mine + 4u * ROW;
+    // Where the lane's operands begin in the activations: of sixteen lanes pieces of four columns (of all rows), of one row the lane's eight
+    // columns.  What comes on top is the same for all lanes.
+    const uint32_t x_mine = x_at + (MT == 1 ? kg * 16u : (8u * kg + (n >> 2)) * ROW + (n & 1u) * 8u);
 
     // (below 2^30 items: fewer than 16 slots an expert)
     const uint32_t all_items = (R.n_tiles ? *R.n_tiles : R.slots) * R.per_tile;
@@ -264,39 +266,33 @@ k_experts_rows(ExMatrix W, ExRows R) {
             const uint32_t scale_bits = __float_as_uint(scale) & 0x7FFFFFFFu;
 
             if (staged != tile || cells != C) {
-                // ---- activations: a pair of columns a lane, all rows ----
+                // activations: a pair of columns a lane, all rows (rows past the last are the last one's, columns past the last the last ones)
                 for (uint32_t task = wave; task < 4u * cells; task += kExWaves) {
                     const uint32_t col = c0 * kLnCols + task * 128u + 2u * lane;
+                    const uint32_t keep = (col < W.in_f ? 0xFFFFu : 0u) | (col + 1u < W.in_f ? 0xFFFF0000u : 0u);
                     uint32_t v[MT];
 #pragma unroll
                     for (uint32_t k = 0; k < MT; ++k) {
-                        v[k] = 0;
-                        if (k < count) {
-                            const uint16_t *const row = R.x + (((int64_t)__builtin_amdgcn_readlane((int)(x_row >> 32), (int)k) << 32) |
-                                                               (uint32_t)__builtin_amdgcn_readlane((int)x_row, (int)k));
-                            if (R.pairs) {
-                                if (col < W.in_f) v[k] = *reinterpret_cast<const uint32_t *>(row + col);
-                            } else {
-                                if (col < W.in_f) v[k] = row[col];
-                                if (col + 1u < W.in_f) v[k] |= (uint32_t)row[col + 1u] << 16;
-                            }
-                        }
+                        const uint32_t r = min(k, count - 1u);
+                        const uint16_t *const row = R.x + (((int64_t)__builtin_amdgcn_readlane((int)(x_row >> 32), (int)r) << 32) |
+                                                           (uint32_t)__builtin_amdgcn_readlane((int)x_row, (int)r));
+                        if (R.pairs) v[k] = *reinterpret_cast<const uint32_t *>(row + min(col, W.in_f - 2u));
+                        else v[k] = row[min(col, W.in_f - 1u)] | (uint32_t)row[min(col + 1u, W.in_f - 1u)] << 16;
                     }
+#pragma unroll
+                    for (uint32_t k = 0; k < MT; ++k) v[k] = k < count ? v[k] & keep : 0u;
                     const uint32_t to = lane_offset(task * 128u + 2u * lane) * MT;
                     if constexpr (MT == 1) {
                         *reinterpret_cast<LN_LDS(uint32_t) *>((uintptr_t)(x_at + to)) = v[0];
-                        continue;
-                    }
+                    } else {
 #pragma unroll
-                    for (uint32_t j = 0; j < 2; ++j)
-#pragma unroll
-                        for (uint32_t h = 0; h < MT / 8u; ++h) {
+                        for (uint32_t j = 0; j < 2; ++j) {
                             ln_u32x4 o;
 #pragma unroll
-                            for (uint32_t k = 0; k < 4; ++k)
-                                o[k] = __builtin_amdgcn_perm(v[8 * h + 2 * k + 1], v[8 * h + 2 * k], j ? 0x07060302u : 0x05040100u);
-                            *reinterpret_cast<LN_LDS(ln_u32x4) *>((uintptr_t)(x_at + (lr_place<MT>(to + j * ROW) ^ (h * 16u)))) = o;
+                            for (uint32_t k = 0; k < 4; ++k) o[k] = __builtin_amdgcn_perm(v[2 * k + 1], v[2 * k], j ? 0x07060302u : 0x05040100u);
+                            *reinterpret_cast<LN_LDS(ln_u32x4) *>((uintptr_t)(x_at + to + j * ROW)) = o;
                         }
+                    }
                 }
                 if (tid < kZeros / 16u) *reinterpret_cast<LN_LDS(ln_u32x4) *>((uintptr_t)(x_at + x_none + tid * 16u)) = ln_u32x4{0, 0, 0, 0};
                 staged = tile;
@@ -332,20 +328,19 @@ k_experts_rows(ExMatrix W, ExRows R) {
                         const uint32_t h = *reinterpret_cast<const LN_LDS(uint16_t) *>((uintptr_t)(x_at + at));
                         ex[0] = __fmaf_rn(wv, __uint_as_float(h << 16), ex[0]);
                     }
-#pragma unroll
-                    for (uint32_t h = 0; h < MT / 8u; ++h) {
-                        const ln_u32x4 v = *reinterpret_cast<const LN_LDS(ln_u32x4) *>((uintptr_t)(x_at + (lr_place<MT>(at) ^ (h * 16u))));
+                    if constexpr (MT == 8) {
+                        const ln_u32x4 v = *reinterpret_cast<const LN_LDS(ln_u32x4) *>((uintptr_t)(x_at + at));
 #pragma unroll
                         for (uint32_t j = 0; j < 4; ++j) {
-                            ex[8 * h + 2 * j] = __fmaf_rn(wv, __uint_as_float(v[j] << 16), ex[8 * h + 2 * j]);
-                            ex[8 * h + 2 * j + 1] = __fmaf_rn(wv, __uint_as_float(v[j] & 0xFFFF0000u), ex[8 * h + 2 * j + 1]);
+                            ex[2 * j] = __fmaf_rn(wv, __uint_as_float(v[j] << 16), ex[2 * j]);
+                            ex[2 * j + 1] = __fmaf_rn(wv, __uint_as_float(v[j] & 0xFFFF0000u), ex[2 * j + 1]);
                         }
                     }
                 }
             };
 #pragma unroll 1
             for (uint32_t u = u0; u < u1; ++u) {
-                const uint32_t x_cell = x_mine + now.c * (512u * ROW), x_second = x_other + now.c * (512u * ROW);
+                const uint32_t x_cell = x_mine + now.c * (512u * ROW);
 #pragma unroll
                 for (uint32_t half = 0; half < 2; ++half) {
                     uint32_t o[2][16];
@@ -362,7 +357,7 @@ k_experts_rows(ExMatrix W, ExRows R) {
                             if constexpr (MT == 1) {  // (one row in all sixteen columns of the product)
                                 x = __builtin_bit_cast(ln_bf16x8, *reinterpret_cast<const LN_LDS(ln_u32x4) *>((uintptr_t)(x_cell + at)));
                             } else {
-                                const lr_bf16x4 lo = lr_turned(x_cell + at), hi = lr_turned(x_second + at);
+                                const lr_bf16x4 lo = lr_turned(x_cell + at), hi = lr_turned(x_cell + at + 4u * ROW);
                                 x = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
                             }
                             acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
@@ -461,17 +456,23 @@ k_experts_join(const float *__restrict__ per_slot, ExCall call, uint32_t experts
     const int32_t *const ids = call.ids + (size_t)t * call.top_k;
     const float *const weights = call.weights + (size_t)t * call.top_k;
     const float *const from = per_slot + (size_t)t * call.top_k * hidden + at;
-#pragma unroll 4
-    for (uint32_t j = 0; j < call.top_k; ++j) {
-        if ((uint32_t)ids[j] >= experts) continue;
-        const float w = weights[j];
-        if constexpr (N == 4) {
-            const Sums p = *reinterpret_cast<const Sums *>(from + (size_t)j * hidden);
+    constexpr uint32_t AHEAD = 8;  // experts asked for at a time (behind the last that one again; what no expert wrote is not used)
+    for (uint32_t j0 = 0; j0 < call.top_k; j0 += AHEAD) {
+        Sums p[AHEAD];
+        bool is[AHEAD];
+        float w[AHEAD];
 #pragma unroll
-            for (int k = 0; k < 4; ++k) v[k] = __fmaf_rn(w, p[k], v[k]);
-        } else {
-            v[0] = __fmaf_rn(w, from[(size_t)j * hidden], v[0]);
+        for (uint32_t i = 0; i < AHEAD; ++i) {
+            const uint32_t j = min(j0 + i, call.top_k - 1u);
+            is[i] = j0 + i < call.top_k && (uint32_t)ids[j] < experts;
+            w[i] = weights[j];
+            if constexpr (N == 4) p[i] = *reinterpret_cast<const Sums *>(from + (size_t)j * hidden);
+            else p[i][0] = from[(size_t)j * hidden];
         }
+#pragma unroll
+        for (uint32_t i = 0; i < AHEAD; ++i)
+#pragma unroll
+            for (int k = 0; k < N; ++k) v[k] = is[i] ? __fmaf_rn(w[i], p[i][k], v[k]) : v[k];
     }
     uint16_t *const y = call.y + (int64_t)t * call.ldy + at;
     const uint16_t *const residual = call.residual + (int64_t)t * call.ld_residual + at;
@@ -519,12 +520,11 @@ template <int BITS, bool FIRST> static int ex_rows(const ExMatrix &W, const ExRo
         const uint32_t per = FIRST && R.gated ? 2u : 1u, blocks = (W.n_tiles + 3u) / 4u;
         const uint32_t share = std::min((uint32_t)(((uint64_t)n_tiles * blocks / per + ln_cus() - 1u) / ln_cus()) * per, blocks);
         if (rows > 1u && (uint64_t)n_tiles * W.n_tiles * W.n_cells > 128ull * ln_cus() && W.n_cells <= kLnSegCells &&
-            (rows <= 8 ? ex_lds<5, 8, true>(W.n_cells, share, false) : ex_lds<5, 16, true>(W.n_cells, share, false)) <= kLnLds)
-            return rows <= 8 ? ex_launch<5, 8, true, FIRST>(W, R, n_tiles, s) : ex_launch<5, 16, true, FIRST>(W, R, n_tiles, s);
+            ex_lds<5, 8, true>(W.n_cells, share, false) <= kLnLds)
+            return ex_launch<5, 8, true, FIRST>(W, R, n_tiles, s);
     }
     constexpr bool WIDE = BITS == 4;
-    if (rows == 1u) return ex_launch<BITS, 1, WIDE, FIRST>(W, R, n_tiles, s);
-    return rows <= 8 ? ex_launch<BITS, 8, WIDE, FIRST>(W, R, n_tiles, s) : ex_launch<BITS, 16, WIDE, FIRST>(W, R, n_tiles, s);
+    return rows == 1u ? ex_launch<BITS, 1, WIDE, FIRST>(W, R, n_tiles, s) : ex_launch<BITS, 8, WIDE, FIRST>(W, R, n_tiles, s);
 }
 template <bool FIRST> static int ex_matrix(const ExMatrix &W, const ExRows &R, uint32_t rows, uint32_t n_tiles, hipStream_t s) {
     switch (W.bits) {
@@ -535,10 +535,13 @@ template <bool FIRST> static int ex_matrix(const ExMatrix &W, const ExRows &R, u
     }
 }
 
-// Many tokens to an expert: 16 and more in the mean.
+// Many tokens to an expert: 20 and more in the mean (us of a call, k_experts_rows / k_experts_prompt at 16, 24 and 32: 64 experts of 2048 x 1024
+// at 5 % listed 207 / 226, 299 / 230, 359 / 232, next to none listed 149 / 196, 224 / 198, 270 / 202; 16 of 4096 x 1536 130 / 168, 161 / 171, 207 / 175;
+// 20 of 1400 x 744 71 / 100, 81 / 100, 94 / 102).
+constexpr uint32_t kExMany = 20;
 // (Rows of up to 2^20 columns: offsets within a tile's rows are 32 bits.)
 static bool ex_many(const ExDev &X, uint32_t slots) {
-    return slots >= 16u * X.experts && std::max(X.first.n_cells, X.second.n_cells) <= 2048u;
+    return slots >= kExMany * X.experts && std::max(X.first.n_cells, X.second.n_cells) <= 2048u;
 }
 
 // A call's scratch: the plan, the intermediate, what each slot's expert makes of it, and in k_experts_prompt the gathered rows.
@@ -562,7 +565,7 @@ static ExScratch ex_scratch(const ExDev &X, uint32_t tokens, uint32_t top_k) {
         w.x = take((size_t)w.blocks * X.first.n_cells * 16384u);
         w.inner = take((size_t)w.blocks * X.second.n_cells * 16384u);
     } else {
-        w.rows = slots <= 4u * X.experts ? 8u : 16u;
+        w.rows = kExTileRows;
         w.n_tiles = std::min(slots, X.experts + slots / 8u);
         w.tiles = take((size_t)w.n_tiles * 12u);
         w.order = take((size_t)slots * 4u);
@@ -577,7 +580,7 @@ static ExScratch ex_scratch(const ExDev &X, uint32_t tokens, uint32_t top_k) {
 // Callers may hold a scratch of a larger call: enough for any count of tokens up to this one.
 size_t experts_workspace_bytes(const ExDev &X, uint32_t tokens, uint32_t top_k) {
     if (!tokens) return 0;
-    const uint32_t few = std::min(tokens, (16u * X.experts - 1u) / top_k);  // the most that are not many
+    const uint32_t few = std::min(tokens, (kExMany * X.experts - 1u) / top_k);  // the most that are not many
     return std::max(ex_scratch(X, tokens, top_k).bytes, few ? ex_scratch(X, few, top_k).bytes : 0u);
 }
 

@@ -1,144 +1,222 @@
 // Routing of tokens to experts: the choice among their logits, and the weights.
+#include <type_traits>
+
 #include "ixh_experts.h"
 
 namespace ixh {
 
-constexpr uint32_t kRtWaves = 4;  // tokens of a workgroup
+constexpr uint32_t kRtWaves = 4;
 
-template <class T> __device__ __forceinline__ float rt_logit(T v) { return (float)v; }
+// ---- all lanes of a token's group get the same: exchanges with the lane 1, 2, (3 and 12 in the mirrored halves), 16 and 32 away ----
+template <int CTRL> __device__ __forceinline__ uint32_t rt_dpp(uint32_t v) {
+    return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, 0xf, 0xf, true);
+}
+template <int CTRL> __device__ __forceinline__ float rt_dpp(float v) { return __uint_as_float(rt_dpp<CTRL>(__float_as_uint(v))); }
+template <int CTRL> __device__ __forceinline__ uint64_t rt_dpp(uint64_t v) {
+    return (uint64_t)rt_dpp<CTRL>((uint32_t)(v >> 32)) << 32 | rt_dpp<CTRL>((uint32_t)v);
+}
+template <int CTRL> __device__ __forceinline__ double rt_dpp(double v) {
+    return __builtin_bit_cast(double, rt_dpp<CTRL>(__builtin_bit_cast(uint64_t, v)));
+}
+template <int LT, class V, class F> __device__ __forceinline__ V rt_all(V v, F f) {
+    v = f(v, rt_dpp<0xB1>(v));   // quad_perm 1, 0, 3, 2
+    v = f(v, rt_dpp<0x4E>(v));   // quad_perm 2, 3, 0, 1
+    v = f(v, rt_dpp<0x141>(v));  // row_half_mirror
+    v = f(v, rt_dpp<0x140>(v));  // row_mirror
+    if constexpr (LT == 64) {
+        v = f(v, (V)__shfl_xor(v, 16));
+        v = f(v, (V)__shfl_xor(v, 32));
+    }
+    return v;
+}
+template <int LT, class V> __device__ __forceinline__ V rt_most(V v) { return rt_all<LT>(v, [](V a, V b) { return a > b ? a : b; }); }
+template <int LT, class V> __device__ __forceinline__ V rt_least(V v) { return rt_all<LT>(v, [](V a, V b) { return a < b ? a : b; }); }
+template <int LT, class V> __device__ __forceinline__ V rt_sum(V v) { return rt_all<LT>(v, [](V a, V b) { return a + b; }); }
 
-__device__ __forceinline__ double rt_shfl_xor(double v, int by) { return __shfl_xor(v, by); }
+// ---- a choice as a whole number of the same order: 0 is closed, NaN as infinity ----
+__device__ __forceinline__ uint32_t rt_key(float v) {
+    if (v == -__builtin_huge_valf()) return 0u;
+    if (v != v) v = __builtin_huge_valf();
+    const uint32_t b = __float_as_uint(v + 0.0f);  // (-0 is 0)
+    return b >> 31 ? ~b : b | 0x80000000u;
+}
+__device__ __forceinline__ uint64_t rt_key(double v) {
+    if (v == -__builtin_huge_val()) return 0u;
+    if (v != v) v = __builtin_huge_val();
+    const uint64_t b = __builtin_bit_cast(uint64_t, v + 0.0);
+    return b >> 63 ? ~b : b | 1ull << 63;
+}
+__device__ __forceinline__ double rt_of_key(uint64_t k) { return k ? __builtin_bit_cast(double, k >> 63 ? k & ~(1ull << 63) : ~k) : -__builtin_huge_val(); }
+// 16-bit logits: their own bits in the high half
+template <class T> __device__ __forceinline__ uint32_t rt_key_16(T t) {
+    const float v = (float)t;
+    if (v == -__builtin_huge_valf()) return 0u;
+    const uint32_t b = v != v ? (uint32_t)__builtin_bit_cast(uint16_t, (T)__builtin_huge_valf()) : v == 0.0f ? 0u : (uint32_t)__builtin_bit_cast(uint16_t, t);
+    return (b >> 15 ? ~b & 0xFFFFu : b | 0x8000u) << 16;
+}
 
 // ---------------------------------------------------------------------------------------------------------------
-// k_route<T, NV>: one wave a token, expert 64 v + lane in register v of the lane.
+// k_route<T, LT, NV, BIAS>: LT lanes a token, expert LT v + l in register v of lane l.
 //
 // Scores p = softmax(l) or sigmoid(l) over the experts that are open (l above -infinity).  The choice is by l itself without a bias, which
 // has the order of the scores, and by p + bias with one, in 64 bits: which experts are chosen must not hang on how exp is rounded.  A NaN
 // counts as the largest, so that it reaches the output.  Equal values go to the lowest index.
+//
+// Bound: vector instructions.  Choices are whole numbers of their order, of 16-bit logits with the index below them in one word, so that a
+// round of the choice is a largest number over the registers, four exchanges within the sixteen lanes of a row and a comparison to strike
+// it out, for four tokens at once: 30 instructions at 128 experts.  (A wave a token, 64-bit pairs of choice and index by permutes through
+// LDS: 16384 tokens by 128 experts, 8 chosen, 35 us.)  Without a bias only the chosen experts' scores are worked out, the sum over
+// all only where the weights are not divided by their own.
 // ---------------------------------------------------------------------------------------------------------------
-template <class T, int NV>
+template <class T, int LT, int NV, bool BIAS>
 __global__ void __launch_bounds__(kRtWaves *kWave)
 k_route(const T *__restrict__ logits, int64_t ld, uint32_t tokens, RouteDev R, const float *__restrict__ bias, int32_t *__restrict__ ids,
         float *__restrict__ weights) {
     extern __shared__ __attribute__((aligned(16))) uint8_t rt_smem[];
-    const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6, t = blockIdx.x * kRtWaves + wave;
-    if (t >= tokens) return;
+    constexpr bool JOINT = !BIAS && sizeof(T) == 2;  // choice and index in one word
+    using Key = std::conditional_t<BIAS, uint64_t, uint32_t>;
+    const uint32_t l = threadIdx.x & (LT - 1u), in_block = threadIdx.x / LT, t = blockIdx.x * (kRtWaves * kWave / LT) + in_block;
+    const T *const row = logits + (int64_t)min(t, tokens - 1u) * ld;
     const double inf = __builtin_huge_val();
-    const T *const row = logits + (int64_t)t * ld;
-    float l[NV];
-    double p[NV], choice[NV];
+    T raw[NV];
+#pragma unroll
+    for (int v = 0; v < NV; ++v) raw[v] = row[min(v * LT + l, R.experts - 1u)];
+    auto logit = [&](int v) { return v * LT + l < R.experts ? (float)raw[v] : -__builtin_huge_valf(); };
+
+    // ---- softmax: the largest logit and the sum, where they are needed ----
+    float most = 0.0f;
+    double sum = 1.0;
+    if (!R.sigmoid && (BIAS || !R.renormalize)) {
+        most = -__builtin_huge_valf();
+#pragma unroll
+        for (int v = 0; v < NV; ++v) most = fmaxf(most, logit(v));
+        most = rt_all<LT>(most, [](float a, float b) { return fmaxf(a, b); });
+        if (most == -__builtin_huge_valf()) most = 0.0f;  // no open expert, or NaN alone
+        sum = 0.0;
+#pragma unroll
+        for (int v = 0; v < NV; ++v) sum += exp((double)logit(v) - (double)most);
+        sum = rt_sum<LT>(sum);
+        if (sum == 0.0) sum = 1.0;
+    }
+    auto score = [&](float v) {
+        if (v == -__builtin_huge_valf()) return 0.0;
+        return R.sigmoid ? 1.0 / (1.0 + exp(-(double)v)) : exp((double)v - (double)most) / sum;
+    };
+
+    // ---- the choices ----
+    Key key[NV];
 #pragma unroll
     for (int v = 0; v < NV; ++v) {
-        const uint32_t e = 64u * v + lane;
-        l[v] = e < R.experts ? rt_logit(row[e]) : -__builtin_huge_valf();
-    }
-    if (R.sigmoid) {
-#pragma unroll
-        for (int v = 0; v < NV; ++v) p[v] = 1.0 / (1.0 + exp(-(double)l[v]));
-    } else {
-        float most = -__builtin_huge_valf();
-#pragma unroll
-        for (int v = 0; v < NV; ++v) most = fmaxf(most, l[v]);
-        for (int by = 32; by; by >>= 1) most = fmaxf(most, __shfl_xor(most, by));
-        if (most == -__builtin_huge_valf()) most = 0.0f;  // no open expert
-        double sum = 0.0;
-#pragma unroll
-        for (int v = 0; v < NV; ++v) {
-            p[v] = exp((double)l[v] - (double)most);
-            sum += p[v];
+        const uint32_t e = v * LT + l;
+        if constexpr (BIAS) {
+            const float of = logit(v);
+            key[v] = of == -__builtin_huge_valf() ? 0u : rt_key(score(of) + (double)bias[e]);
+        } else if constexpr (JOINT) {
+            const uint32_t k = e < R.experts ? rt_key_16(raw[v]) : 0u;
+            key[v] = k ? k | (0xFFFFu - e) : 0u;
+        } else {
+            key[v] = rt_key(logit(v));
         }
-        for (int by = 32; by; by >>= 1) sum += rt_shfl_xor(sum, by);
-        if (sum != 0.0)
-#pragma unroll
-            for (int v = 0; v < NV; ++v) p[v] /= sum;
-    }
-#pragma unroll
-    for (int v = 0; v < NV; ++v) {
-        const uint32_t e = 64u * v + lane;
-        const bool open = !(l[v] == -__builtin_huge_valf());
-        choice[v] = l[v];
-        if (bias && open) choice[v] = p[v] + (double)bias[e];
-        if (choice[v] != choice[v]) choice[v] = inf;
-        if (!open) choice[v] = -inf, p[v] = 0.0;
     }
     if (R.groups > 1u) {
-        // lane g works out group g: its best, or the sum of its two best where a bias takes part
-        double *const mine = reinterpret_cast<double *>(rt_smem) + wave * (R.experts + 64u), *const score = mine + R.experts;
+        // lane g works out group g (and those LT further on): its best, or the sum of its two best where a bias takes part
+        Key *const mine = reinterpret_cast<Key *>(rt_smem) + in_block * (R.experts + 64u), *const of_group = mine + R.experts;
 #pragma unroll
         for (int v = 0; v < NV; ++v)
-            if (64u * v + lane < R.experts) mine[64u * v + lane] = choice[v];
+            if (v * LT + l < R.experts) mine[v * LT + l] = JOINT ? key[v] & 0xFFFF0000u : key[v];
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
         __builtin_amdgcn_wave_barrier();
-        double best = -inf, second = -inf;
-        if (lane < R.groups)
+        for (uint32_t g = l; g < R.groups; g += LT) {
+            Key best = 0, second = 0;
             for (uint32_t i = 0; i < R.group_size; ++i) {
-                const double c = mine[lane * R.group_size + i];
+                const Key c = mine[g * R.group_size + i];
                 second = c > best ? best : c > second ? c : second;
                 best = c > best ? c : best;
             }
-        if (bias && best != -inf && second != -inf) best += second;
-        score[lane] = best;
+            if constexpr (BIAS)
+                if (best && second) best = rt_key(rt_of_key(best) + rt_of_key(second));
+            of_group[g] = best;
+        }
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
         __builtin_amdgcn_wave_barrier();
-        uint32_t before = 0;
-        for (uint32_t g = 0; g < R.groups; ++g) before += score[g] > best || (score[g] == best && g < lane);
-        const uint64_t kept = __ballot(lane < R.groups && before < R.top_groups);
-#pragma unroll
-        for (int v = 0; v < NV; ++v)
-            if (!((kept >> min((64u * v + lane) / R.group_size, 63u)) & 1u)) choice[v] = -inf;
-    }
-    int32_t id = -1;
-    double weight = 0.0;
-    for (uint32_t r = 0; r < R.top_k; ++r) {
-        double best = -inf;
-        uint32_t at = ~0u;
-#pragma unroll
-        for (int v = 0; v < NV; ++v)
-            if (choice[v] > best) best = choice[v], at = 64u * v + lane;
-        for (int by = 32; by; by >>= 1) {
-            const double other = rt_shfl_xor(best, by);
-            const uint32_t other_at = __shfl_xor(at, by);
-            if (other > best || (other == best && other_at < at)) best = other, at = other_at;
+        uint64_t kept = 0;
+        for (uint32_t g = l; g < R.groups; g += LT) {
+            const Key own = of_group[g];
+            uint32_t before = 0;
+            for (uint32_t h = 0; h < R.groups; ++h) before += of_group[h] > own || (of_group[h] == own && h < g);
+            kept |= (uint64_t)(before < R.top_groups) << g;
         }
-        if (best == -inf) break;
-        double of = 0.0;
+        kept = rt_all<LT>(kept, [](uint64_t a, uint64_t b) { return a | b; });
 #pragma unroll
         for (int v = 0; v < NV; ++v)
-            if (64u * v + lane == at) of = p[v], choice[v] = -inf;
-        of = __shfl(of, (int)(at & 63u));
-        if (lane == r) id = (int32_t)at, weight = of;
+            if (!((kept >> min((v * LT + l) / R.group_size, 63u)) & 1u)) key[v] = 0;
     }
+
+    // ---- the chosen ones: lane r has the r-th ----
+    uint32_t id = ~0u;
+    for (uint32_t r = 0; r < R.top_k; ++r) {
+        Key best = key[0];
+#pragma unroll
+        for (int v = 1; v < NV; ++v) best = key[v] > best ? key[v] : best;
+        best = rt_most<LT>(best);
+        uint32_t at;
+        if constexpr (JOINT) {
+            at = best ? 0xFFFFu - (best & 0xFFFFu) : ~0u;
+#pragma unroll
+            for (int v = 0; v < NV; ++v) key[v] = key[v] == best ? 0u : key[v];
+        } else {
+            at = ~0u;
+#pragma unroll
+            for (int v = NV - 1; v >= 0; --v) at = key[v] == best ? v * LT + l : at;
+            at = rt_least<LT>(best ? at : ~0u);
+#pragma unroll
+            for (int v = 0; v < NV; ++v) key[v] = v * LT + l == at ? 0u : key[v];
+        }
+        if (l == r) id = at;
+    }
+    const float chosen = id != ~0u ? (float)row[id] : -__builtin_huge_valf();
+    if (!R.sigmoid && !BIAS && R.renormalize) {  // (their ratios hang on no more than the largest of them)
+        most = __shfl(chosen, (int)(threadIdx.x & 63u & ~(LT - 1u)));
+        if (most == -__builtin_huge_valf()) most = 0.0f;
+    }
+    double weight = score(chosen);
     if (R.renormalize) {
-        double sum = weight;
-        for (int by = 32; by; by >>= 1) sum += rt_shfl_xor(sum, by);
-        weight = sum == 0.0 ? 0.0 : weight / sum;
+        const double all = rt_sum<LT>(weight);
+        weight = all == 0.0 ? 0.0 : weight / all;
     }
-    if (lane < R.top_k) {
-        ids[(size_t)t * R.top_k + lane] = id;
-        weights[(size_t)t * R.top_k + lane] = id < 0 ? 0.0f : (float)(weight * R.scale);
+    if (l < R.top_k && t < tokens) {
+        ids[(size_t)t * R.top_k + l] = (int32_t)id;
+        weights[(size_t)t * R.top_k + l] = id == ~0u ? 0.0f : (float)(weight * R.scale);
     }
 }
 
+template <class T, int LT, int NV>
+static void route_launch(const T *logits, int64_t ld, uint32_t tokens, const RouteDev &R, const float *bias, int32_t *ids, float *weights, hipStream_t s) {
+    constexpr uint32_t per = kRtWaves * kWave / LT;
+    const dim3 grid((tokens + per - 1u) / per), block(kRtWaves * kWave);
+    const size_t lds = R.groups > 1u ? per * (R.experts + 64u) * (bias ? 8u : 4u) : 0;
+    if (bias) IXH_LAUNCH((k_route<T, LT, NV, true>), grid, block, lds, s, logits, ld, tokens, R, bias, ids, weights);
+    else IXH_LAUNCH((k_route<T, LT, NV, false>), grid, block, lds, s, logits, ld, tokens, R, bias, ids, weights);
+}
+
 template <class T>
-static int route_launch(const void *logits, int64_t ld, uint32_t tokens, const RouteDev &R, const float *bias, int32_t *ids, float *weights,
-                        hipStream_t s) {
-    const dim3 grid((tokens + kRtWaves - 1u) / kRtWaves), block(kRtWaves * kWave);
-    const size_t lds = R.groups > 1u ? kRtWaves * (R.experts + 64u) * sizeof(double) : 0;
+static int route_type(const void *logits, int64_t ld, uint32_t tokens, const RouteDev &R, const float *bias, int32_t *ids, float *weights, hipStream_t s) {
     const T *const l = static_cast<const T *>(logits);
-    if (R.experts <= 64u) IXH_LAUNCH((k_route<T, 1>), grid, block, lds, s, l, ld, tokens, R, bias, ids, weights);
-    else if (R.experts <= 128u) IXH_LAUNCH((k_route<T, 2>), grid, block, lds, s, l, ld, tokens, R, bias, ids, weights);
-    else if (R.experts <= 256u) IXH_LAUNCH((k_route<T, 4>), grid, block, lds, s, l, ld, tokens, R, bias, ids, weights);
-    else if (R.experts <= 512u) IXH_LAUNCH((k_route<T, 8>), grid, block, lds, s, l, ld, tokens, R, bias, ids, weights);
-    else IXH_LAUNCH((k_route<T, 16>), grid, block, lds, s, l, ld, tokens, R, bias, ids, weights);
+    if (R.experts <= 64u && R.top_k <= 16u) route_launch<T, 16, 4>(l, ld, tokens, R, bias, ids, weights, s);
+    else if (R.experts <= 128u && R.top_k <= 16u) route_launch<T, 16, 8>(l, ld, tokens, R, bias, ids, weights, s);
+    else if (R.experts <= 128u) route_launch<T, 64, 2>(l, ld, tokens, R, bias, ids, weights, s);
+    else if (R.experts <= 256u) route_launch<T, 64, 4>(l, ld, tokens, R, bias, ids, weights, s);
+    else if (R.experts <= 512u) route_launch<T, 64, 8>(l, ld, tokens, R, bias, ids, weights, s);
+    else route_launch<T, 64, 16>(l, ld, tokens, R, bias, ids, weights, s);
     return hipGetLastError() == hipSuccess ? IXH_OK : IXH_ELAUNCH;
 }
 
 int launch_route(const void *logits, int dtype, int64_t ld, uint32_t tokens, const RouteDev &R, const float *bias, int32_t *ids, float *weights,
                  hipStream_t s) {
     switch (dtype) {
-        case IXH_F32: return route_launch<float>(logits, ld, tokens, R, bias, ids, weights, s);
-        case IXH_F16: return route_launch<_Float16>(logits, ld, tokens, R, bias, ids, weights, s);
-        default: return route_launch<__bf16>(logits, ld, tokens, R, bias, ids, weights, s);
+        case IXH_F32: return route_type<float>(logits, ld, tokens, R, bias, ids, weights, s);
+        case IXH_F16: return route_type<_Float16>(logits, ld, tokens, R, bias, ids, weights, s);
+        default: return route_type<__bf16>(logits, ld, tokens, R, bias, ids, weights, s);
     }
 }
 
