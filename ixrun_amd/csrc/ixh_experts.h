@@ -51,7 +51,7 @@ struct ExCall {
 };
 
 // The slots by expert.  For k_experts_rows tiles of a few slots each, {expert, first place in `order`, how many}; for k_experts_prompt
-// an expert's places are filled up to whole blocks of 16 (with ~0), and the tiles are {expert, first block, blocks}, up to 32 of them.
+// an expert's places are filled up to whole blocks of 16 (with ~0), and the tiles are {expert, first block, blocks}, up to 16 of them.
 struct ExPlan {
     uint32_t *n_tiles, *n_blocks, *tiles, *order;
 };

@@ -16,29 +16,33 @@ namespace ixh {
 // ---------------------------------------------------------------------------------------------------------------
 constexpr uint32_t kExPlanThreads = 1024, kExPlanWaves = kExPlanThreads / kWave;
 
-// Tiles of an expert with n slots: of up to `rows` of them; with rows = 0 of up to 32 blocks of 16, as even as whole eights of blocks
-// allow (what is left of an eighth is as long as the whole).
-__device__ __forceinline__ uint32_t ex_eights(uint32_t n) { return (n + 127u) / 128u; }
-__device__ __forceinline__ uint32_t ex_tiles(uint32_t n, uint32_t rows) { return rows ? (n + rows - 1u) / rows : (ex_eights(n) + 3u) / 4u; }
-// How many of these are of 4, 3, 2 and 1 eights of blocks: the order of the tiles, so that the last ones to be taken are short.  (Tiles of
-// `rows` slots are in the order of the experts.)
+// How an expert's slots are cut into tiles: of up to `rows` of them; with rows = 0 of up to four layers, a layer being 64 slots, a block of 16
+// to each wave of k_experts_prompt, as even as whole layers allow (what is left of a layer takes as long as the whole).
+constexpr uint32_t kExLayer = 64;
+struct ExCut {
+    uint32_t rows;
+    __device__ __forceinline__ uint32_t layers(uint32_t n) const { return (n + kExLayer - 1u) / kExLayer; }
+    __device__ __forceinline__ uint32_t tiles(uint32_t n) const { return rows ? (n + rows - 1u) / rows : (layers(n) + 3u) / 4u; }
+    __device__ __forceinline__ uint32_t places(uint32_t n) const { return rows ? n : (n + 15u) & ~15u; }
+};
+// How many of these are of 4, 3, 2 and 1 layers: the order of the tiles, so that the last ones to be taken are short.  (Tiles of `rows` slots
+// are in the order of the experts.)
 constexpr uint32_t kExSizes = 4;
 struct ExSizes { uint32_t n[kExSizes]; };
-__device__ __forceinline__ ExSizes ex_sizes(uint32_t n, uint32_t rows) {
+__device__ __forceinline__ ExSizes ex_sizes(uint32_t n, const ExCut &cut) {
     ExSizes of{};
-    if (rows) {
-        of.n[0] = ex_tiles(n, rows);
+    if (cut.rows) {
+        of.n[0] = cut.tiles(n);
     } else if (n) {
-        const uint32_t tiles = ex_tiles(n, 0), each = ex_eights(n) / tiles, longer = ex_eights(n) - each * tiles;
+        const uint32_t tiles = cut.tiles(n), each = cut.layers(n) / tiles, longer = cut.layers(n) - each * tiles;
 #pragma unroll
         for (uint32_t k = 0; k < kExSizes; ++k) of.n[k] = each == 4u - k ? tiles - longer : each + 1u == 4u - k ? longer : 0u;
     }
     return of;
 }
-__device__ __forceinline__ uint32_t ex_places(uint32_t n, uint32_t rows) { return rows ? n : (n + 15u) & ~15u; }
 
 __global__ void __launch_bounds__(kExPlanThreads)
-k_experts_plan(const int32_t *__restrict__ ids, uint32_t slots, uint32_t experts, uint32_t rows, ExPlan plan) {
+k_experts_plan(const int32_t *__restrict__ ids, uint32_t slots, uint32_t experts, ExCut cut, ExPlan plan) {
     __shared__ uint32_t hist[kExMostExperts], of_wave[kExPlanWaves], sums[1u + kExSizes][kExPlanWaves];
     const uint32_t tid = threadIdx.x, lane = tid & 63u, wave = tid >> 6, e = blockIdx.x;
     for (uint32_t i = tid; i < experts; i += kExPlanThreads) hist[i] = 0;
@@ -64,8 +68,8 @@ k_experts_plan(const int32_t *__restrict__ ids, uint32_t slots, uint32_t experts
     // in front of this expert: places, and, of each size, tiles; with them all tiles of larger sizes
     uint32_t sum[1u + kExSizes] = {};
     for (uint32_t i = tid; i < experts; i += kExPlanThreads) {
-        const ExSizes of = ex_sizes(hist[i], rows);
-        if (i < e) sum[0] += ex_places(hist[i], rows);
+        const ExSizes of = ex_sizes(hist[i], cut);
+        if (i < e) sum[0] += cut.places(hist[i]);
 #pragma unroll
         for (uint32_t k = 0; k < kExSizes; ++k) {
             uint32_t larger = 0;
@@ -85,25 +89,25 @@ k_experts_plan(const int32_t *__restrict__ ids, uint32_t slots, uint32_t experts
         sum[k] = 0;
         for (uint32_t w = 0; w < kExPlanWaves; ++w) sum[k] += sums[k][w];
     }
-    const uint32_t before = sum[0], n = hist[e], n_tiles = ex_tiles(n, rows), places = ex_places(n, rows);
-    const ExSizes own_sizes = ex_sizes(n, rows);
+    const uint32_t before = sum[0], n = hist[e], n_tiles = cut.tiles(n), places = cut.places(n);
+    const ExSizes own_sizes = ex_sizes(n, cut);
     for (uint32_t i = tid; i < n_tiles; i += kExPlanThreads) {
-        if (rows) {
+        if (cut.rows) {
             uint32_t *const t = plan.tiles + 3u * (sum[1] + i);
-            t[0] = e, t[1] = before + i * rows, t[2] = min(rows, n - i * rows);
+            t[0] = e, t[1] = before + i * cut.rows, t[2] = min(cut.rows, n - i * cut.rows);
         } else {  // the longer ones of an expert's tiles come first
-            const uint32_t eights = ex_eights(n), each = eights / n_tiles, longer = eights - each * n_tiles;
-            const uint32_t b0 = (i * each + min(i, longer)) * 8u, size = each + (i < longer);
+            const uint32_t layers = cut.layers(n), each = layers / n_tiles, longer = layers - each * n_tiles;
+            const uint32_t b0 = (i * each + min(i, longer)) * (kExLayer / 16u), size = each + (i < longer);
             uint32_t at = i < longer ? i : i - longer;
 #pragma unroll
             for (uint32_t k = 0; k < kExSizes; ++k) at += size == 4u - k ? sum[1u + k] : 0u;
             uint32_t *const t = plan.tiles + 3u * at;
-            t[0] = e, t[1] = before / 16u + b0, t[2] = min(size * 8u, places / 16u - b0);
+            t[0] = e, t[1] = before / 16u + b0, t[2] = min(size * (kExLayer / 16u), places / 16u - b0);
         }
     }
     for (uint32_t i = n + tid; i < places; i += kExPlanThreads) plan.order[before + i] = ~0u;
     if (e + 1u == experts && tid == 0) {
-        *plan.n_tiles = rows ? sum[1] + n_tiles : sum[kExSizes] + own_sizes.n[kExSizes - 1u];  // (in front of this one: all larger ones, and all others')
+        *plan.n_tiles = cut.rows ? sum[1] + n_tiles : sum[kExSizes] + own_sizes.n[kExSizes - 1u];  // (in front of this one: all larger ones, and all others')
         *plan.n_blocks = (before + places) / 16u;
     }
     uint32_t at = before;
@@ -535,10 +539,10 @@ template <bool FIRST> static int ex_matrix(const ExMatrix &W, const ExRows &R, u
     }
 }
 
-// Many tokens to an expert: 20 and more in the mean (us of a call, k_experts_rows / k_experts_prompt at 16, 24 and 32: 64 experts of 2048 x 1024
-// at 5 % listed 207 / 226, 299 / 230, 359 / 232, next to none listed 149 / 196, 224 / 198, 270 / 202; 16 of 4096 x 1536 130 / 168, 161 / 171, 207 / 175;
-// 20 of 1400 x 744 71 / 100, 81 / 100, 94 / 102).
-constexpr uint32_t kExMany = 20;
+// Many tokens to an expert: 11 and more in the mean (us of a call, k_experts_rows with 8 / 12 / 16 tokens each, and k_experts_prompt with 24,
+// whose time hardly hangs on that up to 64: 64 experts of 2048 x 1024 at 5 % listed 138 / 179 / 207, 171; next to none listed 102 / 129 / 149, 138;
+// 16 of 4096 x 1536 93 / 111 / 130, 101; 20 of 1400 x 744 60 / 67 / 71, 62).
+constexpr uint32_t kExMany = 11;
 // (Rows of up to 2^20 columns: offsets within a tile's rows are 32 bits.)
 static bool ex_many(const ExDev &X, uint32_t slots) {
     return slots >= kExMany * X.experts && std::max(X.first.n_cells, X.second.n_cells) <= 2048u;
@@ -547,7 +551,7 @@ static bool ex_many(const ExDev &X, uint32_t slots) {
 // A call's scratch: the plan, the intermediate, what each slot's expert makes of it, and in k_experts_prompt the gathered rows.
 struct ExScratch {
     bool many;
-    uint32_t rows, n_tiles, blocks;  // slots of a tile (0: see ExPlan); tiles and blocks at most
+    uint32_t rows, n_tiles, blocks;  // as ExCut; tiles and blocks at most
     size_t tiles, order, x, inner, per_slot, bytes;
     int64_t ld_inner;
 };
@@ -558,7 +562,7 @@ static ExScratch ex_scratch(const ExDev &X, uint32_t tokens, uint32_t top_k) {
     size_t at = 256;
     auto take = [&](size_t n) { const size_t from = at; at += (n + 255u) & ~(size_t)255u; return from; };
     if (w.many) {
-        w.n_tiles = std::min(slots, X.experts) + slots / 512u;
+        w.n_tiles = std::min(slots, X.experts) + slots / (4u * kExLayer);
         w.blocks = std::min(slots, X.experts) + slots / 16u;
         w.tiles = take((size_t)w.n_tiles * 12u);
         w.order = take((size_t)w.blocks * 64u);
@@ -593,7 +597,7 @@ int launch_experts(const ExDev &X, const ExCall &call, void *workspace, hipStrea
     uint32_t *const counts = reinterpret_cast<uint32_t *>(ws);
     const ExPlan plan{counts, counts + 1, reinterpret_cast<uint32_t *>(ws + w.tiles), reinterpret_cast<uint32_t *>(ws + w.order)};
     float *const per_slot = reinterpret_cast<float *>(ws + w.per_slot);
-    if (planned) IXH_LAUNCH(k_experts_plan, dim3(X.experts), dim3(kExPlanThreads), 0, s, call.ids, slots, X.experts, w.rows, plan);
+    if (planned) IXH_LAUNCH(k_experts_plan, dim3(X.experts), dim3(kExPlanThreads), 0, s, call.ids, slots, X.experts, ExCut{w.rows}, plan);
     int rc;
     if (w.many) {
         rc = launch_experts_prompt(X, call, plan, n_tiles, w.blocks, ws + w.x, ws + w.inner, per_slot, s);

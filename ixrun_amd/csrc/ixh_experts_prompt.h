@@ -6,16 +6,16 @@
 
 namespace ixh {
 
-constexpr uint32_t kEpWaves = 8, kEpThreads = kEpWaves * kWave;
+constexpr uint32_t kEpWaves = 4, kEpThreads = kEpWaves * kWave;
 constexpr uint32_t kEpRows = 16u * kEpWaves;       // weight rows of a workgroup
-constexpr uint32_t kEpTile = kEpRows * 128u * 2u;  // bytes of a stage's weights: 128 rows x 128 columns
+constexpr uint32_t kEpTile = kEpRows * 128u * 2u;  // bytes of a stage's weights: 64 rows x 128 columns
 constexpr uint32_t kEpRounds = 3;                  // groups of 16 quads of a cell's list that a wave holds
 constexpr uint32_t kEpNone = ~0u;
 
 struct EpCall {
     const ln_u32x4 *xt;       // the rows in operand order
     const uint32_t *n_tiles;  // row tiles
-    const uint32_t *tiles;    // {expert, first block, blocks} each, up to 32 blocks of 16 rows
+    const uint32_t *tiles;    // {expert, first block, blocks} each, up to four blocks of 16 rows to each wave
     const uint32_t *order;    // slots of the blocks' rows, or kEpNone
     uint8_t *inner;           // FIRST: the other matrix's rows in operand order
     float *out;               // else: what each slot's expert makes of it
@@ -25,28 +25,31 @@ struct EpCall {
 };
 
 // ---------------------------------------------------------------------------------------------------------------
-// k_experts_prompt<BITS, FIRST>: a tile of up to 512 rows of one expert by 128 weight rows.
+// k_experts_prompt<BITS, FIRST>: a tile of up to 256 rows of one expert by 64 weight rows.
 //
-// Eight waves decode 128 weight rows x 128 columns a stage to LDS in operand order, 16 rows each, while they multiply the stage before;
-// the activations come from the L2 straight to registers as operands.  A wave has MI blocks of 16 rows, MI = 2 .. 4 by the tile's, and all
-// 128 weight rows.  (Up to 128 rows half of the waves, one a SIMD, have two blocks and the others only decode: as many products a SIMD
-// as with a block a wave, and half the reads of weights.)  The tiles of one expert's rows run on one XCD, whose L2 holds them.
+// Four waves decode 64 weight rows x 128 columns a stage to LDS in operand order, 16 rows each, while they multiply the stage before; the
+// activations come from the L2 straight to registers as operands.  A wave has MI blocks of 16 rows, MI = 1 .. 4 by the tile's, and all 64
+// weight rows.  The tiles of one expert's rows run on one XCD, whose L2 holds them.
+//
+// Bound: a stage's waits (codes and lists from memory, look-ups, barriers), until products of three and more blocks a wave cover them.
+// Three workgroups to a CU, by registers (168) and LDS (53 KB with the smaller pair table), fill in for one another; one of eight waves
+// with 128 weight rows, up to 512 rows and the larger table, as in k_lanes_prompt, decodes a weight half as often and waits alone: us of
+// a call, eight / four waves, 64 experts of 2048 x 1024 at 5 % listed with 24, 64, 128, 200, 400, 600 tokens each 238 / 171, 252 / 191, 308 / 249,
+// 386 / 324, 566 / 550, 760 / 778, 16 of 4096 x 1536 with next to none 172 / 101, 197 / 120, 220 / 189, 284 / 239, 404 / 390, 505 / 506.
 // ---------------------------------------------------------------------------------------------------------------
 template <int BITS, int MI, bool FIRST>
 __device__ __forceinline__ void ep_tile(const ExMatrix &W, const EpCall &R, uint32_t e, uint32_t block0, uint32_t n_blocks, uint32_t tile,
                                         uint8_t *ep_smem) {
-    using P = LnPairs<BITS, true>;
-    constexpr uint32_t NI = 8;
-    constexpr uint32_t AHEAD = MI == 2 ? 8 : MI == 3 ? 4 : 2;  // steps of 32 columns that the activations' operands are asked for ahead
-    constexpr uint32_t CODES = MI == 4 ? 1 : 2;  // stages that the codes are asked for ahead of their decode
-    constexpr bool FLOAT = MI != 4;
+    using P = LnPairs<BITS, false>;
+    constexpr uint32_t NI = kEpWaves;
+    constexpr uint32_t AHEAD = MI == 1 ? 8 : MI == 2 ? 4 : 2;  // steps of 32 columns that the activations' operands are asked for ahead
+    constexpr uint32_t CODES = 2;  // stages that the codes are asked for ahead of their decode
     const uint32_t smem = (uint32_t)(uintptr_t)(LN_LDS(uint8_t) *)ep_smem;
     const uint32_t tid = threadIdx.x, lane = tid & 63u, n = lane & 15u, kg = lane >> 4;
     const uint32_t wave = (uint32_t)__builtin_amdgcn_readfirstlane((int)(tid >> 6));
     const uint32_t n_cells = W.n_cells, n_tiles = W.n_tiles, n_kb = n_cells * 16u;
     const uint32_t mb0 = wave * MI;  // the wave's first block of rows, in the tile
     const float scale = bf16_bits_to_f32(W.scale[e]);
-    if constexpr (MI == 4) ln_build_lut<BITS, true>(smem, scale, tid, kEpThreads);
 
     // ---- the wave's part of the decode: block `wave` of the workgroup's eight, lane (n, kg) the codes of row n ----
     const uint32_t *const exc_off = W.exc_off + (size_t)e * (n_tiles * n_cells + 1u);
@@ -120,7 +123,7 @@ __device__ __forceinline__ void ep_tile(const ExMatrix &W, const EpCall &R, uint
     };
 #pragma unroll
     for (uint32_t t = 0; t < AHEAD; ++t) x_load(0u, t);
-    if constexpr (MI != 4) ln_build_lut<BITS, true>(smem, scale, tid, kEpThreads);
+    ln_build_lut<BITS, false>(smem, scale, tid, kEpThreads);
     asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
 
     const uint32_t lut_lane = smem + ((lane & ((1u << P::kCopies) - 1u)) << 2);
@@ -164,7 +167,7 @@ __device__ __forceinline__ void ep_tile(const ExMatrix &W, const EpCall &R, uint
     auto store = [&](uint32_t q) {  // stage q of the cell, to its half of the tile
         const uint32_t base = store_at + (q & 1u) * kEpTile;
         uint32_t o[16];
-        ln_decode<BITS, true, FLOAT>(w[q % CODES], lut_lane, scale, o);
+        ln_decode<BITS, false>(w[q % CODES], lut_lane, scale, o);
 #pragma unroll
         for (uint32_t k = 0; k < 4; ++k)
             *reinterpret_cast<LN_LDS(ln_u32x4) *>((uintptr_t)(base + ((k ^ q) << 10) + lane * 16u)) =
@@ -177,19 +180,13 @@ __device__ __forceinline__ void ep_tile(const ExMatrix &W, const EpCall &R, uint
         for (uint32_t r = 0; r < kEpRounds; ++r)
             if (BITS == 8 ? any[r] : (in_stage[r] & (1u << q)) != 0) {
                 const ln_u32x4 put = put_at[r];
-                if constexpr (MI == 4) {
+                // (elements of other stages go aside, a dword a lane)
+                const Place me = place();
+                const uint32_t aside = smem + P::kLutBytes + 2u * kEpTile + kEpThreads * (16u * kEpRounds) + (me.kg * 16u + me.quad + me.row) * 4u;
 #pragma unroll
-                    for (uint32_t k = 0; k < 4; ++k)
-                        if ((put[k] & 0x7000u) == (q << 12))
-                            *reinterpret_cast<LN_LDS(uint16_t) *>((uintptr_t)(base + (put[k] & 0xFFFu))) = (uint16_t)(put[k] >> 16);
-                } else {  // (elements of other stages go aside, a dword a lane)
-                    const Place me = place();
-                    const uint32_t aside = smem + P::kLutBytes + 2u * kEpTile + kEpThreads * (16u * kEpRounds) + (me.kg * 16u + me.quad + me.row) * 4u;
-#pragma unroll
-                    for (uint32_t k = 0; k < 4; ++k) {
-                        const uint32_t to = (put[k] ^ (q << 12)) & 0x7FFFu;
-                        *reinterpret_cast<LN_LDS(uint16_t) *>((uintptr_t)(to < 4096u ? base + to : aside)) = (uint16_t)(put[k] >> 16);
-                    }
+                for (uint32_t k = 0; k < 4; ++k) {
+                    const uint32_t to = (put[k] ^ (q << 12)) & 0x7FFFu;
+                    *reinterpret_cast<LN_LDS(uint16_t) *>((uintptr_t)(to < 4096u ? base + to : aside)) = (uint16_t)(put[k] >> 16);
                 }
             }
         if (more) {  // rows with yet more listed elements in the cell
@@ -219,7 +216,7 @@ __device__ __forceinline__ void ep_tile(const ExMatrix &W, const EpCall &R, uint
             const uint32_t c_next = min(c + 1u, n_cells - 1u);
 #pragma unroll
             for (uint32_t q = 0; q < 4; ++q) {
-                if (q == (MI >= 3 ? 2u : 1u)) list = quads(e_now);
+                if (q == 1) list = quads(e_now);
                 if (q == 3) take_list(c + 1u);
                 store((q + 1u) & 3u);
                 patch((q + 1u) & 3u);
@@ -256,7 +253,7 @@ __device__ __forceinline__ void ep_tile(const ExMatrix &W, const EpCall &R, uint
                     if (j == 0) {
                         if (b && b * PER % 4 == 0) piece(b * PER / 4 - 1);
                         uint32_t d[16];
-                        ln_decode<BITS, true, FLOAT>(w[p % CODES], lut_lane, scale, d);
+                        ln_decode<BITS, false>(w[p % CODES], lut_lane, scale, d);
 #pragma unroll
                         for (uint32_t k = b * PER; k < b * PER + PER; ++k) o[k] = d[k];
                         __builtin_amdgcn_sched_barrier(0);
@@ -265,13 +262,13 @@ __device__ __forceinline__ void ep_tile(const ExMatrix &W, const EpCall &R, uint
                     for (uint32_t i = 0; i < MI; ++i)
                         acc[i][b] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(ln_bf16x8, v[b & 1u]),
                                                                             __builtin_bit_cast(ln_bf16x8, a[t % AHEAD][i]), acc[i][b], 0, 0, 0);
-                    if (MI != 4 || BITS == 8 || j == 0) __builtin_amdgcn_sched_barrier(0);
+                    __builtin_amdgcn_sched_barrier(0);
                 }
                 if (j == 0) piece(3);
                 x_load(t + AHEAD < 16u ? c : c_next, (t + AHEAD) & 15u);
                 __builtin_amdgcn_sched_barrier(0);
             };
-            if (q == (MI >= 3 ? 2u : 1u)) list = quads(e_now);
+            if (q == 1) list = quads(e_now);
             if (q == 3) {
                 take_list(c + 1u);
                 __builtin_amdgcn_sched_barrier(0);
@@ -329,7 +326,7 @@ __device__ __forceinline__ void ep_tile(const ExMatrix &W, const EpCall &R, uint
         }
         // columns of the intermediate's last cell that no weight row makes: zeros
         if (tile + 1u == R.w_tiles) {
-            const uint32_t from = R.w_tiles * (R.gated ? 64u : 128u) / 32u;
+            const uint32_t from = R.w_tiles * (kEpRows / per) / 32u;
             for (uint32_t i = 0; i < MI && mb0 + i < n_blocks; ++i)
                 for (uint32_t kb = from; kb < R.n_kb_inner; ++kb)
                     reinterpret_cast<ln_u32x4 *>(R.inner)[((size_t)(block0 + mb0 + i) * R.n_kb_inner + kb) * 64u + lane] = ln_u32x4{0u, 0u, 0u, 0u};
@@ -362,24 +359,26 @@ __device__ __forceinline__ void ep_tile(const ExMatrix &W, const EpCall &R, uint
 }
 
 template <int BITS, bool FIRST>
-__global__ void __launch_bounds__(kEpThreads) __attribute__((amdgpu_waves_per_eu(2, 2)))
+__global__ void __launch_bounds__(kEpThreads) __attribute__((amdgpu_waves_per_eu(3)))
 k_experts_prompt(ExMatrix W, EpCall R) {
     extern __shared__ __attribute__((aligned(16))) uint8_t ep_smem[];
     // workgroups go round the eight XCDs: all weight tiles of a row tile to one of them
     const uint32_t id = blockIdx.x, turn = id >> 3, row_tile = (turn / R.w_tiles) * 8u + (id & 7u), tile = turn % R.w_tiles;
     if (row_tile >= *R.n_tiles) return;
     const uint32_t e = R.tiles[3u * row_tile], block0 = R.tiles[3u * row_tile + 1u], n_blocks = R.tiles[3u * row_tile + 2u];
-    if (n_blocks <= 16u) ep_tile<BITS, 2, FIRST>(W, R, e, block0, n_blocks, tile, ep_smem);
-    else if (n_blocks <= 24u) ep_tile<BITS, 3, FIRST>(W, R, e, block0, n_blocks, tile, ep_smem);
+    if (n_blocks <= kEpWaves) ep_tile<BITS, 1, FIRST>(W, R, e, block0, n_blocks, tile, ep_smem);
+    else if (n_blocks <= 2u * kEpWaves) ep_tile<BITS, 2, FIRST>(W, R, e, block0, n_blocks, tile, ep_smem);
+    else if (n_blocks <= 3u * kEpWaves) ep_tile<BITS, 3, FIRST>(W, R, e, block0, n_blocks, tile, ep_smem);
     else ep_tile<BITS, 4, FIRST>(W, R, e, block0, n_blocks, tile, ep_smem);
 }
 
-template <int BITS, bool FIRST> int ep_launch(const ExMatrix &W, const EpCall &R, uint32_t row_tiles, hipStream_t s) {
-    constexpr size_t lds = LnPairs<BITS, true>::kLutBytes + 2u * kEpTile + 16u * kEpRounds * kEpThreads + kWave * 4u;
-    static_assert(lds <= kLnLds, "LDS of a CU");
+template <int BITS, bool FIRST> int ep_launch(const ExMatrix &W, EpCall R, uint32_t row_tiles, hipStream_t s) {
+    constexpr size_t lds = LnPairs<BITS, false>::kLutBytes + 2u * kEpTile + 16u * kEpRounds * kEpThreads + kWave * 4u;
+    static_assert(3u * lds <= kLnLds, "LDS of a CU");
     static const bool raised = hipFuncSetAttribute(reinterpret_cast<const void *>(k_experts_prompt<BITS, FIRST>),
                                                    hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds) == hipSuccess;
     if (!raised) return IXH_ELAUNCH;
+    R.w_tiles = (W.n_tiles * 4u + kEpRows - 1u) / kEpRows;
     IXH_LAUNCH((k_experts_prompt<BITS, FIRST>), dim3((row_tiles + 7u) / 8u * 8u * R.w_tiles), dim3(kEpThreads), lds, s, W, R);
     return hipGetLastError() == hipSuccess ? IXH_OK : IXH_ELAUNCH;
 }
@@ -391,7 +390,7 @@ template <bool FIRST> int ep_matrix(const ExMatrix &W, const EpCall &R, uint32_t
         default: return ep_launch<8, FIRST>(W, R, row_tiles, s);
     }
 }
-// (a source file each: they take the compiler a minute)
+// (a source file each: they take the compiler a while)
 int ep_first(const ExMatrix &W, const EpCall &R, uint32_t row_tiles, hipStream_t s);
 int ep_second(const ExMatrix &W, const EpCall &R, uint32_t row_tiles, hipStream_t s);
 

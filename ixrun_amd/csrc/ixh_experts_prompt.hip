@@ -42,10 +42,9 @@ int launch_experts_prompt(const ExDev &X, const ExCall &call, const ExPlan &plan
     const bool whole = ((uintptr_t)call.x & 15u) == 0 && call.ldx % 8 == 0 && X.hidden % 8u == 0;
     IXH_LAUNCH(k_experts_xtile, dim3(blocks, std::min((n_kb + 15u) / 16u, 16u)), dim3(256), 0, s, call.x, call.ldx, call.top_k, X.hidden, n_kb, whole,
                plan.n_blocks, plan.order, static_cast<ln_u32x4 *>(xt));
-    R.w_tiles = (X.first.n_tiles * 4u + kEpRows - 1u) / kEpRows;
     int rc = ep_first(X.first, R, row_tiles, s);
     if (rc != IXH_OK) return rc;
-    R.xt = static_cast<const ln_u32x4 *>(inner), R.out = per_slot, R.w_tiles = (X.second.n_tiles * 4u + kEpRows - 1u) / kEpRows;
+    R.xt = static_cast<const ln_u32x4 *>(inner), R.out = per_slot;
     return ep_second(X.second, R, row_tiles, s);
 }
 

@@ -18,14 +18,39 @@ template <int CTRL> __device__ __forceinline__ uint64_t rt_dpp(uint64_t v) {
 template <int CTRL> __device__ __forceinline__ double rt_dpp(double v) {
     return __builtin_bit_cast(double, rt_dpp<CTRL>(__builtin_bit_cast(uint64_t, v)));
 }
+// a value of the lane and of the one 16 or 32 further, in either order
+template <class V> struct RtTwo { V a, b; };
+template <int BY> __device__ __forceinline__ RtTwo<uint32_t> rt_swapped(uint32_t v) {
+    if constexpr (BY == 16) {
+        const auto h = __builtin_amdgcn_permlane16_swap(v, v, false, false);
+        return {h[0], h[1]};
+    } else {
+        const auto h = __builtin_amdgcn_permlane32_swap(v, v, false, false);
+        return {h[0], h[1]};
+    }
+}
+template <int BY> __device__ __forceinline__ RtTwo<uint64_t> rt_swapped(uint64_t v) {
+    const auto lo = rt_swapped<BY>((uint32_t)v), hi = rt_swapped<BY>((uint32_t)(v >> 32));
+    return {(uint64_t)hi.a << 32 | lo.a, (uint64_t)hi.b << 32 | lo.b};
+}
+template <int BY> __device__ __forceinline__ RtTwo<float> rt_swapped(float v) {
+    const auto h = rt_swapped<BY>(__float_as_uint(v));
+    return {__uint_as_float(h.a), __uint_as_float(h.b)};
+}
+template <int BY> __device__ __forceinline__ RtTwo<double> rt_swapped(double v) {
+    const auto h = rt_swapped<BY>(__builtin_bit_cast(uint64_t, v));
+    return {__builtin_bit_cast(double, h.a), __builtin_bit_cast(double, h.b)};
+}
 template <int LT, class V, class F> __device__ __forceinline__ V rt_all(V v, F f) {
     v = f(v, rt_dpp<0xB1>(v));   // quad_perm 1, 0, 3, 2
     v = f(v, rt_dpp<0x4E>(v));   // quad_perm 2, 3, 0, 1
     v = f(v, rt_dpp<0x141>(v));  // row_half_mirror
     v = f(v, rt_dpp<0x140>(v));  // row_mirror
     if constexpr (LT == 64) {
-        v = f(v, (V)__shfl_xor(v, 16));
-        v = f(v, (V)__shfl_xor(v, 32));
+        const auto rows = rt_swapped<16>(v);
+        v = f(rows.a, rows.b);
+        const auto halves = rt_swapped<32>(v);
+        v = f(halves.a, halves.b);
     }
     return v;
 }
@@ -128,6 +153,7 @@ k_route(const T *__restrict__ logits, int64_t ld, uint32_t tokens, RouteDev R, c
         __builtin_amdgcn_wave_barrier();
         for (uint32_t g = l; g < R.groups; g += LT) {
             Key best = 0, second = 0;
+#pragma unroll 4
             for (uint32_t i = 0; i < R.group_size; ++i) {
                 const Key c = mine[g * R.group_size + i];
                 second = c > best ? best : c > second ? c : second;
