@@ -59,6 +59,21 @@ struct ExPlan {
 int launch_experts_prompt(const ExDev &X, const ExCall &call, const ExPlan &plan, uint32_t row_tiles, uint32_t blocks, void *xt, void *inner,
                           float *per_slot, hipStream_t s);
 
+// a slot by itself (ixh_experts_one.hip): rows of up to sixteen cells, eight of a gated first matrix
+struct ExOne {
+    const uint16_t *x;
+    int64_t ldx;
+    uint32_t rows;  // of x
+    const int32_t *ids;
+    void *out;  // the intermediate in bf16, or fp32
+    int64_t ld_out;
+    uint32_t experts, tokens, top_k;
+    int activation;
+    bool gated;
+};
+bool experts_one_takes(const ExMatrix &W, bool gated);
+int launch_experts_one(const ExMatrix &W, const ExOne &R, bool first, hipStream_t s);
+
 size_t experts_workspace_bytes(const ExDev &X, uint32_t tokens, uint32_t top_k);
 int launch_experts(const ExDev &X, const ExCall &call, void *workspace, hipStream_t s);
 

@@ -1,0 +1,193 @@
+// The experts' products of single tokens: each slot (token, j) by itself.
+#include <algorithm>
+
+#include "ixh_epilogue.h"
+#include "ixh_experts.h"
+#include "ixh_lanes_dev.h"
+
+namespace ixh {
+
+// ---------------------------------------------------------------------------------------------------------------
+// k_experts_one<BITS, FIRST>: one slot by a run of blocks of 16 weight rows, a wave for each cell (16 rows x 512 columns).
+//
+// Bound: a launch, one chain of requests (the expert's id, then its codes, the extents of their lists, scale and activations at once, then the
+// lists) and the instructions of a cell.  Products and listed elements as in k_experts_rows, of whose kernel for one row some 350 of 1100
+// instructions a wave only find its share: one token by 6 experts of 2048 x 1024, 25 MB of codes and lists, first / second matrix 13.2 / 9.6 us
+// there, 9.1 / 6.9 us here (1.6 TB/s with their starts and ends).
+// ---------------------------------------------------------------------------------------------------------------
+template <int BITS, bool FIRST>
+__global__ void __launch_bounds__(1024)
+k_experts_one(const int32_t *__restrict__ ids, const uint32_t *__restrict__ plane, const uint16_t *__restrict__ x, const uint32_t *__restrict__ exc_off,
+              const uint16_t *__restrict__ scale_at, uint32_t shape, uint32_t n_tiles, uint32_t plane_words, uint32_t experts, uint32_t in_f, int64_t ldx,
+              const uint16_t *__restrict__ exc_pos, const int8_t *__restrict__ exc_val, const uint16_t *__restrict__ bias, void *__restrict__ out,
+              int64_t ld_out, uint32_t outputs, int activation) {
+    extern __shared__ __attribute__((aligned(16))) uint8_t eo_smem[];
+    using P = LnPairs<BITS, false>;
+    const uint32_t smem = (uint32_t)(uintptr_t)(LN_LDS(uint8_t) *)eo_smem;
+    // blocks: row quads from 4 b0 on, all blocks' cells to a wave each
+    const uint32_t C = shape & 31u, blocks = (shape >> 5) & 31u, inv_cells = shape >> 12;
+    const bool gated = (shape >> 10) & 1u, whole = (shape >> 11) & 1u;
+    const uint32_t slot = blockIdx.z * gridDim.y + blockIdx.y, e = (uint32_t)ids[slot];
+    if (e >= experts) return;
+    const uint32_t tid = threadIdx.x, lane = tid & 63u, n = lane & 15u, kg = lane >> 4, n_threads = blocks * C * kWave;
+    const uint32_t wave = (uint32_t)__builtin_amdgcn_readfirstlane((int)(tid >> 6));
+    const uint32_t b0 = blockIdx.x * blocks, b = (wave * inv_cells) >> 16, c = wave - b * C;
+
+    // ---- all requests ----
+    const uint32_t scale_raw = scale_at[e];
+    constexpr uint32_t kCell = 256u * BITS, kLane = BITS == 3 ? 12u : 16u;
+    const __amdgpu_buffer_rsrc_t codes_rs = __builtin_amdgcn_make_buffer_rsrc((void *)(plane + (size_t)e * plane_words), 0, (int)(plane_words * 4u), 0x00020000);
+    const uint32_t quad = 4u * (b0 + b), in_cell = 4u * kg + (n & 3u), codes = min(quad + (n >> 2), n_tiles - 1u) * (C * kCell) + in_cell * kLane;
+    uint32_t w[4][BITS];
+#pragma unroll
+    for (uint32_t q = 0; q < 4; ++q) {
+        uint32_t(&d)[BITS] = w[q];
+        if constexpr (BITS == 3) {
+            const ln_u32x3 v = __builtin_bit_cast(ln_u32x3, __builtin_amdgcn_raw_buffer_load_b96(codes_rs, (int)(codes + q * 192u), (int)(c * kCell), 0));
+            d[0] = v[0]; d[1] = v[1]; d[2] = v[2];
+        } else {
+            const ln_u32x4 v = __builtin_bit_cast(ln_u32x4, __builtin_amdgcn_raw_buffer_load_b128(codes_rs, (int)(codes + q * 256u), (int)(c * kCell), 0));
+            d[0] = v[0]; d[1] = v[1]; d[2] = v[2]; d[3] = v[3];
+            if constexpr (BITS == 5)
+                d[4] = __builtin_amdgcn_raw_buffer_load_b32(codes_rs, (int)(codes - 12u * in_cell + (1024u + q * 64u)), (int)(c * kCell), 0);
+            if constexpr (BITS == 8) {
+                const ln_u32x4 u = __builtin_bit_cast(ln_u32x4, __builtin_amdgcn_raw_buffer_load_b128(codes_rs, (int)(codes + (1024u + q * 256u)), (int)(c * kCell), 0));
+                d[4] = u[0]; d[5] = u[1]; d[6] = u[2]; d[7] = u[3];
+            }
+        }
+    }
+    const uint32_t *const off = exc_off + (size_t)e * (n_tiles * C + 1u) + (min(quad + kg, n_tiles - 1u) * C + c);
+    const uint32_t l0 = off[0], l1 = quad + kg < n_tiles ? off[1] : l0;
+    // a piece of eight columns a thread: there are as many threads as pieces, or more
+    const uint16_t *const row = x + (int64_t)(FIRST ? blockIdx.z : slot) * ldx;
+    const uint32_t col = tid * 8u;
+    ln_u32x4 piece = {0u, 0u, 0u, 0u};
+    if (whole) {
+        piece = *reinterpret_cast<const ln_u32x4 *>(row + min(col, in_f - 8u));
+    } else {
+        uint32_t h[8];
+#pragma unroll
+        for (uint32_t k = 0; k < 8; ++k) h[k] = row[min(col + k, in_f - 1u)];
+#pragma unroll
+        for (uint32_t k = 0; k < 4; ++k) piece[k] = (col + 2u * k < in_f ? h[2 * k] : 0u) | (col + 2u * k + 1u < in_f ? h[2 * k + 1] << 16 : 0u);
+    }
+    struct Group { ln_u32x2 pos; uint32_t val; };
+    auto quad_of = [&](uint32_t i) { return (l0 & ~3u) + 16u * i + (n & ~3u); };
+    auto g_load = [&](uint32_t i) {
+        const uint32_t q = quad_of(i), at = q < l1 ? lane_listed(q, n & 3u) : 0u;
+        return Group{*reinterpret_cast<const ln_u32x2 *>(exc_pos + at), *reinterpret_cast<const uint32_t *>(exc_val + at)};
+    };
+    Group list[2];
+#pragma unroll
+    for (uint32_t i = 0; i < 2; ++i) list[i] = g_load(i);
+    __builtin_amdgcn_sched_barrier(0);
+
+    // ---- pair table and activations to LDS ----
+    const float scale = bf16_bits_to_f32(scale_raw);
+    ln_build_lut<BITS, false>(smem, scale, tid, n_threads);
+    const uint32_t x_at = smem + P::kLutBytes, x_none = C * 1024u;
+    float *const parts = reinterpret_cast<float *>(eo_smem + P::kLutBytes + x_none + 64u);  // [wave][16]
+    if (tid < C * 64u) {
+        if (whole && col >= in_f) piece = ln_u32x4{0u, 0u, 0u, 0u};
+        *reinterpret_cast<LN_LDS(ln_u32x4) *>((uintptr_t)(x_at + lane_offset(col))) = piece;
+    }
+    if (tid < 4u) *reinterpret_cast<LN_LDS(ln_u32x4) *>((uintptr_t)(x_at + x_none + tid * 16u)) = ln_u32x4{0u, 0u, 0u, 0u};
+    asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+
+    // ---- the cell's products: the row's activations in all sixteen columns (columns 128 q + 32 i of a cell lie at 128 q + 32 (i ^ q)) ----
+    const uint32_t lut_lane = smem + ((lane & ((1u << P::kCopies) - 1u)) << 2), x_cell = x_at + c * 1024u + kg * 16u;
+    ln_f32x4 acc = {0, 0, 0, 0};
+#pragma unroll
+    for (uint32_t q = 0; q < 4; ++q) {
+        uint32_t o[16];
+        ln_decode<BITS, false>(w[q], lut_lane, scale, o);
+#pragma unroll
+        for (uint32_t i = 0; i < 4; ++i) {
+            const ln_u32x4 a = *reinterpret_cast<const LN_LDS(ln_u32x4) *>((uintptr_t)(x_cell + q * 256u + ((q ^ i) << 6)));
+            acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(ln_bf16x8, ln_u32x4{o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]}),
+                                                          __builtin_bit_cast(ln_bf16x8, a), acc, 0, 0, 0);
+        }
+    }
+    // ---- its listed elements ----
+    float ex = 0.0f;
+    const uint32_t scale_bits = __float_as_uint(scale) & 0x7FFFFFFFu;
+    auto listed = [&](const Group &g, uint32_t i) {
+        const uint32_t q = quad_of(i) - l0;
+        const uint32_t w01 = ln_pack((float)(int)(int8_t)g.val * scale, (float)(int)(int8_t)(g.val >> 8) * scale);
+        const uint32_t w23 = ln_pack((float)(int)(int8_t)(g.val >> 16) * scale, (float)((int)g.val >> 24) * scale);
+#pragma unroll
+        for (uint32_t k = 0; k < 4; ++k) {
+            const uint32_t p = k & 1 ? g.pos[k >> 1] >> 16 : g.pos[k >> 1] & 0xFFFFu;  // (rows of up to 16 cells: places without an element have one of their own)
+            const uint32_t h = *reinterpret_cast<const LN_LDS(uint16_t) *>((uintptr_t)(x_at + (q + k < l1 - l0 ? p : x_none)));
+            const uint32_t wk = k & 2 ? w23 : w01, wbits = k & 1 ? wk & 0xFFFF0000u : wk << 16;
+            ex = __fmaf_rn(__uint_as_float(wbits) - __uint_as_float((wbits & 0x80000000u) | scale_bits), __uint_as_float(h << 16), ex);
+        }
+    };
+    const uint32_t groups = l1 > l0 ? (l1 - (l0 & ~3u) + 15u) / 16u : 0u;
+    if (__any(groups > 0u)) listed(list[0], 0);
+    if (__any(groups > 1u)) listed(list[1], 1);
+#pragma unroll 1
+    for (uint32_t i = 2; __any(groups > i); ++i) listed(g_load(i), i);
+    ex += ln_dpp<0x124>(ex);
+    ex += ln_dpp<0x128>(ex);
+    // row 4 kg + k: the plane's sum is acc[k] of any lane of kg, the list's is with lane n = k
+    const float plane_sum = n == 0u ? acc[0] : n == 1u ? acc[1] : n == 2u ? acc[2] : acc[3];
+    if (n < 4u) parts[wave * 16u + 4u * kg + n] = plane_sum + ex;
+    __syncthreads();
+
+    // ---- outputs: a row's sums over the columns ----
+    const uint32_t per = FIRST && gated ? 2u : 1u, at = tid & 15u, item = tid >> 4, out_row = (b0 / per + item) * 16u + at;
+    if (item * per >= blocks || out_row >= outputs) return;
+    auto sum_of = [&](uint32_t block) {
+        float v = 0.0f;
+        for (uint32_t k = 0; k < C; ++k) v += parts[(block * C + k) * 16u + at];
+        return v;
+    };
+    const uint16_t *const plus = bias ? bias + (size_t)e * (per * outputs) : nullptr;
+    float v = sum_of(item * per);
+    if (plus) v += bf16_bits_to_f32(plus[out_row]);
+    if constexpr (FIRST) {
+        v = ep_activation(activation, v);
+        if (gated) {
+            float u = sum_of(item * 2u + 1u);
+            if (plus) u += bf16_bits_to_f32(plus[outputs + out_row]);
+            v *= u;
+        }
+        static_cast<uint16_t *>(out)[(int64_t)slot * ld_out + out_row] = ep_bf16(v);
+    } else {
+        static_cast<float *>(out)[(int64_t)slot * ld_out + out_row] = v;
+    }
+}
+
+// blocks of a workgroup: as many as sixteen waves have cells for, and few enough for a workgroup to each CU; 0 where a block has too many cells
+static uint32_t eo_blocks(const ExMatrix &W, uint32_t per, uint32_t slots) {
+    const uint32_t all = (W.n_tiles + 3u) / 4u;
+    if (W.n_cells * per > 16u) return 0;
+    return std::max(std::min(std::min(16u / W.n_cells, all * slots / ln_cus()), all) / per * per, per);
+}
+
+bool experts_one_takes(const ExMatrix &W, bool gated) { return W.n_cells * (gated ? 2u : 1u) <= 16u; }
+
+template <int BITS, bool FIRST> static int eo_launch(const ExMatrix &W, const ExOne &R, hipStream_t s) {
+    const uint32_t per = FIRST && R.gated ? 2u : 1u, C = W.n_cells, all = (W.n_tiles + 3u) / 4u, blocks = eo_blocks(W, per, R.tokens * R.top_k);
+    if (!blocks) return IXH_EUNSUPPORTED;
+    const bool whole = ((uintptr_t)R.x & 15u) == 0 && W.in_f % 8u == 0 && (R.ldx % 8 == 0 || R.rows == 1u);
+    const size_t lds = LnPairs<BITS, false>::kLutBytes + C * 1024u + 64u + blocks * C * 64u;
+    // (a wave / C as a product with 2^16 / C, rounded up: exact for sixteen waves)
+    const uint32_t shape = C | blocks << 5 | (uint32_t)R.gated << 10 | (uint32_t)whole << 11 | (65536u / C + 1u) << 12;
+    IXH_LAUNCH((k_experts_one<BITS, FIRST>), dim3((all + blocks - 1u) / blocks, R.top_k, R.tokens), dim3(blocks * C * kWave), lds, s, R.ids, W.plane, R.x,
+               W.exc_off, W.scale, shape, W.n_tiles, (uint32_t)W.plane_words, R.experts, W.in_f, R.ldx, W.exc_pos, W.exc_val, W.bias, R.out, R.ld_out,
+               W.outputs, R.activation);
+    return hipGetLastError() == hipSuccess ? IXH_OK : IXH_ELAUNCH;
+}
+template <bool FIRST> static int eo_matrix(const ExMatrix &W, const ExOne &R, hipStream_t s) {
+    switch (W.bits) {
+        case 3: return eo_launch<3, FIRST>(W, R, s);
+        case 4: return eo_launch<4, FIRST>(W, R, s);
+        case 5: return eo_launch<5, FIRST>(W, R, s);
+        default: return eo_launch<8, FIRST>(W, R, s);
+    }
+}
+int launch_experts_one(const ExMatrix &W, const ExOne &R, bool first, hipStream_t s) { return first ? eo_matrix<true>(W, R, s) : eo_matrix<false>(W, R, s); }
+
+}  // namespace ixh

@@ -298,3 +298,78 @@ def test_experts_from_a_graph_and_another_stream(dev, tokens):
         torch.cuda.synchronize()
         assert torch.equal(y, eager) and torch.equal(ids, eager_ids)
         _close(y, *ref.experts(x, ids, weights, **dense, residual=residual))
+
+
+# ---- the same by the kernel that takes a call: slots one by one, tiles of an expert's slots, rows of many cells ----
+def _repeated_layer(dev, experts, hidden, inner, recipe, level_bits, distinct=3, **kw):
+    """A layer of a few matrices, each with several experts."""
+    from ixrun_amd import StreamingExperts
+    from ixrun_amd.quantize import decode_to_weight, int8x_quantize
+
+    make, rows = RECIPES[recipe], 2 * inner if kw.get("gated", True) else inner
+    gate_up = [int8x_quantize(make(rows, hidden, seed=2 * e), level_bits) for e in range(distinct)]
+    down = [int8x_quantize(make(hidden, inner, seed=2 * e + 1), level_bits) for e in range(distinct)]
+    of = [e % distinct for e in range(experts)]
+    g = torch.Generator().manual_seed(experts)
+    b1, b2 = ((torch.randn(experts, n, generator=g) * 0.1).bfloat16() for n in (rows, hidden))
+    layer = StreamingExperts([gate_up[e] for e in of], [down[e] for e in of], gate_up_bias=b1, down_bias=b2, **kw)
+    stack = lambda packs: torch.stack([decode_to_weight(p).to(dev) for p in packs])[of]
+    dense = dict(gate_up=stack(gate_up), down=stack(down), act=kw.get("activation", "silu"), gated=kw.get("gated", True), gate_up_bias=b1.to(dev),
+                 down_bias=b2.to(dev))
+    return layer, dense
+
+
+@pytest.mark.parametrize("recipe,level_bits", [("t", (3, 5, 8)), ("real", (3, 5, 8)), ("outlier", (4, 8)), ("real", (6, 8))])
+@pytest.mark.parametrize("gated", [True, False])
+@pytest.mark.parametrize("hidden,inner", [(4100, 40), (8200, 24), (72, 8200), (12301, 9)])
+@pytest.mark.parametrize("tokens", [1, 2, 9, 37])
+def test_experts_of_long_rows(dev, recipe, level_bits, gated, hidden, inner, tokens):
+    layer, dense = _repeated_layer(dev, 12, hidden, inner, recipe, level_bits, gated=gated)
+    x, ids, weights, residual = _call(dev, tokens, 3, 12, hidden, skew=0.2, residual=True)
+    _close(layer(x, ids, weights, residual), *ref.experts(x, ids, weights, **dense, residual=residual))
+
+
+@pytest.mark.parametrize("recipe,level_bits", [("t", (3, 5, 8)), ("real", (3, 5, 8)), ("outlier", (4, 8)), ("real", (6, 8))])
+@pytest.mark.parametrize("experts,hidden,inner,tokens,top_k", [(24, 2048, 600, 38, 6), (48, 1024, 512, 100, 3), (30, 1001, 515, 62, 5)])
+def test_experts_by_tiles(dev, recipe, level_bits, experts, hidden, inner, tokens, top_k):
+    """Up to ten slots an expert, more cells than go one by one; uneven, and with places and tokens of no expert."""
+    layer, dense = _repeated_layer(dev, experts, hidden, inner, recipe, level_bits)
+    for skew in (0.0, 0.15):
+        x, ids, weights, residual = _call(dev, tokens, top_k, experts, hidden, skew=skew, residual=True)
+        ids[3, 1:] = -1
+        ids[7] = experts
+        y = layer(x, ids, weights, residual)
+        clean = torch.where((ids >= 0) & (ids < experts), weights, 0)
+        _close(y, *ref.experts(x, ids, clean, **dense, residual=residual))
+        assert torch.equal(y[7], residual[7])
+        wild = x.clone()
+        wild[5], wild[17, 3] = math.inf, math.nan
+        same = torch.ones(tokens, dtype=torch.bool)
+        same[[5, 17]] = False
+        assert torch.equal(layer(wild, ids, weights, residual)[same], y[same])
+
+
+@pytest.mark.parametrize("recipe,level_bits", [("t", (3, 5, 8)), ("real", (3, 5, 8)), ("outlier", (4, 8)), ("real", (6, 8))])
+@pytest.mark.parametrize("hidden,inner", [(2048, 1024), (8, 8), (4096, 33), (1037, 520), (4090, 700)])
+def test_experts_one_by_one(dev, recipe, level_bits, hidden, inner):
+    """Slots by themselves: rows of one to eight cells, the same expert in several slots and twice in a token, places without one, rows of any
+    alignment, a row of infinities beside others."""
+    layer, dense = _repeated_layer(dev, 9, hidden, inner, recipe, level_bits)
+    for tokens, top_k in ((1, 1), (1, 9), (3, 4), (8, 2)):
+        x, ids, weights, residual = _call(dev, tokens, top_k, 9, hidden, seed=tokens + top_k, residual=True)
+        if tokens > 1:
+            ids[0] = 4
+            ids[1, 0] = -7
+        clean = torch.where(ids >= 0, weights, 0)
+        y = layer(x, ids, weights, residual)
+        _close(y, *ref.experts(x, ids, clean, **dense, residual=residual))
+        apart = torch.zeros(tokens, hidden + 9, dtype=torch.bfloat16, device=dev)
+        for start in (1, 8):
+            view = apart[:, start:start + hidden]
+            view.copy_(x)
+            assert torch.equal(layer(view, ids, weights, residual), y)
+        if tokens > 1:
+            wild = x.clone()
+            wild[1] = math.inf
+            same = torch.arange(tokens) != 1
+            assert torch.equal(layer(wild, ids, weights, residual)[same], y[same])
