@@ -2,6 +2,7 @@
 #include "ixh_experts.h"
 
 #include <algorithm>
+#include <type_traits>
 
 #include "ixh_epilogue.h"
 #include "ixh_lanes_dev.h"
@@ -12,7 +13,10 @@ namespace ixh {
 // k_experts_plan: the slots (token, j) that have an expert, by expert and in their order within one, cut into tiles of `rows` slots.
 //
 // A workgroup an expert, no two of which wait for each other: each counts the slots of all experts (in LDS; sums of whole numbers do not
-// hang on their order), so it knows where its own begin, and then writes these.  Reads the ids twice, from the L2.
+// hang on their order), so it knows where its own begin, and then writes these.
+//
+// Bound: a launch and two waits for memory with few slots (384 and 615 slots of 64 and 20 experts 5.2 us), the counting in LDS with many
+// (24576 slots of 64 experts 12 us; ids that all are kept from the first look to the second make no difference there).
 // ---------------------------------------------------------------------------------------------------------------
 constexpr uint32_t kExPlanThreads = 1024, kExPlanWaves = kExPlanThreads / kWave;
 
@@ -41,23 +45,30 @@ __device__ __forceinline__ ExSizes ex_sizes(uint32_t n, const ExCut &cut) {
     return of;
 }
 
+// (N ids a lane at a time, kept from the first look at them to the second where that is all of them: 615 slots 6.2 -> 5.2 us)
+template <uint32_t N>
 __global__ void __launch_bounds__(kExPlanThreads)
 k_experts_plan(const int32_t *__restrict__ ids, uint32_t slots, uint32_t experts, ExCut cut, ExPlan plan) {
     __shared__ uint32_t hist[kExMostExperts], of_wave[kExPlanWaves], sums[1u + kExSizes][kExPlanWaves];
     const uint32_t tid = threadIdx.x, lane = tid & 63u, wave = tid >> 6, e = blockIdx.x;
-    for (uint32_t i = tid; i < experts; i += kExPlanThreads) hist[i] = 0;
-    __syncthreads();
     // a wave has whole 64 slots one after another
     const uint32_t share = ((slots + kExPlanThreads - 1u) / kExPlanThreads) * kWave, from = min(wave * share, slots), to = min(from + share, slots);
-    constexpr uint32_t N = 8;  // ids of a lane in flight
+    uint32_t id[N];
+    auto load = [&](uint32_t i0) {
+#pragma unroll
+        for (uint32_t k = 0; k < N; ++k) id[k] = (uint32_t)ids[min(i0 + k * kWave + lane, slots - 1u)];
+#pragma unroll
+        for (uint32_t k = 0; k < N; ++k)
+            if (i0 + k * kWave + lane >= to) id[k] = ~0u;
+    };
+    load(from);
+    for (uint32_t i = tid; i < experts; i += kExPlanThreads) hist[i] = 0;
+    __syncthreads();
     uint32_t mine = 0;
     for (uint32_t i0 = from; i0 < to; i0 += N * kWave) {
-        uint32_t id[N];
-#pragma unroll
-        for (uint32_t k = 0; k < N; ++k) id[k] = (uint32_t)ids[min(i0 + k * kWave + lane, to - 1u)];
+        if (i0 != from) load(i0);
 #pragma unroll
         for (uint32_t k = 0; k < N; ++k) {
-            if (i0 + k * kWave + lane >= to) id[k] = ~0u;
             if (id[k] < experts) atomicAdd(hist + id[k], 1u);
             mine += id[k] == e;
         }
@@ -112,16 +123,14 @@ k_experts_plan(const int32_t *__restrict__ ids, uint32_t slots, uint32_t experts
     }
     uint32_t at = before;
     for (uint32_t w = 0; w < wave; ++w) at += of_wave[w];
+    const bool again = share > N * kWave;
     for (uint32_t i0 = from; i0 < to; i0 += N * kWave) {
-        uint32_t id[N];
-#pragma unroll
-        for (uint32_t k = 0; k < N; ++k) id[k] = (uint32_t)ids[min(i0 + k * kWave + lane, to - 1u)];
+        if (again) load(i0);
 #pragma unroll
         for (uint32_t k = 0; k < N; ++k) {
-            const uint32_t i = i0 + k * kWave + lane;
-            const bool own = i < to && id[k] == e;
+            const bool own = id[k] == e;
             const uint64_t all = __ballot(own);
-            if (own) plan.order[at + lanes_below(all)] = i;
+            if (own) plan.order[at + lanes_below(all)] = i0 + k * kWave + lane;
             at += (uint32_t)__popcll(all);
         }
     }
@@ -606,7 +615,13 @@ int launch_experts(const ExDev &X, const ExCall &call, void *workspace, hipStrea
     uint32_t *const counts = reinterpret_cast<uint32_t *>(ws);
     const ExPlan plan{counts, counts + 1, reinterpret_cast<uint32_t *>(ws + w.tiles), reinterpret_cast<uint32_t *>(ws + w.order)};
     float *const per_slot = reinterpret_cast<float *>(ws + w.per_slot);
-    if (planned) IXH_LAUNCH(k_experts_plan, dim3(X.experts), dim3(kExPlanThreads), 0, s, call.ids, slots, X.experts, ExCut{w.rows}, plan);
+    if (planned) {
+        const auto run = [&](auto n) {
+            IXH_LAUNCH(k_experts_plan<n()>, dim3(X.experts), dim3(kExPlanThreads), 0, s, call.ids, slots, X.experts, ExCut{w.rows}, plan);
+        };
+        if (slots <= kExPlanThreads) run(std::integral_constant<uint32_t, 1>{});
+        else run(std::integral_constant<uint32_t, 8>{});
+    }
     int rc;
     if (w.many) {
         rc = launch_experts_prompt(X, call, plan, n_tiles, w.blocks, ws + w.x, ws + w.inner, per_slot, s);
