@@ -548,10 +548,11 @@ template <bool FIRST> static int ex_matrix(const ExMatrix &W, const ExRows &R, u
     }
 }
 
-// Many tokens to an expert: 11 and more in the mean (us of a call, k_experts_rows with 8 / 12 / 16 tokens each, and k_experts_prompt with 24,
-// whose time hardly hangs on that up to 64: 64 experts of 2048 x 1024 at 5 % listed 138 / 179 / 207, 171; next to none listed 102 / 129 / 149, 138;
-// 16 of 4096 x 1536 93 / 111 / 130, 101; 20 of 1400 x 744 60 / 67 / 71, 62).
-constexpr uint32_t kExMany = 11;
+// Many tokens to an expert: 9 and more in the mean (us of a call with 6 / 8 / 9 / 12 / 16 tokens each, by k_experts_rows and by k_experts_prompt:
+// 64 experts of 2048 x 1024 at 5 % listed 118 / 131 / 146 / 168 / 198 and 130 / 135 / 136 / 140 / 151; next to none listed 88 / 97 / 106 / 122 /
+// 142 and 99 / 107 / 107 / 114 / 124; 16 of 4096 x 1536 82 / 92 / 103 / 107 / 130 and 91 / 93 / 93 / 93 / 96; 20 of 1400 x 744
+// 56 / 59 / 59 / 65 / 71 and 49 / 50 / 50 / 55 / 56).
+constexpr uint32_t kExMany = 9;
 // (Rows of up to 2^20 columns: offsets within a tile's rows are 32 bits.)
 static bool ex_many(const ExDev &X, uint32_t slots) {
     return slots >= kExMany * X.experts && std::max(X.first.n_cells, X.second.n_cells) <= 2048u;

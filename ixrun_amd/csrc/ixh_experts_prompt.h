@@ -31,27 +31,35 @@ struct EpCall {
 // activations come from the L2 straight to registers as operands.  A wave has MI blocks of 16 rows, MI = 1 .. 4 by the tile's, and all 64
 // weight rows.  The tiles of one expert's rows run on one XCD, whose L2 holds them.
 //
-// Bound: a stage's waits (codes and lists from memory, look-ups, barriers), until products of three and more blocks a wave cover them.
-// Three workgroups to a CU, by registers (168) and LDS (53 KB with the smaller pair table), fill in for one another; one of eight waves
-// with 128 weight rows, up to 512 rows and the larger table, as in k_lanes_prompt, decodes a weight half as often and waits alone: us of
-// a call, eight / four waves, 64 experts of 2048 x 1024 at 5 % listed with 24, 64, 128, 200, 400, 600 tokens each 238 / 171, 252 / 191, 308 / 249,
-// 386 / 324, 566 / 550, 760 / 778, 16 of 4096 x 1536 with next to none 172 / 101, 197 / 120, 220 / 189, 284 / 239, 404 / 390, 505 / 506.
+// NARROW, one block of rows: each wave multiplies the 16 weight rows that it decodes, and no wave waits for another before the end (us of a call
+// with 12 tokens to each expert, of the others' kind / this: 64 experts of 2048 x 1024 at 5 % listed 161 / 140, next to none 126 / 114, 16 of
+// 4096 x 1536 97 / 93).  With two and four blocks the rows, which each wave then takes from the L2, cost more than that saves (32 / 64 tokens
+// each, 64 experts, next to none listed: 135 / 162 become 156 / 192).
+//
+// Bound: nothing alone.  With 384 rows an expert the vector unit is busy for 45 % of the time, matrix unit 37 %, LDS 46 % and L1 50 %, and the L2
+// gives 12 TB/s; a call of 558 us without its products' waits for the L2 took 470, without lists 494, without any decode 425.  With 64 rows LDS:
+// each wave reads all 64 weight rows for a block of its own.
+// Three workgroups to a CU, by registers (168) and LDS (53 KB with the smaller pair table), fill in for one another.  us of a call here / with
+// eight waves, 128 weight rows, up to 512 rows and the larger table as in k_lanes_prompt, which waits alone: 64 experts of 2048 x 1024 at 5 % listed
+// with 64, 128, 200, 400, 600 tokens each 191 / 252, 249 / 308, 324 / 386, 550 / 566, 778 / 760, 16 of 4096 x 1536 with next to none 120 / 197,
+// 189 / 220, 239 / 284, 390 / 404, 506 / 505.  Tiles of up to 384 rows and two workgroups, which decode half as often: 200, 384, 600 tokens 329 /
+// 344, 523 / 549, 787 / 779.  Operands of weights asked for two and three blocks ahead: the same.
 // ---------------------------------------------------------------------------------------------------------------
-template <int BITS, int MI, bool FIRST>
+template <int BITS, int MI, bool NARROW, bool FIRST>
 __device__ __forceinline__ void ep_tile(const ExMatrix &W, const EpCall &R, uint32_t e, uint32_t block0, uint32_t n_blocks, uint32_t tile,
                                         uint8_t *ep_smem) {
     using P = LnPairs<BITS, false>;
-    constexpr uint32_t NI = kEpWaves;
+    constexpr uint32_t NI = NARROW ? 1 : kEpWaves;  // a wave's blocks of weight rows
     constexpr uint32_t AHEAD = MI == 1 ? 8 : MI == 2 ? 4 : 2;  // steps of 32 columns that the activations' operands are asked for ahead
     constexpr uint32_t CODES = 2;  // stages that the codes are asked for ahead of their decode
     const uint32_t smem = (uint32_t)(uintptr_t)(LN_LDS(uint8_t) *)ep_smem;
     const uint32_t tid = threadIdx.x, lane = tid & 63u, n = lane & 15u, kg = lane >> 4;
     const uint32_t wave = (uint32_t)__builtin_amdgcn_readfirstlane((int)(tid >> 6));
     const uint32_t n_cells = W.n_cells, n_tiles = W.n_tiles, n_kb = n_cells * 16u;
-    const uint32_t mb0 = wave * MI;  // the wave's first block of rows, in the tile
+    const uint32_t mb0 = NARROW ? 0u : wave * MI;  // the wave's first block of rows, in the tile
     const float scale = bf16_bits_to_f32(W.scale[e]);
 
-    // ---- the wave's part of the decode: block `wave` of the workgroup's eight, lane (n, kg) the codes of row n ----
+    // ---- the wave's part of the decode: block `wave` of the workgroup's four, lane (n, kg) the codes of row n ----
     const uint32_t *const exc_off = W.exc_off + (size_t)e * (n_tiles * n_cells + 1u);
     const uint16_t *const exc_pos = W.exc_pos;
     const int8_t *const exc_val = W.exc_val;
@@ -208,100 +216,144 @@ __device__ __forceinline__ void ep_tile(const ExMatrix &W, const EpCall &R, uint
     codes(0u, CODES);
     asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
 
-    // A stage of products, and the next stage's decode (past the end: the last cell's first stage again, which nobody reads).  Requests are
-    // never inside a branch: the compiler counts what is in flight.
-    if (mb0 >= n_blocks) {  // no rows: the decode only
-#pragma unroll 1
-        for (uint32_t c = 0; c < n_cells; ++c) {
-            const uint32_t c_next = min(c + 1u, n_cells - 1u);
-#pragma unroll
-            for (uint32_t q = 0; q < 4; ++q) {
-                if (q == 1) list = quads(e_now);
-                if (q == 3) take_list(c + 1u);
-                store((q + 1u) & 3u);
-                patch((q + 1u) & 3u);
-                codes(q + 1u + CODES < 4u ? c : c_next, (q + 1u + CODES) & 3u);
-                asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
-            }
-        }
-        return;
-    }
     ln_f32x4 acc[MI][NI];
 #pragma unroll
     for (uint32_t i = 0; i < MI; ++i)
 #pragma unroll
         for (uint32_t j = 0; j < NI; ++j) acc[i][j] = ln_f32x4{0, 0, 0, 0};
+    if constexpr (NARROW) {
+        // A wave's weights are its own: nothing waits for another wave.
+        const LN_LDS(ln_u32x4) *const own = w_at + wave * 256u;
 #pragma unroll 1
-    for (uint32_t c = 0; c < n_cells; ++c) {
-        const uint32_t c_next = min(c + 1u, n_cells - 1u);
+        for (uint32_t c = 0; c < n_cells; ++c) {
+            const uint32_t c_next = min(c + 1u, n_cells - 1u);
 #pragma unroll
-        for (uint32_t q = 0; q < 4; ++q) {
-            constexpr uint32_t PER = 16 / NI;  // pairs of weights decoded with each block's products
-            const uint32_t p = (q + 1u) & 3u, base = store_at + (p & 1u) * kEpTile + lane * 16u;
-            uint32_t o[16];
-            auto piece = [&](uint32_t k) {
-                *reinterpret_cast<LN_LDS(ln_u32x4) *>((uintptr_t)(base + ((k ^ p) << 10))) = ln_u32x4{o[4 * k], o[4 * k + 1], o[4 * k + 2], o[4 * k + 3]};
-            };
-            auto products = [&](uint32_t j) {
-                const uint32_t t = 4u * q + j;
-                ln_u32x4 v[2];
-                auto weights = [&](uint32_t b) { v[b & 1u] = w_at[(q & 1u) * (kEpTile / 16u) + b * 256u + j * 64u]; };
-                weights(0);
+            for (uint32_t q = 0; q < 4; ++q) {
+                const uint32_t p = (q + 1u) & 3u;
+                if (q == 1) list = quads(e_now);
+                if (q == 3) take_list(c + 1u);
+                ln_wave_order();
+                ln_u32x4 v[4];
 #pragma unroll
-                for (uint32_t b = 0; b < NI; ++b) {
-                    if (b + 1 < NI) weights(b + 1);
-                    if (j == 0) {
-                        if (b && b * PER % 4 == 0) piece(b * PER / 4 - 1);
-                        uint32_t d[16];
-                        ln_decode<BITS, false>(w[p % CODES], lut_lane, scale, d);
+                for (uint32_t j = 0; j < 4; ++j) v[j] = own[(q & 1u) * (kEpTile / 16u) + j * 64u];
+                store(p);
 #pragma unroll
-                        for (uint32_t k = b * PER; k < b * PER + PER; ++k) o[k] = d[k];
-                        __builtin_amdgcn_sched_barrier(0);
-                    }
+                for (uint32_t j = 0; j < 4; ++j) {
+                    const uint32_t t = 4u * q + j;
 #pragma unroll
                     for (uint32_t i = 0; i < MI; ++i)
-                        acc[i][b] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(ln_bf16x8, v[b & 1u]),
-                                                                            __builtin_bit_cast(ln_bf16x8, a[t % AHEAD][i]), acc[i][b], 0, 0, 0);
-                    __builtin_amdgcn_sched_barrier(0);
+                        acc[i][0] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(ln_bf16x8, v[j]), __builtin_bit_cast(ln_bf16x8, a[t % AHEAD][i]),
+                                                                            acc[i][0], 0, 0, 0);
+                    x_load(t + AHEAD < 16u ? c : c_next, (t + AHEAD) & 15u);
                 }
-                if (j == 0) piece(3);
-                x_load(t + AHEAD < 16u ? c : c_next, (t + AHEAD) & 15u);
-                __builtin_amdgcn_sched_barrier(0);
-            };
-            if (q == 1) list = quads(e_now);
-            if (q == 3) {
-                take_list(c + 1u);
+                patch(p);
+                codes(q + 1u + CODES < 4u ? c : c_next, (q + 1u + CODES) & 3u);
                 __builtin_amdgcn_sched_barrier(0);
             }
-            products(0);
-            products(1);
-            patch(p);
-            __builtin_amdgcn_sched_barrier(0);
-            codes(q + 1u + CODES < 4u ? c : c_next, (q + 1u + CODES) & 3u);
-            products(2);
-            products(3);
-            asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
         }
     }
+    if constexpr (!NARROW) {
+        // A stage of products, and the next stage's decode (past the end: the last cell's first stage again, which nobody reads).  Requests are
+        // never inside a branch: the compiler counts what is in flight.
+        if (mb0 >= n_blocks) {  // no rows: the decode only
+#pragma unroll 1
+            for (uint32_t c = 0; c < n_cells; ++c) {
+                const uint32_t c_next = min(c + 1u, n_cells - 1u);
+#pragma unroll
+                for (uint32_t q = 0; q < 4; ++q) {
+                    if (q == 1) list = quads(e_now);
+                    if (q == 3) take_list(c + 1u);
+                    store((q + 1u) & 3u);
+                    patch((q + 1u) & 3u);
+                    codes(q + 1u + CODES < 4u ? c : c_next, (q + 1u + CODES) & 3u);
+                    asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+                }
+            }
+            return;
+        }
+#pragma unroll 1
+        for (uint32_t c = 0; c < n_cells; ++c) {
+            const uint32_t c_next = min(c + 1u, n_cells - 1u);
+#pragma unroll
+            for (uint32_t q = 0; q < 4; ++q) {
+                constexpr uint32_t PER = 16 / NI;  // pairs of weights decoded with each block's products
+                const uint32_t p = (q + 1u) & 3u, base = store_at + (p & 1u) * kEpTile + lane * 16u;
+                uint32_t o[16];
+                auto piece = [&](uint32_t k) {
+                    *reinterpret_cast<LN_LDS(ln_u32x4) *>((uintptr_t)(base + ((k ^ p) << 10))) = ln_u32x4{o[4 * k], o[4 * k + 1], o[4 * k + 2], o[4 * k + 3]};
+                };
+                auto products = [&](uint32_t j) {
+                    const uint32_t t = 4u * q + j;
+                    ln_u32x4 v[2];
+                    auto weights = [&](uint32_t b) { v[b & 1u] = w_at[(q & 1u) * (kEpTile / 16u) + b * 256u + j * 64u]; };
+                    weights(0);
+#pragma unroll
+                    for (uint32_t b = 0; b < NI; ++b) {
+                        if (b + 1 < NI) weights(b + 1);
+                        if (j == 0) {
+                            if (b && b * PER % 4 == 0) piece(b * PER / 4 - 1);
+                            uint32_t d[16];
+                            ln_decode<BITS, false>(w[p % CODES], lut_lane, scale, d);
+#pragma unroll
+                            for (uint32_t k = b * PER; k < b * PER + PER; ++k) o[k] = d[k];
+                            __builtin_amdgcn_sched_barrier(0);
+                        }
+#pragma unroll
+                        for (uint32_t i = 0; i < MI; ++i)
+                            acc[i][b] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(ln_bf16x8, v[b & 1u]),
+                                                                                __builtin_bit_cast(ln_bf16x8, a[t % AHEAD][i]), acc[i][b], 0, 0, 0);
+                        __builtin_amdgcn_sched_barrier(0);
+                    }
+                    if (j == 0) piece(3);
+                    x_load(t + AHEAD < 16u ? c : c_next, (t + AHEAD) & 15u);
+                    __builtin_amdgcn_sched_barrier(0);
+                };
+                if (q == 1) list = quads(e_now);
+                if (q == 3) {
+                    take_list(c + 1u);
+                    __builtin_amdgcn_sched_barrier(0);
+                }
+                products(0);
+                products(1);
+                patch(p);
+                __builtin_amdgcn_sched_barrier(0);
+                codes(q + 1u + CODES < 4u ? c : c_next, (q + 1u + CODES) & 3u);
+                products(2);
+                products(3);
+                asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+            }
+        }
 
+    }
     // ---- the sums: lane (n, kg) of block (i, b) has weight rows 4 kg .. + 3 of row n ----
     if constexpr (FIRST) {
         // The sums of a block of rows go through LDS, which takes an index, so that a short loop works out four columns at a time: a copy of
         // the activations for each register of sums is 60 KB of instructions, of which every tile fetches what it passes through (512 rows
         // 14.7 us).
         const uint16_t *const bias = W.bias ? W.bias + (size_t)e * (R.gated ? 2u * W.outputs : W.outputs) : nullptr;
-        LN_LDS(ln_f32x4) *const sums = reinterpret_cast<LN_LDS(ln_f32x4) *>((uintptr_t)(smem + P::kLutBytes + wave * (NI * 1024u) + lane * 16u));
+        LN_LDS(ln_f32x4) *const sums = reinterpret_cast<LN_LDS(ln_f32x4) *>((uintptr_t)(smem + P::kLutBytes + wave * 4096u + lane * 16u));
         const uint32_t per = R.gated ? 2u : 1u;
+        // (of narrow tiles a wave has a block of rows, of which the four waves have the weight rows)
+        constexpr uint32_t BLOCKS = NARROW ? 1 : MI;
+        const uint32_t m0 = NARROW ? wave : mb0;
+        if constexpr (NARROW) {
+            __syncthreads();
 #pragma unroll
-        for (uint32_t i = 0; i < MI; ++i) {
-            if (mb0 + i >= n_blocks) break;
+            for (uint32_t i = 0; i < MI; ++i) sums[((int)i - (int)wave) * 256 + (int)wave * 64] = acc[i][0];
+            __syncthreads();
+        }
 #pragma unroll
-            for (uint32_t b = 0; b < NI; ++b) sums[b * 64u] = acc[i][b];
-            ln_wave_order();
-            uint8_t *const block = R.inner + (size_t)(block0 + mb0 + i) * R.n_kb_inner * 1024u;
+        for (uint32_t i = 0; i < BLOCKS; ++i) {
+            if (m0 + i >= n_blocks) break;
+            if constexpr (!NARROW) {
+#pragma unroll
+                for (uint32_t b = 0; b < NI; ++b) sums[b * 64u] = acc[i][b];
+                ln_wave_order();
+            }
+            uint8_t *const block = R.inner + (size_t)(block0 + m0 + i) * R.n_kb_inner * 1024u;
 #pragma unroll 1
-            for (uint32_t b = 0; b < NI; b += per) {
-                const uint32_t col = (tile * NI + b) / per * 16u + 4u * kg;
+            for (uint32_t b = 0; b < kEpWaves; b += per) {
+                const uint32_t col = (tile * kEpWaves + b) / per * 16u + 4u * kg;
                 if (col >= R.n_kb_inner * 32u) continue;
                 ln_f32x4 v = sums[b * 64u];
                 if (bias)
@@ -327,9 +379,9 @@ __device__ __forceinline__ void ep_tile(const ExMatrix &W, const EpCall &R, uint
         // columns of the intermediate's last cell that no weight row makes: zeros
         if (tile + 1u == R.w_tiles) {
             const uint32_t from = R.w_tiles * (kEpRows / per) / 32u;
-            for (uint32_t i = 0; i < MI && mb0 + i < n_blocks; ++i)
+            for (uint32_t i = 0; i < BLOCKS && m0 + i < n_blocks; ++i)
                 for (uint32_t kb = from; kb < R.n_kb_inner; ++kb)
-                    reinterpret_cast<ln_u32x4 *>(R.inner)[((size_t)(block0 + mb0 + i) * R.n_kb_inner + kb) * 64u + lane] = ln_u32x4{0u, 0u, 0u, 0u};
+                    reinterpret_cast<ln_u32x4 *>(R.inner)[((size_t)(block0 + m0 + i) * R.n_kb_inner + kb) * 64u + lane] = ln_u32x4{0u, 0u, 0u, 0u};
         }
     } else {
         const uint16_t *const bias = W.bias ? W.bias + (size_t)e * W.outputs : nullptr;
@@ -341,7 +393,7 @@ __device__ __forceinline__ void ep_tile(const ExMatrix &W, const EpCall &R, uint
             float *const to = R.out + (size_t)slot * W.outputs;
 #pragma unroll
             for (uint32_t b = 0; b < NI; ++b) {
-                const uint32_t col = (tile * NI + b) * 16u + 4u * kg;
+                const uint32_t col = (tile * kEpWaves + (NARROW ? wave : b)) * 16u + 4u * kg;
                 ln_f32x4 v = acc[i][b];
                 if (bias)
 #pragma unroll
@@ -366,10 +418,11 @@ k_experts_prompt(ExMatrix W, EpCall R) {
     const uint32_t id = blockIdx.x, turn = id >> 3, row_tile = (turn / R.w_tiles) * 8u + (id & 7u), tile = turn % R.w_tiles;
     if (row_tile >= *R.n_tiles) return;
     const uint32_t e = R.tiles[3u * row_tile], block0 = R.tiles[3u * row_tile + 1u], n_blocks = R.tiles[3u * row_tile + 2u];
-    if (n_blocks <= kEpWaves) ep_tile<BITS, 1, FIRST>(W, R, e, block0, n_blocks, tile, ep_smem);
-    else if (n_blocks <= 2u * kEpWaves) ep_tile<BITS, 2, FIRST>(W, R, e, block0, n_blocks, tile, ep_smem);
-    else if (n_blocks <= 3u * kEpWaves) ep_tile<BITS, 3, FIRST>(W, R, e, block0, n_blocks, tile, ep_smem);
-    else ep_tile<BITS, 4, FIRST>(W, R, e, block0, n_blocks, tile, ep_smem);
+    if (n_blocks == 1u) ep_tile<BITS, 1, true, FIRST>(W, R, e, block0, n_blocks, tile, ep_smem);
+    else if (n_blocks <= kEpWaves) ep_tile<BITS, 1, false, FIRST>(W, R, e, block0, n_blocks, tile, ep_smem);
+    else if (n_blocks <= 2u * kEpWaves) ep_tile<BITS, 2, false, FIRST>(W, R, e, block0, n_blocks, tile, ep_smem);
+    else if (n_blocks <= 3u * kEpWaves) ep_tile<BITS, 3, false, FIRST>(W, R, e, block0, n_blocks, tile, ep_smem);
+    else ep_tile<BITS, 4, false, FIRST>(W, R, e, block0, n_blocks, tile, ep_smem);
 }
 
 template <int BITS, bool FIRST> int ep_launch(const ExMatrix &W, EpCall R, uint32_t row_tiles, hipStream_t s) {

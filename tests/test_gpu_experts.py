@@ -322,7 +322,7 @@ def _repeated_layer(dev, experts, hidden, inner, recipe, level_bits, distinct=3,
 @pytest.mark.parametrize("recipe,level_bits", [("t", (3, 5, 8)), ("real", (3, 5, 8)), ("outlier", (4, 8)), ("real", (6, 8))])
 @pytest.mark.parametrize("gated", [True, False])
 @pytest.mark.parametrize("hidden,inner", [(4100, 40), (8200, 24), (72, 8200), (12301, 9)])
-@pytest.mark.parametrize("tokens", [1, 2, 9, 37])
+@pytest.mark.parametrize("tokens", [1, 2, 9, 30, 37])
 def test_experts_of_long_rows(dev, recipe, level_bits, gated, hidden, inner, tokens):
     layer, dense = _repeated_layer(dev, 12, hidden, inner, recipe, level_bits, gated=gated)
     x, ids, weights, residual = _call(dev, tokens, 3, 12, hidden, skew=0.2, residual=True)
@@ -330,7 +330,8 @@ def test_experts_of_long_rows(dev, recipe, level_bits, gated, hidden, inner, tok
 
 
 @pytest.mark.parametrize("recipe,level_bits", [("t", (3, 5, 8)), ("real", (3, 5, 8)), ("outlier", (4, 8)), ("real", (6, 8))])
-@pytest.mark.parametrize("experts,hidden,inner,tokens,top_k", [(24, 2048, 600, 38, 6), (48, 1024, 512, 100, 3), (30, 1001, 515, 62, 5)])
+@pytest.mark.parametrize("experts,hidden,inner,tokens,top_k", [(24, 2048, 600, 38, 6), (48, 1024, 512, 100, 3), (30, 1001, 515, 62, 5), (24, 2048, 600, 34, 6),
+                                                               (30, 1001, 515, 52, 5)])
 def test_experts_by_tiles(dev, recipe, level_bits, experts, hidden, inner, tokens, top_k):
     """Up to ten slots an expert, more cells than go one by one; uneven, and with places and tokens of no expert."""
     layer, dense = _repeated_layer(dev, experts, hidden, inner, recipe, level_bits)
