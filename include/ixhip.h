@@ -295,7 +295,7 @@ int ixh_lanes_product(const IxhLanes *lanes, const uint16_t *x, int64_t ldx, con
                       uint16_t *y, int64_t ldy, void *workspace, size_t workspace_bytes, ixh_stream_t stream);
 size_t ixh_lanes_product_workspace_bytes(const IxhLanes *lanes, int32_t m);
 
-/* The same of sums that are there already, in bf16 [m, ldv]: y = bf16( act(v) * multiplier + residual ), any m; y may be v. */
+/* The same of sums that are there already, in bf16 [m, ldv]: y = bf16( act(v) * multiplier + residual ), any m, rows of fewer than 2^24; y may be v. */
 int ixh_epilogue(const uint16_t *v, int64_t ldv, int64_t m, int64_t out_f, const IxhEpilogue *epilogue, uint16_t *y, int64_t ldy,
                  ixh_stream_t stream);
 
@@ -327,10 +327,11 @@ int ixh_route(const IxhRouting *routing, const void *logits, int32_t dtype, int6
  *   y[t] = bf16( residual[t] + sum_j weights[t, j] * second_e( h ) ),  e = ids[t, j], in the order of j,
  *   h = bf16( act(gate_e x[t] + b) * (up_e x[t] + b) ),  or bf16( act(first_e x[t] + b) ) if not `gated`.
  * x bf16 [tokens, ldx], y and residual (may be NULL) bf16 [tokens, ld]; ids and weights (fp32) [tokens, top_k].  A place whose id is none of
- * 0 .. n_experts - 1 adds nothing, and its weight is not read.  tokens * top_k up to 2^20.  Sums, biases and the sum over the experts are fp32.
+ * 0 .. n_experts - 1 adds nothing, and its weight is not used.  y may be x or residual, at its stride.
+ * tokens * top_k up to 2^20, up to 1024 experts, hidden below 2^24.  Sums, biases and the sum over the experts are fp32.
  *
  * IxhExpertMatrix: one matrix of all experts, out_f x in_f each: planes one after another (ixh_lanes_plane_words each), exc_off of
- * ixh_lanes_cells + 1 entries for each expert, all of them places in one list, and a scale for each expert.  `first` is inner x hidden, or,
+ * ixh_lanes_cells + 1 entries for each expert, all of them places in one list (exc_pos 8-byte aligned, exc_val 4-byte), and a scale for each.  `first` is inner x hidden, or,
  * gated, 2 * inner16 x hidden with inner16 = inner rounded up to 16: blocks of 16 rows, of the gate and of the other half in turn, rows past
  * the last zero.  Its bias (bf16, may be NULL) is [n_experts, 2 * inner], the gate's first ([n_experts, inner] if not gated).  `second` is
  * hidden x inner, its bias [n_experts, hidden].

@@ -725,7 +725,7 @@ int ixh_epilogue(const uint16_t *v, int64_t ldv, int64_t m, int64_t out_f, const
     Epilogue ep;
     const int rc = to_epilogue(epilogue, m, out_f, &ep);
     if (rc) return rc;
-    if (m < 0 || m >= (1ll << 31) || out_f < 1 || out_f >= (1ll << 31)) { set_error("epilogue: %lld x %lld", (long long)m, (long long)out_f); return IXH_EINVAL; }
+    if (m < 0 || m >= (1ll << 31) || out_f < 1 || out_f >= (1ll << 24)) { set_error("epilogue: %lld x %lld", (long long)m, (long long)out_f); return IXH_EINVAL; }
     if (m == 0) return IXH_OK;
     if (!v || !y) { set_error("epilogue: v or y is NULL"); return IXH_EINVAL; }
     if (m > 1 && (ldv < out_f || ldy < out_f)) { set_error("epilogue: ldv or ldy shorter than a row"); return IXH_EINVAL; }
@@ -780,6 +780,10 @@ static int to_matrix(const IxhExpertMatrix &p, int64_t experts, int64_t out_f, i
         set_error("experts: %s: scale, exc_off or the list is NULL, or the list holds no whole groups of 64 quads, or 2^30 quads", name);
         return IXH_EINVAL;
     }
+    if (((uintptr_t)p.exc_off & 3u) || ((uintptr_t)p.exc_pos & 7u) || ((uintptr_t)p.exc_val & 3u)) {
+        set_error("experts: %s: exc_off and exc_val must be 4-byte aligned, exc_pos 8-byte", name);
+        return IXH_EINVAL;
+    }
     *out = ExMatrix{p.plane, p.exc_off, p.exc_pos, p.exc_val, p.scale, p.bias, (uint64_t)words, (uint32_t)((out_f + 3) / 4),
                     (uint32_t)((in_f + kLnCols - 1) / kLnCols), (uint32_t)in_f, (uint32_t)outputs, p.bits};
     return IXH_OK;
@@ -788,7 +792,7 @@ static int to_matrix(const IxhExpertMatrix &p, int64_t experts, int64_t out_f, i
 static int to_experts(const IxhExperts *p, int64_t tokens, int32_t top_k, ExDev *out) {
     if (!p) { set_error("experts is NULL"); return IXH_EINVAL; }
     if (p->n_experts < 1 || p->n_experts > (int32_t)kExMostExperts) { set_error("experts: %d experts not in 1..%u", p->n_experts, kExMostExperts); return IXH_EINVAL; }
-    if (p->hidden < 1 || p->inner < 1 || p->hidden >= (1ll << 31) || p->inner >= (1ll << 29)) { set_error("experts: %lld x %lld", (long long)p->inner, (long long)p->hidden); return IXH_EINVAL; }
+    if (p->hidden < 1 || p->inner < 1 || p->hidden >= (1ll << 24) || p->inner >= (1ll << 29)) { set_error("experts: %lld x %lld", (long long)p->inner, (long long)p->hidden); return IXH_EINVAL; }
     if (!ep_known(p->activation)) { set_error("experts: activation %d", p->activation); return IXH_EINVAL; }
     if (top_k < 1 || tokens < 0 || tokens > (int64_t)kExMostSlots / top_k) {
         set_error("experts: %lld tokens of %d experts each, not 2^20 places at most", (long long)tokens, top_k);

@@ -190,7 +190,7 @@ k_experts_rows(ExMatrix W, ExRows R) {
     // columns.  What comes on top is the same for all lanes.
     const uint32_t x_mine = x_at + (MT == 1 ? kg * 16u : (8u * kg + (n >> 2)) * ROW + (n & 1u) * 8u);
 
-    // (below 2^30 items: fewer than 16 slots an expert)
+    // (below 2^31 items)
     const uint32_t all_items = (R.n_tiles ? *R.n_tiles : R.slots) * R.per_tile;
     uint32_t item, item_end;
     if (R.of_tile) {
@@ -505,6 +505,7 @@ static int ex_launch(const ExMatrix &W, ExRows R, uint32_t n_tiles, hipStream_t 
     // as few chunks as leave room for the sums of eight blocks, and as many blocks of a part as then fit, up to those that a workgroup has at all
     // Few tiles: as many workgroups to each, so that none begins a second one (which takes as long as some ten cells).
     const uint64_t items = (uint64_t)n_tiles * R.per_tile;
+    if (items >= 1ull << 31) return IXH_EUNSUPPORTED;  // (their numbers are 32 bits)
     R.of_tile = R.n_tiles || n_tiles > ln_cus() ? 0u : std::min(ln_cus() / n_tiles, R.per_tile);
     const uint32_t groups = R.of_tile ? n_tiles * R.of_tile : (uint32_t)std::min<uint64_t>(items, ln_cus());
     const uint32_t share = (uint32_t)std::min<uint64_t>((items + groups - 1u) / groups, R.per_tile) * per;

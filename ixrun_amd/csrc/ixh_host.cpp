@@ -543,7 +543,9 @@ PyObject *route(PyObject *, PyObject *const *args, Py_ssize_t n_args) {
         PyErr_Clear();
         Py_RETURN_NONE;
     }
-    if (v[0] < 1 || v[0] > experts || experts > 1024) Py_RETURN_NONE;  // (what has to raise)
+    if (experts > 1024) Py_RETURN_NONE;  // (what has to raise)
+    for (int i = 0; i < 3; ++i)
+        if (v[i] < 1 || v[i] > experts) Py_RETURN_NONE;
     const IxhRouting routing{(int32_t)experts, (int32_t)v[0], (int32_t)v[1], (int32_t)v[2], (int32_t)v[3], (int32_t)v[4], (float)scale};
     c10::SmallVector<int64_t, 4> shape(l.sizes().begin(), l.sizes().end());
     shape.back() = v[0];

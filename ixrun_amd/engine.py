@@ -467,7 +467,8 @@ class StreamingLinear(nn.Module):
         ``forward`` runs and the rest follows as a launch of its own, from the product rounded to bf16."""
         act = _lib.ACTIVATIONS.get(activation)
         if self._native is not None and self._use_fused and self._gemm_ok and not self._gemv_flags and act is not None:
-            y = _lib.host().product(self._lanes_at, self._bias_ptr or 0, self._scale.device.index, x, act, multiplier, residual)
+            index = self._scale.device.index
+            y = _lib.host().product(self._lanes_at, self._bias_ptr or 0, index, x, act, multiplier, residual) if index is not None else None
             if y is not None:
                 return y
         for name, t in (("x", x), ("multiplier", multiplier), ("residual", residual)):
@@ -475,8 +476,8 @@ class StreamingLinear(nn.Module):
                 continue
             if t.dtype is not torch.bfloat16:
                 raise TypeError(f"{name} must be bf16 (got {t.dtype})")
-            if t.device != self._scale.device:
-                raise RuntimeError(f"{name} must live on {self._scale.device} (got {t.device}); the HIP path has no CPU fallback")
+            if t.device != self._scale.device or not t.is_cuda:
+                raise RuntimeError(f"{name} must live on the layer's GPU (got {t.device}, layer on {self._scale.device}); the HIP path has no CPU fallback")
             if t.requires_grad and torch.is_grad_enabled():
                 raise RuntimeError("StreamingLinear.product has no gradient: call it under torch.no_grad(), or with tensors that need none")
         if activation not in _lib.ACTIVATIONS:

@@ -20,6 +20,7 @@ __all__ = ["StreamingExperts", "route_experts"]
 
 LOGIT_TYPES = {torch.float32: _lib.IXH_F32, torch.float16: _lib.IXH_F16, torch.bfloat16: _lib.IXH_BF16}
 SCORINGS = {"softmax": _lib.IXH_SCORE_SOFTMAX, "sigmoid": _lib.IXH_SCORE_SIGMOID}
+MOST_EXPERTS = 1024
 MOST_PLACES = 1 << 17  # tokens times experts of each in one call of the library: bounds the call's scratch
 
 
@@ -61,6 +62,8 @@ def route_experts(logits, top_k: int, *, scoring: str = "softmax", bias=None, n_
         if bias.device != dev or bias.numel() != experts:
             raise ValueError(f"bias must hold {experts} elements on {dev}")
         bias = bias.to(torch.float32).contiguous()
+    if not (0 <= top_k <= experts and 0 <= n_groups <= experts and 0 <= top_groups <= experts):  # (as 32-bit numbers they might pass)
+        raise ValueError(f"top_k {top_k}, n_groups {n_groups} or top_groups {top_groups} of {experts} experts")
     routing = _lib.IxhRouting(experts, top_k, n_groups, top_groups, SCORINGS[scoring], bool(renormalize), scale)
     shape = logits.shape[:-1] + (max(top_k, 0),)
     ids = torch.empty(shape, dtype=torch.int32, device=dev)
@@ -89,6 +92,8 @@ class StreamingExperts(nn.Module):
         super().__init__()
         if not gate_up or len(gate_up) != len(down):
             raise ValueError(f"{len(gate_up)} and {len(down)} matrices: one of each for every expert")
+        if len(gate_up) > MOST_EXPERTS:
+            raise ValueError(f"{len(gate_up)} experts, {MOST_EXPERTS} at most")
         if activation not in _lib.ACTIVATIONS:
             raise ValueError(f"activation {activation!r} is none of {[a for a in _lib.ACTIVATIONS if a]}")
         self.n_experts, self.gated, self.activation = len(gate_up), bool(gated), activation
@@ -177,22 +182,32 @@ class StreamingExperts(nn.Module):
                                     pos.numel() // 4, scale.data_ptr(), bias.data_ptr() if bias is not None else None)
 
     def _bind(self):
+        """Point the library's arguments at the buffers; those of a layer that is not on a GPU are none."""
+        self._struct, self._struct_at = None, 0
+        if not self._first_plane.is_cuda:
+            return
         rows = -(-self.inner // 16) * 32 if self.gated else self.inner
         self._struct = _lib.IxhExperts(self.n_experts, self.gated, _lib.ACTIVATIONS[self.activation], self.hidden, self.inner,
                                        self._matrix("first", rows, self.hidden), self._matrix("second", self.hidden, self.inner))
-        self._struct_ref, self._struct_at, self._device_index = C.byref(self._struct), C.addressof(self._struct), self._first_plane.device.index
+        self._struct_at, self._device_index = C.addressof(self._struct), self._first_plane.device.index
+
+    def __getstate__(self):
+        return {**self.__dict__, "_struct": None, "_struct_at": 0}
+
+    def __setstate__(self, state):
+        super().__setstate__(state)
+        self._bind()
 
     def _apply(self, fn, recurse=True):
         # .to() may move the buffers: point the arguments at the new storage.  (Their types are the layout's and stay.)
-        kept = {name: (t, t.dtype) for name, t in self.named_buffers(recurse=False)}
+        kept = dict(self.named_buffers(recurse=False))
         out = super()._apply(fn, recurse)
-        for name, (_, dtype) in kept.items():
-            t = getattr(self, name)
-            if t.dtype != dtype:
-                raise TypeError(f"an experts' layer cannot be cast: {name} is {dtype}")
-        self._struct_at = 0
-        if self._first_plane.is_cuda:
-            self._bind()
+        cast = [name for name, t in kept.items() if getattr(self, name).dtype != t.dtype]
+        if cast:
+            for name, t in kept.items():
+                setattr(self, name, t)
+            raise TypeError(f"an experts' layer cannot be cast: {cast[0]} is {kept[cast[0]].dtype}")
+        self._bind()
         return out
 
     def _load_from_state_dict(self, state_dict, prefix, local_metadata, strict, missing_keys, unexpected_keys, error_msgs):
@@ -203,15 +218,22 @@ class StreamingExperts(nn.Module):
             if given and len(given) != len(keys):
                 error_msgs.append(f"a part of an experts' layout: {[k for k in keys if k not in state_dict]} are missing")
                 return
+            for k, part in zip(given, LAYOUT):
+                t, own = state_dict[k], getattr(self, f"_{name}_{part}")
+                if t.dtype != own.dtype or t.shape != own.shape or not t.is_contiguous():
+                    error_msgs.append(f"{k} is {t.dtype} {tuple(t.shape)}, expected {own.dtype} {tuple(own.shape)}, contiguous")
+                    return
             if given:
                 off, pos = state_dict[keys[1]], state_dict[keys[2]]
-                if off.dtype != torch.int32 or off.dim() != 2 or bool((off[:, 1:] < off[:, :-1]).any()) or int(off[:, 0].min()) < 0 \
-                        or int(off[:, -1].max()) > pos.numel() // 4:
+                if bool((off[:, 1:] < off[:, :-1]).any()) or int(off[:, 0].min()) < 0 or int(off[:, -1].max()) > pos.numel() // 4:
                     error_msgs.append(f"{keys[1]} does not fit the list")
                     return
+            k, own = f"{prefix}_{name}_bias", getattr(self, f"_{name}_bias")
+            if own is not None and k in state_dict and (state_dict[k].dtype != own.dtype or state_dict[k].shape != own.shape or not state_dict[k].is_contiguous()):
+                error_msgs.append(f"{k} is {state_dict[k].dtype} {tuple(state_dict[k].shape)}, expected {own.dtype} {tuple(own.shape)}, contiguous")
+                return
         super()._load_from_state_dict(state_dict, prefix, local_metadata, strict, missing_keys, unexpected_keys, error_msgs)
-        if self._first_plane.is_cuda:
-            self._bind()
+        self._bind()
 
     def extra_repr(self) -> str:
         return f"experts={self.n_experts}, hidden={self.hidden}, inner={self.inner}, gated={self.gated}, activation={self.activation}"
@@ -235,6 +257,8 @@ class StreamingExperts(nn.Module):
             if y is not None:
                 return y
         _inference_only("StreamingExperts", x, weights, residual)
+        if self._struct is None:
+            raise RuntimeError(f"the layer is on {self._first_plane.device}; the HIP path has no CPU fallback")
         dev = self._first_plane.device
         if x.dim() < 1 or x.shape[-1] != self.hidden:
             raise ValueError(f"x is {tuple(x.shape)}, expected [..., {self.hidden}]")
@@ -254,10 +278,10 @@ class StreamingExperts(nn.Module):
         step = max(MOST_PLACES // top_k, 1)
         L = _lib.lib()
         with _lib.on_device(dev):
-            need = L.ixh_experts_workspace_bytes(self._struct_ref, min(n, step), top_k)
+            need = L.ixh_experts_workspace_bytes(C.byref(self._struct), min(n, step), top_k)
             ws = torch.empty(need, dtype=torch.uint8, device=dev)
             for t in range(0, n, step):
-                _lib.check(L.ixh_experts(self._struct_ref, rows.data_ptr() + 2 * t * rows.stride(0), rows.stride(0), min(step, n - t),
+                _lib.check(L.ixh_experts(C.byref(self._struct), rows.data_ptr() + 2 * t * rows.stride(0), rows.stride(0), min(step, n - t),
                                          ids.data_ptr() + 4 * t * top_k, weights.data_ptr() + 4 * t * top_k, top_k,
                                          res.data_ptr() + 2 * t * res.stride(0) if res is not None else None,
                                          res.stride(0) if res is not None else 0, y.data_ptr() + 2 * t * self.hidden, self.hidden,

@@ -76,6 +76,10 @@ def _experts(hidden=96, inner=40, gated=1):
     (lambda e: setattr(e.second, "exc_off", None), "scale"),
     (lambda e: setattr(e.second, "n_quads", 65), "groups of 64"),
     (lambda e: setattr(e.second, "n_quads", 1 << 30), "groups of 64"),
+    (lambda e: setattr(e, "hidden", 1 << 24), "experts: 40 x 16777216"),
+    (lambda e: setattr(e.second, "exc_pos", 0x1004), "8-byte"),
+    (lambda e: setattr(e.first, "exc_val", 0x1002), "aligned"),
+    (lambda e: setattr(e.first, "exc_off", 0x1002), "aligned"),
 ])
 def test_malformed_experts_are_refused(change, needle):
     lib = _lib.lib()

@@ -374,3 +374,122 @@ def test_experts_one_by_one(dev, recipe, level_bits, hidden, inner):
             wild[1] = math.inf
             same = torch.arange(tokens) != 1
             assert torch.equal(layer(wild, ids, weights, residual)[same], y[same])
+
+
+def test_routing_refusals(dev):
+    from ixrun_amd import route_experts
+
+    logits = torch.zeros(3, 16, device=dev)
+    for wrong in (dict(top_k=17), dict(top_k=2 ** 32 + 2), dict(top_k=2, n_groups=2 ** 32 + 1, top_groups=1), dict(top_k=2, n_groups=4, top_groups=2 ** 32 + 1),
+                  dict(top_k=-1), dict(top_k=2, scoring="max"), dict(top_k=2, bias=torch.zeros(15, device=dev))):
+        with pytest.raises((ValueError, RuntimeError)):
+            route_experts(logits, **wrong)
+    with pytest.raises(TypeError):
+        route_experts(logits.double(), 2)
+    with pytest.raises(RuntimeError, match="no gradient"):
+        route_experts(logits.clone().requires_grad_(), 2)
+
+
+def test_experts_off_the_gpu_are_refused(dev):
+    layer, _ = _layer(dev, 3, 64, 16)
+    x, ids, weights, _ = _call(dev, 3, 1, 3, 64)
+    want = layer(x, ids, weights)
+    layer.cpu()
+    for on in ("cpu", dev):
+        with pytest.raises(RuntimeError, match="no CPU fallback"):
+            layer(x.to(on), ids.to(on), weights.to(on))
+    layer.to(dev)
+    assert torch.equal(layer(x, ids, weights), want)
+
+
+def test_experts_after_a_refused_cast_and_copied(dev):
+    """A refused cast leaves the layer as it was; a copy has weights of its own."""
+    import copy
+
+    layer, _ = _layer(dev, 3, 64, 16, bias=True)
+    x, ids, weights, _ = _call(dev, 5, 2, 3, 64)
+    want = layer(x, ids, weights)
+    for cast in (lambda: layer.float(), lambda: layer.half(), lambda: layer.to(torch.float64)):
+        with pytest.raises(TypeError, match="cast"):
+            cast()
+    torch.randn(1 << 20, device=dev)  # (what might take freed memory)
+    assert torch.equal(layer(x, ids, weights), want)
+    other = copy.deepcopy(layer)
+    for t in layer.state_dict().values():
+        t.zero_()
+    assert torch.equal(other(x, ids, weights), want)
+
+
+def test_experts_states_of_other_types_are_refused(dev):
+    layer, _ = _layer(dev, 3, 256, 48, "t", bias=True)
+    x, ids, weights, _ = _call(dev, 5, 2, 3, 256)
+    want = layer(x, ids, weights)
+    state = {k: v.clone() for k, v in layer.state_dict().items()}
+    changes = dict(_first_plane=lambda t: t.to(torch.int8), _first_pos=lambda t: t.int(), _second_off=lambda t: t.long(), _second_scale=lambda t: t.float(),
+                   _first_val=lambda t: t[:-64], _first_bias=lambda t: t.t().contiguous().t(), _second_bias=lambda t: t.float())
+    for name, change in changes.items():
+        with pytest.raises(RuntimeError, match=name):
+            layer.load_state_dict(dict(state, **{name: change(state[name])}), assign=True)
+        assert torch.equal(layer(x, ids, weights), want)
+
+
+def test_experts_of_a_long_call_are_taken_in_parts(dev, monkeypatch):
+    from ixrun_amd import experts
+
+    layer, dense = _layer(dev, 4, 264, 64, "t")
+    x, ids, weights, residual = _call(dev, 71, 2, 4, 264, residual=True)
+    for most in (1, 7, 60, 100):
+        monkeypatch.setattr(experts, "MOST_PLACES", most)
+        _close(layer(x, ids, weights, residual), *ref.experts(x, ids, weights, **dense, residual=residual))
+
+
+def test_experts_write_over_their_input(dev):
+    """The C entry: y may be the residual or x, and what lies behind the rows stays."""
+    import ctypes as C
+
+    from ixrun_amd import _lib
+
+    layer, _ = _layer(dev, 4, 264, 64, "t")
+    for tokens in (1, 9, 60):
+        x, ids, weights, residual = _call(dev, tokens, 2, 4, 264, residual=True)
+        want = layer(x, ids, weights, residual)
+        need = _lib.lib().ixh_experts_workspace_bytes(C.byref(layer._struct), tokens, 2)
+        ws = torch.empty(need, dtype=torch.uint8, device=dev)
+        for over_x in (False, True):
+            held = torch.full((tokens + 1, 280), 7.0, dtype=torch.bfloat16, device=dev)
+            held[:tokens, :264] = x if over_x else residual
+            a, r = (held, residual) if over_x else (x, held)
+            _lib.check(_lib.lib().ixh_experts(C.byref(layer._struct), a.data_ptr(), a.stride(0), tokens, ids.data_ptr(), weights.data_ptr(), 2, r.data_ptr(),
+                                              r.stride(0), held.data_ptr(), 280, ws.data_ptr(), need, _lib.current_stream(dev)))
+            assert torch.equal(held[:tokens, :264], want)
+            assert bool((held[tokens] == 7).all()) and bool((held[:, 264:] == 7).all())
+
+
+def test_two_calls_at_once_and_graphs_in_turn(dev):
+    """Calls of two streams side by side, and two graphs of one layer replayed in turn, with other work in between."""
+    layer, dense = _layer(dev, 8, 512, 128, "real")
+    calls = [_call(dev, tokens, 3, 8, 512, seed=tokens, residual=True) for tokens in (1, 40, 300)]
+    want = [layer(*c) for c in calls]
+    streams = [torch.cuda.Stream() for _ in calls]
+    for s in streams:
+        s.wait_stream(torch.cuda.current_stream())
+    for _ in range(5):
+        got = []
+        for s, c in zip(streams, calls):
+            with torch.cuda.stream(s):
+                got.append(layer(*c))
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+    graphs, outs = [], []
+    for c in calls:
+        graphs.append(torch.cuda.CUDAGraph())
+        with torch.cuda.graph(graphs[-1]):
+            outs.append(layer(*c))
+    for turn in range(4):
+        for y in outs:
+            y.zero_()
+        for g in (graphs if turn % 2 else graphs[::-1]):
+            g.replay()
+            layer(*calls[turn % 3])
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(outs, want))

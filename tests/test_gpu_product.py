@@ -200,3 +200,15 @@ def test_a_gated_block_from_a_graph_and_another_stream(dev, rows):
         eager = block(x)
         torch.cuda.synchronize()
         assert torch.equal(y, eager)
+
+
+def test_a_layer_off_the_gpu_is_refused(dev):
+    layer, _, _ = _layer(dev, 64, 128)
+    x, m, r = _operands(dev, 3, 64, 128, True, True)
+    want = layer.product(x, "silu", m, r)
+    layer.cpu()
+    for given in (x, x.cpu()):
+        with pytest.raises(RuntimeError, match="no CPU fallback"):
+            layer.product(given, "silu")
+    layer.to(dev)
+    assert torch.equal(layer.product(x, "silu", m, r), want)

@@ -39,7 +39,7 @@ def test_product_scratch_is_that_of_the_product_by_itself():
 
 @pytest.mark.parametrize("change,needle", [
     (dict(v=None), "NULL"), (dict(y=None), "NULL"), (dict(m=-1), "-1 x"), (dict(out_f=0), "x 0"), (dict(ldv=7), "shorter"), (dict(ldy=7), "shorter"),
-    (dict(act=9), "activation"),
+    (dict(act=9), "activation"), (dict(out_f=1 << 24, ldv=1 << 24, ldy=1 << 24), "2 x 16777216"),
 ])
 def test_malformed_epilogues_are_refused(change, needle):
     lib = _lib.lib()
