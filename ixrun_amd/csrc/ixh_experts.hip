@@ -20,13 +20,13 @@ namespace ixh {
 // ---------------------------------------------------------------------------------------------------------------
 constexpr uint32_t kExPlanThreads = 1024, kExPlanWaves = kExPlanThreads / kWave;
 
-// How an expert's slots are cut into tiles: of up to `rows` of them; with rows = 0 of up to four layers, a layer being 64 slots, a block of 16
+// How an expert's slots are cut into tiles: of up to `rows` of them; with rows = 0 of up to `most` layers, a layer being 64 slots, a block of 16
 // to each wave of k_experts_prompt, as even as whole layers allow (what is left of a layer takes as long as the whole).
 constexpr uint32_t kExLayer = 64;
 struct ExCut {
-    uint32_t rows;
+    uint32_t rows, most;  // most: layers of a tile
     __device__ __forceinline__ uint32_t layers(uint32_t n) const { return (n + kExLayer - 1u) / kExLayer; }
-    __device__ __forceinline__ uint32_t tiles(uint32_t n) const { return rows ? (n + rows - 1u) / rows : (layers(n) + 3u) / 4u; }
+    __device__ __forceinline__ uint32_t tiles(uint32_t n) const { return rows ? (n + rows - 1u) / rows : (layers(n) + most - 1u) / most; }
     __device__ __forceinline__ uint32_t places(uint32_t n) const { return rows ? n : (n + 15u) & ~15u; }
 };
 // How many of these are of 4, 3, 2 and 1 layers: the order of the tiles, so that the last ones to be taken are short.  (Tiles of `rows` slots
@@ -559,6 +559,14 @@ static bool ex_many(const ExDev &X, uint32_t slots) {
     return slots >= kExMany * X.experts && std::max(X.first.n_cells, X.second.n_cells) <= 2048u;
 }
 
+// Layers of a tile of k_experts_prompt, two instead of four where all layers by the 64 weight rows of a workgroup are up to eight a CU in the mean of
+// both matrices (us with four / two: 2279 tokens by 3 of 7 experts of 512 x 192, 3 a CU, 50 / 45; 1000 by 2 of 8 of 2048 x 512, 3.4, 64 / 57;
+// 400 and 800 by 2 of 8 of 4096 x 1536, 3.5 and 6.3, 100 / 110 and 147 / 129; 1600 of these, 11.8, 173 / 216; 4000 of the ones before, 12, 115 / 126).
+static uint32_t ex_layers(const ExDev &X, uint32_t slots) {
+    const uint64_t w_tiles = (X.first.n_tiles + 15u) / 16u + (X.second.n_tiles + 15u) / 16u;
+    return (slots / kExLayer + X.experts / 2u) * w_tiles <= 16ull * ln_cus() ? 2u : 4u;
+}
+
 // Slots by expert, not one by one: of k_experts_one from 160 cells a CU on (us one by one / planned: 64 experts of 2048 x 1024, 24 / 48 / 72
 // slots, which are 72 / 144 / 216 cells a CU, 34 / 50 / 67, 53 / 54 / 61; 16 of 4096 x 1536, 8 / 16 / 24 slots 31 / 47 / 60, 46 / 52 / 59; 128 of
 // 2048 x 768, 48 / 96 slots 46 / 72, 58 / 69); of k_experts_rows, whose workgroups begin more slowly, where tiles of several slots are likely.
@@ -571,7 +579,7 @@ static bool ex_planned(const ExDev &X, uint32_t slots) {
 // A call's scratch: the plan, the intermediate, what each slot's expert makes of it, and in k_experts_prompt the gathered rows.
 struct ExScratch {
     bool many;
-    uint32_t rows, n_tiles, blocks;  // as ExCut; tiles and blocks at most
+    uint32_t rows, most, n_tiles, blocks;  // as ExCut; tiles and blocks at most
     size_t tiles, order, x, inner, per_slot, bytes;
     int64_t ld_inner;
 };
@@ -582,9 +590,10 @@ static ExScratch ex_scratch(const ExDev &X, uint32_t tokens, uint32_t top_k) {
     size_t at = 256;
     auto take = [&](size_t n) { const size_t from = at; at += (n + 255u) & ~(size_t)255u; return from; };
     if (w.many) {
-        w.n_tiles = std::min(slots, X.experts) + slots / (4u * kExLayer);
+        w.most = ex_layers(X, slots);
+        w.n_tiles = std::min(slots, X.experts) + slots / (w.most * kExLayer);
         w.blocks = std::min(slots, X.experts) + slots / 16u;
-        w.tiles = take((size_t)w.n_tiles * 12u);
+        w.tiles = take((std::min(slots, X.experts) + slots / (2u * kExLayer)) * (size_t)12u);  // (of either height)
         w.order = take((size_t)w.blocks * 64u);
         w.x = take((size_t)w.blocks * X.first.n_cells * 16384u);
         w.inner = take((size_t)w.blocks * X.second.n_cells * 16384u);
@@ -619,7 +628,7 @@ int launch_experts(const ExDev &X, const ExCall &call, void *workspace, hipStrea
     float *const per_slot = reinterpret_cast<float *>(ws + w.per_slot);
     if (planned) {
         const auto run = [&](auto n) {
-            IXH_LAUNCH(k_experts_plan<n()>, dim3(X.experts), dim3(kExPlanThreads), 0, s, call.ids, slots, X.experts, ExCut{w.rows}, plan);
+            IXH_LAUNCH(k_experts_plan<n()>, dim3(X.experts), dim3(kExPlanThreads), 0, s, call.ids, slots, X.experts, ExCut{w.rows, w.most}, plan);
         };
         if (slots <= kExPlanThreads) run(std::integral_constant<uint32_t, 1>{});
         else run(std::integral_constant<uint32_t, 8>{});
