@@ -197,8 +197,10 @@ k_experts_rows(ExMatrix W, ExRows R) {
         const uint32_t tile = blockIdx.x / R.of_tile, part = blockIdx.x - tile * R.of_tile;
         item = tile * R.per_tile + part * R.per_tile / R.of_tile, item_end = min(tile * R.per_tile + (part + 1u) * R.per_tile / R.of_tile, all_items);
     } else {
+        // (workgroups go round the eight XCDs: those of one have runs in a row, so that the tiles of an expert share its weights in an L2)
         const uint32_t share = all_items / gridDim.x, more = all_items - share * gridDim.x;
-        item = blockIdx.x * share + min(blockIdx.x, more), item_end = item + share + (blockIdx.x < more);
+        const uint32_t run = gridDim.x & 7u ? blockIdx.x : (blockIdx.x & 7u) * (gridDim.x >> 3) + (blockIdx.x >> 3);
+        item = run * share + min(run, more), item_end = item + share + (run < more);
     }
     uint32_t staged = ~0u, e_table = ~0u;  // the tile whose activations are in LDS, the expert whose pairs are
     for (uint32_t blocks; item < item_end; item += blocks / per) {
