@@ -65,14 +65,20 @@ struct ExOne {
     int64_t ldx;
     uint32_t rows;  // of x
     const int32_t *ids;
-    void *out;  // the intermediate in bf16, or fp32
+    void *out;  // the intermediate in bf16, fp32, or (joined) y
     int64_t ld_out;
     uint32_t experts, tokens, top_k;
     int activation;
     bool gated;
+    const float *weights;  // joined: what a token's slots are added with
+    const uint16_t *residual;
+    int64_t ld_residual;
 };
 bool experts_one_takes(const ExMatrix &W, bool gated);
 int launch_experts_one(const ExMatrix &W, const ExOne &R, bool first, hipStream_t s);
+// the second matrix with the sum over a token's slots
+bool experts_joined_takes(const ExMatrix &W, uint32_t tokens, uint32_t top_k);
+int launch_experts_joined(const ExMatrix &W, const ExOne &R, hipStream_t s);
 
 size_t experts_workspace_bytes(const ExDev &X, uint32_t tokens, uint32_t top_k);
 int launch_experts(const ExDev &X, const ExCall &call, void *workspace, hipStream_t s);

@@ -643,13 +643,18 @@ int launch_experts(const ExDev &X, const ExCall &call, void *workspace, hipStrea
         R.x = call.x, R.ldx = call.ldx, R.ids = call.ids, R.experts = X.experts, R.top_k = call.top_k, R.slots = slots;
         if (planned) R.n_tiles = plan.n_tiles, R.tiles = plan.tiles, R.order = plan.order;
         R.out = ws + w.inner, R.ld_out = w.ld_inner, R.activation = X.activation, R.gated = X.gated;
-        ExOne one{call.x, call.ldx, call.tokens, call.ids, R.out, R.ld_out, X.experts, call.tokens, call.top_k, X.activation, X.gated};
+        ExOne one{call.x, call.ldx, call.tokens, call.ids, R.out, R.ld_out, X.experts, call.tokens, call.top_k, X.activation, X.gated, call.weights, call.residual, call.ld_residual};
         if (!planned && experts_one_takes(X.first, X.gated)) rc = launch_experts_one(X.first, one, true, s);
         else rc = ex_matrix<true>(X.first, R, planned ? w.rows : 1u, n_tiles, s);
         if (rc != IXH_OK) return rc;
         R.x = reinterpret_cast<const uint16_t *>(ws + w.inner), R.ldx = w.ld_inner;
         R.out = per_slot, R.ld_out = X.hidden;
-        one.x = R.x, one.ldx = R.ldx, one.rows = slots, one.out = R.out, one.ld_out = R.ld_out;
+        one.x = R.x, one.ldx = R.ldx, one.rows = slots;
+        if (!planned && experts_joined_takes(X.second, call.tokens, call.top_k)) {
+            one.out = call.y, one.ld_out = call.ldy;
+            return launch_experts_joined(X.second, one, s);
+        }
+        one.out = R.out, one.ld_out = R.ld_out;
         if (!planned && experts_one_takes(X.second, false)) rc = launch_experts_one(X.second, one, false, s);
         else rc = ex_matrix<false>(X.second, R, planned ? w.rows : 1u, n_tiles, s);
     }

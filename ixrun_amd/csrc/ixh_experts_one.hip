@@ -8,30 +8,40 @@
 namespace ixh {
 
 // ---------------------------------------------------------------------------------------------------------------
-// k_experts_one<BITS, FIRST>: one slot by a run of blocks of 16 weight rows, a wave for each cell (16 rows x 512 columns).
+// k_experts_one<BITS, FIRST, JOIN>: one slot by a run of blocks of 16 weight rows, a wave for each cell (16 rows x 512 columns).
 //
 // Bound: a launch, one chain of requests (the expert's id, then its codes, the extents of their lists, scale and activations at once, then the
 // lists) and the instructions of a cell.  Products and listed elements as in k_experts_rows, of whose kernel for one row some 350 of 1100
 // instructions a wave only find its share: one token by 6 experts of 2048 x 1024, 25 MB of codes and lists, first / second matrix 13.2 / 9.6 us
 // there, 9.1 / 6.9 us here (1.6 TB/s with their starts and ends).
+//
+// JOIN, the second matrix for a few tokens: a workgroup has a block of rows of all of a token's slots, with a pair table and activations for
+// each, and ends with the sum over them, in their order, so that no launch follows: 20.0 -> 18.3 us for that token (second matrix and sum 6.9 + 2.7 -> 8.5).
 // ---------------------------------------------------------------------------------------------------------------
-template <int BITS, bool FIRST>
+struct EoJoin {  // what a token's outputs are made with
+    const float *weights;
+    const uint16_t *residual;
+    int64_t ld_residual;
+};
+template <int BITS, bool FIRST, bool JOIN>
 __global__ void __launch_bounds__(1024)
 k_experts_one(const int32_t *__restrict__ ids, const uint32_t *__restrict__ plane, const uint16_t *__restrict__ x, const uint32_t *__restrict__ exc_off,
               const uint16_t *__restrict__ scale_at, uint32_t shape, uint32_t n_tiles, uint32_t plane_words, uint32_t experts, uint32_t in_f, int64_t ldx,
               const uint16_t *__restrict__ exc_pos, const int8_t *__restrict__ exc_val, const uint16_t *__restrict__ bias, void *__restrict__ out,
-              int64_t ld_out, uint32_t outputs, int activation) {
+              int64_t ld_out, uint32_t outputs, int activation, EoJoin join) {
     extern __shared__ __attribute__((aligned(16))) uint8_t eo_smem[];
     using P = LnPairs<BITS, false>;
     const uint32_t smem = (uint32_t)(uintptr_t)(LN_LDS(uint8_t) *)eo_smem;
-    // blocks: row quads from 4 b0 on, all blocks' cells to a wave each
-    const uint32_t C = shape & 31u, blocks = (shape >> 5) & 31u, inv_cells = shape >> 12;
+    // items: the workgroup's blocks of a slot, or (JOIN) a block of each of a token's slots; an item's cells to a wave each
+    const uint32_t C = shape & 31u, items = (shape >> 5) & 31u, inv_cells = shape >> 12;
     const bool gated = (shape >> 10) & 1u, whole = (shape >> 11) & 1u;
-    const uint32_t slot = blockIdx.z * gridDim.y + blockIdx.y, e = (uint32_t)ids[slot];
-    if (e >= experts) return;
-    const uint32_t tid = threadIdx.x, lane = tid & 63u, n = lane & 15u, kg = lane >> 4, n_threads = blocks * C * kWave;
-    const uint32_t wave = (uint32_t)__builtin_amdgcn_readfirstlane((int)(tid >> 6));
-    const uint32_t b0 = blockIdx.x * blocks, b = (wave * inv_cells) >> 16, c = wave - b * C;
+    const uint32_t wave = (uint32_t)__builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6)), item = (wave * inv_cells) >> 16, c = wave - item * C;
+    const uint32_t slot = JOIN ? blockIdx.z * items + item : blockIdx.z * gridDim.y + blockIdx.y, id = (uint32_t)ids[slot];
+    if (!JOIN && id >= experts) return;
+    const uint32_t e = min(id, experts - 1u);  // (what a place without an expert adds is not used)
+    // the threads that share a pair table and a row of activations
+    const uint32_t tid = JOIN ? threadIdx.x - item * C * kWave : threadIdx.x, n_threads = (JOIN ? C : items * C) * kWave, own = JOIN ? item : 0u;
+    const uint32_t lane = threadIdx.x & 63u, n = lane & 15u, kg = lane >> 4, b0 = blockIdx.x * (JOIN ? 1u : items), b = JOIN ? 0u : item;
 
     // ---- all requests ----
     const uint32_t scale_raw = scale_at[e];
@@ -71,6 +81,13 @@ k_experts_one(const int32_t *__restrict__ ids, const uint32_t *__restrict__ plan
 #pragma unroll
         for (uint32_t k = 0; k < 4; ++k) piece[k] = (col + 2u * k < in_f ? h[2 * k] : 0u) | (col + 2u * k + 1u < in_f ? h[2 * k + 1] << 16 : 0u);
     }
+    float plus = 0.0f, residual = 0.0f;
+    if constexpr (JOIN) {
+        if (bias && c == 0u && n < 4u) plus = bf16_bits_to_f32(bias[(size_t)e * outputs + min(b0 * 16u + 4u * kg + n, outputs - 1u)]);
+        if (join.residual && threadIdx.x < 16u)
+            residual = bf16_bits_to_f32(join.residual[(int64_t)blockIdx.z * join.ld_residual + min(b0 * 16u + threadIdx.x, outputs - 1u)]);
+    }
+    const float weight = JOIN ? join.weights[slot] : 0.0f;
     struct Group { ln_u32x2 pos; uint32_t val; };
     auto quad_of = [&](uint32_t i) { return (l0 & ~3u) + 16u * i + (n & ~3u); };
     auto g_load = [&](uint32_t i) {
@@ -84,9 +101,11 @@ k_experts_one(const int32_t *__restrict__ ids, const uint32_t *__restrict__ plan
 
     // ---- pair table and activations to LDS ----
     const float scale = bf16_bits_to_f32(scale_raw);
-    ln_build_lut<BITS, false>(smem, scale, tid, n_threads);
-    const uint32_t x_at = smem + P::kLutBytes, x_none = C * 1024u;
-    float *const parts = reinterpret_cast<float *>(eo_smem + P::kLutBytes + x_none + 64u);  // [wave][16]
+    const uint32_t tables = JOIN ? items : 1u, x_none = C * 1024u, lut = smem + own * P::kLutBytes;
+    ln_build_lut<BITS, false>(lut, scale, tid, n_threads);
+    const uint32_t x_at = smem + tables * P::kLutBytes + own * (x_none + 64u);
+    float *const parts = reinterpret_cast<float *>(eo_smem + tables * (P::kLutBytes + x_none + 64u));  // [wave][16]
+    float *const pluses = parts + items * C * 16u, *const item_weights = pluses + items * 16u;         // JOIN: [item][16], [item]{weight, whether it has an expert}
     if (tid < C * 64u) {
         if (whole && col >= in_f) piece = ln_u32x4{0u, 0u, 0u, 0u};
         *reinterpret_cast<LN_LDS(ln_u32x4) *>((uintptr_t)(x_at + lane_offset(col))) = piece;
@@ -95,7 +114,7 @@ k_experts_one(const int32_t *__restrict__ ids, const uint32_t *__restrict__ plan
     asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
 
     // ---- the cell's products: the row's activations in all sixteen columns (columns 128 q + 32 i of a cell lie at 128 q + 32 (i ^ q)) ----
-    const uint32_t lut_lane = smem + ((lane & ((1u << P::kCopies) - 1u)) << 2), x_cell = x_at + c * 1024u + kg * 16u;
+    const uint32_t lut_lane = lut + ((lane & ((1u << P::kCopies) - 1u)) << 2), x_cell = x_at + c * 1024u + kg * 16u;
     ln_f32x4 acc = {0, 0, 0, 0};
 #pragma unroll
     for (uint32_t q = 0; q < 4; ++q) {
@@ -133,24 +152,43 @@ k_experts_one(const int32_t *__restrict__ ids, const uint32_t *__restrict__ plan
     // row 4 kg + k: the plane's sum is acc[k] of any lane of kg, the list's is with lane n = k
     const float plane_sum = n == 0u ? acc[0] : n == 1u ? acc[1] : n == 2u ? acc[2] : acc[3];
     if (n < 4u) parts[wave * 16u + 4u * kg + n] = plane_sum + ex;
+    if constexpr (JOIN) {
+        if (c == 0u) {
+            if (n < 4u) pluses[item * 16u + 4u * kg + n] = plus;
+            if (lane == 0u) item_weights[2u * item] = weight, item_weights[2u * item + 1u] = id < experts ? 1.0f : 0.0f;
+        }
+        __syncthreads();
+        // y = residual + the sum over the slots, in their order
+        const uint32_t row_out = b0 * 16u + threadIdx.x;
+        if (threadIdx.x >= 16u || row_out >= outputs) return;
+        float v = 0.0f;
+        for (uint32_t j = 0; j < items; ++j) {
+            float p = 0.0f;
+            for (uint32_t k = 0; k < C; ++k) p += parts[(j * C + k) * 16u + threadIdx.x];
+            if (bias) p += pluses[j * 16u + threadIdx.x];
+            if (item_weights[2u * j + 1u] != 0.0f) v = __fmaf_rn(item_weights[2u * j], p, v);
+        }
+        static_cast<uint16_t *>(out)[(int64_t)blockIdx.z * ld_out + row_out] = ep_bf16(join.residual ? v + residual : v);
+        return;
+    }
     __syncthreads();
 
     // ---- outputs: a row's sums over the columns ----
-    const uint32_t per = FIRST && gated ? 2u : 1u, at = tid & 15u, item = tid >> 4, out_row = (b0 / per + item) * 16u + at;
-    if (item * per >= blocks || out_row >= outputs) return;
+    const uint32_t per = FIRST && gated ? 2u : 1u, at = tid & 15u, of = tid >> 4, out_row = (b0 / per + of) * 16u + at;
+    if (of * per >= items || out_row >= outputs) return;
     auto sum_of = [&](uint32_t block) {
         float v = 0.0f;
         for (uint32_t k = 0; k < C; ++k) v += parts[(block * C + k) * 16u + at];
         return v;
     };
-    const uint16_t *const plus = bias ? bias + (size_t)e * (per * outputs) : nullptr;
-    float v = sum_of(item * per);
-    if (plus) v += bf16_bits_to_f32(plus[out_row]);
+    const uint16_t *const biases = bias ? bias + (size_t)e * (per * outputs) : nullptr;
+    float v = sum_of(of * per);
+    if (biases) v += bf16_bits_to_f32(biases[out_row]);
     if constexpr (FIRST) {
         v = ep_activation(activation, v);
         if (gated) {
-            float u = sum_of(item * 2u + 1u);
-            if (plus) u += bf16_bits_to_f32(plus[outputs + out_row]);
+            float u = sum_of(of * 2u + 1u);
+            if (biases) u += bf16_bits_to_f32(biases[outputs + out_row]);
             v *= u;
         }
         static_cast<uint16_t *>(out)[(int64_t)slot * ld_out + out_row] = ep_bf16(v);
@@ -168,26 +206,42 @@ static uint32_t eo_blocks(const ExMatrix &W, uint32_t per, uint32_t slots) {
 
 bool experts_one_takes(const ExMatrix &W, bool gated) { return W.n_cells * (gated ? 2u : 1u) <= 16u; }
 
-template <int BITS, bool FIRST> static int eo_launch(const ExMatrix &W, const ExOne &R, hipStream_t s) {
-    const uint32_t per = FIRST && R.gated ? 2u : 1u, C = W.n_cells, all = (W.n_tiles + 3u) / 4u, blocks = eo_blocks(W, per, R.tokens * R.top_k);
-    if (!blocks) return IXH_EUNSUPPORTED;
+template <int BITS, bool FIRST, bool JOIN> static int eo_launch(const ExMatrix &W, const ExOne &R, hipStream_t s) {
+    const uint32_t per = FIRST && R.gated ? 2u : 1u, C = W.n_cells, all = (W.n_tiles + 3u) / 4u;
+    const uint32_t blocks = JOIN ? 1u : eo_blocks(W, per, R.tokens * R.top_k), items = JOIN ? R.top_k : blocks, tables = JOIN ? items : 1u;
+    if (!items || items * C > 16u) return IXH_EUNSUPPORTED;
     const bool whole = ((uintptr_t)R.x & 15u) == 0 && W.in_f % 8u == 0 && (R.ldx % 8 == 0 || R.rows == 1u);
-    const size_t lds = LnPairs<BITS, false>::kLutBytes + C * 1024u + 64u + blocks * C * 64u;
+    const size_t lds = tables * (LnPairs<BITS, false>::kLutBytes + C * 1024u + 64u) + items * C * 64u + (JOIN ? items * 72u : 0u);
+    if constexpr (JOIN) {
+        static const bool raised = hipFuncSetAttribute(reinterpret_cast<const void *>(k_experts_one<BITS, FIRST, JOIN>),
+                                                       hipFuncAttributeMaxDynamicSharedMemorySize, (int)kLnLds) == hipSuccess;
+        if (!raised || lds > kLnLds) return IXH_ELAUNCH;
+    }
     // (a wave / C as a product with 2^16 / C, rounded up: exact for sixteen waves)
-    const uint32_t shape = C | blocks << 5 | (uint32_t)R.gated << 10 | (uint32_t)whole << 11 | (65536u / C + 1u) << 12;
-    IXH_LAUNCH((k_experts_one<BITS, FIRST>), dim3((all + blocks - 1u) / blocks, R.top_k, R.tokens), dim3(blocks * C * kWave), lds, s, R.ids, W.plane, R.x,
-               W.exc_off, W.scale, shape, W.n_tiles, (uint32_t)W.plane_words, R.experts, W.in_f, R.ldx, W.exc_pos, W.exc_val, W.bias, R.out, R.ld_out,
-               W.outputs, R.activation);
+    const uint32_t shape = C | items << 5 | (uint32_t)R.gated << 10 | (uint32_t)whole << 11 | (65536u / C + 1u) << 12;
+    IXH_LAUNCH((k_experts_one<BITS, FIRST, JOIN>), dim3((all + blocks - 1u) / blocks, JOIN ? 1u : R.top_k, R.tokens), dim3(items * C * kWave), lds, s, R.ids,
+               W.plane, R.x, W.exc_off, W.scale, shape, W.n_tiles, (uint32_t)W.plane_words, R.experts, W.in_f, R.ldx, W.exc_pos, W.exc_val, W.bias, R.out,
+               R.ld_out, W.outputs, R.activation, EoJoin{R.weights, R.residual, R.ld_residual});
     return hipGetLastError() == hipSuccess ? IXH_OK : IXH_ELAUNCH;
 }
-template <bool FIRST> static int eo_matrix(const ExMatrix &W, const ExOne &R, hipStream_t s) {
+template <bool FIRST, bool JOIN> static int eo_matrix(const ExMatrix &W, const ExOne &R, hipStream_t s) {
     switch (W.bits) {
-        case 3: return eo_launch<3, FIRST>(W, R, s);
-        case 4: return eo_launch<4, FIRST>(W, R, s);
-        case 5: return eo_launch<5, FIRST>(W, R, s);
-        default: return eo_launch<8, FIRST>(W, R, s);
+        case 3: return eo_launch<3, FIRST, JOIN>(W, R, s);
+        case 4: return eo_launch<4, FIRST, JOIN>(W, R, s);
+        case 5: return eo_launch<5, FIRST, JOIN>(W, R, s);
+        default: return eo_launch<8, FIRST, JOIN>(W, R, s);
     }
 }
-int launch_experts_one(const ExMatrix &W, const ExOne &R, bool first, hipStream_t s) { return first ? eo_matrix<true>(W, R, s) : eo_matrix<false>(W, R, s); }
+int launch_experts_one(const ExMatrix &W, const ExOne &R, bool first, hipStream_t s) {
+    return first ? eo_matrix<true, false>(W, R, s) : eo_matrix<false, false>(W, R, s);
+}
+
+// Up to twelve waves a workgroup and six tokens: us of a call apart / joined, 1 / 2 / 4 / 8 tokens by 6 of 64 experts of 2048 x 1024 (12 waves) 16.4 / 26.4 /
+// 34.6 / 50.6 and 16.0 / 22.8 / 32.5 / 51.8; by 2 of 16 of 4096 x 1536 (6) 14.0 / 19.4 / 29.5 / 45.8 and 12.3 / 18.4 / 27.0 / 44.0; by 8 of 128 of
+// 2048 x 512 (8) 13.8 / 19.4 / 28.2 / 42.7 and 14.2 / 19.0 / 27.9 / 44.9; of 2048 x 768 (16) 15.8 / 25.4 / 35.1 / 54 and 17.2 / 24.9 / 39.2 / 67.
+bool experts_joined_takes(const ExMatrix &W, uint32_t tokens, uint32_t top_k) {
+    return tokens <= 6u && W.n_cells <= 12u && top_k <= 12u && top_k * W.n_cells <= 12u;
+}
+int launch_experts_joined(const ExMatrix &W, const ExOne &R, hipStream_t s) { return eo_matrix<false, true>(W, R, s); }
 
 }  // namespace ixh
