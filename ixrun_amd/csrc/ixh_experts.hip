@@ -148,6 +148,12 @@ k_experts_plan(const int32_t *__restrict__ ids, uint32_t slots, uint32_t experts
 // of which each workgroup, one a CU, has an equal run: its parts of one tile after another.  Of such a part the cells (16 rows x 512
 // columns) are dealt to the waves in equal runs as well; what a wave has of a block goes to LDS, and the epilogue adds the waves' parts in
 // the columns' order.  Rows longer than LDS holds are taken in chunks of cells, whose sums are added there.
+//
+// The intermediate is rounded to bf16, which the matrix unit's operands have to be: half a step, 2^-9 to 2^-8 of each element, which a row of the second
+// matrix averages (relative error of a call 0.0017 from the output's own rounding, 0.0023 with it).
+//
+// Bound: memory, then vector instructions.  64 tokens by 6 of 64 experts of 2048 x 1024, 5 bits: 54 us for the first matrix, which reads 223 MB
+// (4.1 TB/s; 168 MB of codes, some experts' twice), the vector unit busy for 65 % of it, LDS for 55 %; 35 us for the second, 114 MB.
 // ---------------------------------------------------------------------------------------------------------------
 // (Tiles of 16, which halve the decoding of an expert with more than eight, take longer: their listed elements cost twice as much, and 24 registers
 // go to memory.  us of a call, 8 / 16, 64 experts of 2048 x 1024 with 2, 8 and 16 tokens each: 68 / 91, 101 / 124, 149 / 156.)
@@ -460,7 +466,8 @@ k_experts_rows(ExMatrix W, ExRows R) {
     }
 }
 
-// y[t] = residual[t] + sum_j weights[t, j] * (what its expert made of it), in the order of j.  Bound: memory.  N columns a thread.
+// y[t] = residual[t] + sum_j weights[t, j] * (what its expert made of it), in the order of j.  Bound: memory (4096 tokens of 6 experts, 2048 columns:
+// 218 MB in 39 us, some of it from the last-level cache) or a launch (64 tokens 4.1 us).  N columns a thread.
 template <int N>
 __global__ void __launch_bounds__(256)
 k_experts_join(const float *__restrict__ per_slot, ExCall call, uint32_t experts, uint32_t hidden) {
