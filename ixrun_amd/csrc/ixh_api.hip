@@ -692,7 +692,7 @@ static int to_epilogue(const IxhEpilogue *p, int64_t m, int64_t out_f, Epilogue 
         set_error("epilogue: ld_multiplier or ld_residual shorter than a row");
         return IXH_EINVAL;
     }
-    *out = Epilogue{p->multiplier, p->residual, p->ld_multiplier, p->ld_residual, p->activation};
+    *out = Epilogue{p->multiplier, p->residual, p->ld_multiplier, p->ld_residual, p->activation, false};
     return IXH_OK;
 }
 
@@ -710,6 +710,8 @@ int ixh_lanes_product(const IxhLanes *lanes, const uint16_t *x, int64_t ldx, con
     if (m < 1 || m > kLanesGemmMost) { set_error("m = %d not in 1..%d", m, kLanesGemmMost); return IXH_EINVAL; }
     if (!x || !y) { set_error("x or y is NULL"); return IXH_EINVAL; }
     if (m > 1 && (ldx < (int64_t)d.in_f || ldy < (int64_t)d.out_f)) { set_error("ldx or ldy shorter than a row"); return IXH_EINVAL; }
+    const auto fours = [&](const uint16_t *p, int64_t ld) { return ((uintptr_t)p & 7u) == 0 && (!p || m == 1 || ld % 4 == 0); };
+    ep.wide = fours(bias, 0) && fours(ep.multiplier, ep.ld_multiplier) && fours(ep.residual, ep.ld_residual) && fours(y, ldy);
     LnScratch ws{(float *)workspace, workspace_bytes, 0};
     if (m <= 16) return lanes_status(launch_lanes_gemv(d, x, m, ldx, bias, y, ldy, ws, ep, (hipStream_t)stream), ws, "lanes_product");
     if (!lanes_gemm_aligned(d, x, m, ldx)) {

@@ -322,6 +322,10 @@ EP(k_lanes_gemm)(const uint32_t *__restrict__ plane, const uint16_t *__restrict_
                         else
 #pragma unroll
                             for (uint32_t k = 0; k < 4; ++k) to[k] = acc[b][k];
+#ifdef IXH_EP
+                    } else if (ep.wide && at + 4u <= out_f) {
+                        ep.put(acc[b], ep.fetch(bias, r, at), bias != nullptr, y + (int64_t)r * ldy + at);
+#endif
                     } else {
 #pragma unroll
                         for (uint32_t k = 0; k < 4; ++k) {

@@ -23,6 +23,9 @@ struct LpOut {
 __device__ __forceinline__ void lp_store(const LpOut &out EP_PARAM, uint32_t r, uint32_t row, ln_f32x4 sum) {
     if (r >= out.m || row >= out.out_f) return;
     uint16_t *const to = out.y + (int64_t)r * out.ldy + row;
+#ifdef IXH_EP
+    if (ep.wide && row + 4u <= out.out_f) return ep.put(sum, ep.fetch(out.bias, r, row), out.bias != nullptr, to);
+#endif
     uint16_t v[4];
 #pragma unroll
     for (uint32_t k = 0; k < 4; ++k)
@@ -363,11 +366,27 @@ EP(k_lanes_prompt)(const uint32_t *__restrict__ plane, const ln_u32x4 *__restric
 
         // ---- the sums: lane (n, kg) of block (i, b) has weight rows 4 kg .. + 3 of activation row n.  A whole tile's go to y ----
         if (c0 == 0 && c1 == n_cells) {
+#ifdef IXH_EP
+            // (through the wave's own part of the tiles in LDS, which takes an index: a copy of the epilogue for each register of sums is
+            // fetched by every tile: 17408 x 5120 at 2048 rows 440 us, 385 so)
+            LN_LDS(ln_f32x4) *const sums = reinterpret_cast<LN_LDS(ln_f32x4) *>((uintptr_t)(smem + P::kLutBytes + wave * 4096u + lane * 16u));
+#pragma unroll
+            for (uint32_t i = 0; i < MI; ++i) {
+#pragma unroll
+                for (uint32_t b = 0; b < NI; ++b) sums[(b & 3u) * 64u + (b >> 2) * (kLpTile / 16u)] = acc[i][b];
+                ln_wave_order();
+#pragma unroll 1
+                for (uint32_t b = 0; b < NI; ++b)
+                    lp_store(out EP_ARG, (mb0 + i) * 16u + n, tile * kLpRows + (nw * NI + b) * 16u + 4u * kg, sums[(b & 3u) * 64u + (b >> 2) * (kLpTile / 16u)]);
+                ln_wave_order();
+            }
+#else
 #pragma unroll
             for (uint32_t i = 0; i < MI; ++i)
 #pragma unroll
                 for (uint32_t b = 0; b < NI; ++b)
                     lp_store(out EP_ARG, (mb0 + i) * 16u + n, tile * kLpRows + (nw * NI + b) * 16u + 4u * kg, acc[i][b]);
+#endif
             continue;
         }
         const uint32_t part = mg * out.parts + lp_part(blockIdx.x, tile, begins, gridDim.x, lp_tiles(n_tiles));
@@ -398,9 +417,16 @@ EP(k_lanes_prompt_reduce)(const ln_f32x4 *__restrict__ ws, uint32_t groups, uint
     if (g0 == g1) return;  // its one workgroup wrote y
     if (r >= out.m || row >= out.out_f) return;
     const ln_f32x4 *const from = ws + (size_t)mg * out.parts * SIZE + at;
+#ifdef IXH_EP
+    const bool whole = ep.wide && row + 4u <= out.out_f;
+    const EpFour with = whole ? ep.fetch(out.bias, r, row) : EpFour{};
+#endif
     ln_f32x4 sum = from[(size_t)head * SIZE];
 #pragma unroll 4
     for (uint32_t g = g0 + 1u; g <= g1; ++g) sum += from[(size_t)g * SIZE];
+#ifdef IXH_EP
+    if (whole) return ep.put(sum, with, out.bias != nullptr, out.y + (int64_t)r * out.ldy + row);
+#endif
     lp_store(out EP_ARG, r, row, sum);
 }
 
