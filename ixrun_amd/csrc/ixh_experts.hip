@@ -568,12 +568,12 @@ static bool ex_many(const ExDev &X, uint32_t slots) {
     return slots >= kExMany * X.experts && std::max(X.first.n_cells, X.second.n_cells) <= 2048u;
 }
 
-// Layers of a tile of k_experts_prompt, two instead of four where all layers by the 64 weight rows of a workgroup are up to eight a CU in the mean of
-// both matrices (us with four / two: 2279 tokens by 3 of 7 experts of 512 x 192, 3 a CU, 50 / 45; 1000 by 2 of 8 of 2048 x 512, 3.4, 64 / 57;
-// 400 and 800 by 2 of 8 of 4096 x 1536, 3.5 and 6.3, 100 / 110 and 147 / 129; 1600 of these, 11.8, 173 / 216; 4000 of the ones before, 12, 115 / 126).
+// Layers of a tile of k_experts_prompt, two instead of four where the workgroups then still are all there at once, three a CU (us with four / two: 2279
+// tokens by 3 of 7 experts of 512 x 192, which are 480 of 768 workgroups at most, 50 / 45; 1000 by 2 of 8 of 2048 x 512, 750, 64 / 57; 400 by 2 of 8 of
+// 4096 x 1536, 910, 100 / 110; 512 by 2 of 16 of these, 1500, 119 / 156; 1333 by 3 of 20 of 1400 x 744, 1200, 87 / 104).
 static uint32_t ex_layers(const ExDev &X, uint32_t slots) {
-    const uint64_t w_tiles = (X.first.n_tiles + 15u) / 16u + (X.second.n_tiles + 15u) / 16u;
-    return (slots / kExLayer + X.experts / 2u) * w_tiles <= 16ull * ln_cus() ? 2u : 4u;
+    const uint64_t w_tiles = (std::max(X.first.n_tiles, X.second.n_tiles) + 15u) / 16u;
+    return (slots / (2u * kExLayer) + X.experts) * w_tiles <= 3ull * ln_cus() ? 2u : 4u;
 }
 
 // Slots by expert, not one by one: of k_experts_one from 160 cells a CU on (us one by one / planned: 64 experts of 2048 x 1024, 24 / 48 / 72
