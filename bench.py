@@ -50,17 +50,17 @@ _ENCODE = ("ixh_encode.hip", "ixh_dev.h")
 _OLD = ((), "measured-on-earlier-sources")  # figures kept for the record; reported as null
 MEASURED_TRAFFIC_BYTES = {
     # k_lanes_gemv; eight rows k_lanes_rows, sixteen with k_lanes_reduce
-    "down_proj_5120x17408_m1_student_t": (18521.0 * 2.0 * 1024 + 16.0 * 1024, _LANES, "e5dd4cabcbebf53f"),
-    "down_proj_5120x17408_m1_calibrated": (40732.0 * 2.0 * 1024 + 16.0 * 1024, _LANES, "e5dd4cabcbebf53f"),
-    "down_proj_5120x17408_m1_five_level_calibrated": (40731.8 * 2.0 * 1024 + 16.0 * 1024, _LANES, "e5dd4cabcbebf53f"),
-    "gate_up_17408x5120_m8_calibrated": (36774.0 * 2.0 * 1024 + 272.0 * 1024, _LANES, "e5dd4cabcbebf53f"),
-    "down_proj_5120x17408_m16_student_t": ((19440.5 + 974.0) * 2.0 * 1024 + (1920.0 + 160.0) * 1024, _LANES, "e5dd4cabcbebf53f"),
+    "down_proj_5120x17408_m1_student_t": (18521.0 * 2.0 * 1024 + 16.0 * 1024, _LANES, "472f0d74c39d2277"),
+    "down_proj_5120x17408_m1_calibrated": (40732.0 * 2.0 * 1024 + 16.0 * 1024, _LANES, "472f0d74c39d2277"),
+    "down_proj_5120x17408_m1_five_level_calibrated": (40731.8 * 2.0 * 1024 + 16.0 * 1024, _LANES, "472f0d74c39d2277"),
+    "gate_up_17408x5120_m8_calibrated": (36774.0 * 2.0 * 1024 + 272.0 * 1024, _LANES, "472f0d74c39d2277"),
+    "down_proj_5120x17408_m16_student_t": ((19440.5 + 974.0) * 2.0 * 1024 + (1920.0 + 160.0) * 1024, _LANES, "472f0d74c39d2277"),
     # k_lanes_xtile, k_lanes_prompt and k_lanes_prompt_reduce
     "prefill_5120x17408_m512_five_level": ((8715.5 + 57939.8 + 30739.5) * 2.0 * 1024 + (17408.0 + 66720.0 + 5122.2) * 1024,
-                                           _LANES, "e5dd4cabcbebf53f"),
-    "down_proj_5120x17408_m1_student_t_packed": (23032.0 * 2.0 * 1024 + 16.0 * 1024, _ROWS, "9c5848bbce659441"),
-    "gate_up_17408x5120_m1_student_t_packed": (22935.9 * 2.0 * 1024 + 40.0 * 1024, _ROWS, "9c5848bbce659441"),
-    "attn_proj_5120x5120_m1_student_t_packed": (7135.5 * 2.0 * 1024 + 16.0 * 1024, _ROWS, "9c5848bbce659441"),
+                                           _LANES, "472f0d74c39d2277"),
+    "down_proj_5120x17408_m1_student_t_packed": (23032.0 * 2.0 * 1024 + 16.0 * 1024, _ROWS, "c9d70b0faeabf7ee"),
+    "gate_up_17408x5120_m1_student_t_packed": (22935.9 * 2.0 * 1024 + 40.0 * 1024, _ROWS, "c9d70b0faeabf7ee"),
+    "attn_proj_5120x5120_m1_student_t_packed": (7135.5 * 2.0 * 1024 + 16.0 * 1024, _ROWS, "c9d70b0faeabf7ee"),
     "down_proj_5120x17408_m1_calibrated_packed": (33834.1 * 2.0 * 1024 + 40.0 * 1024, _DENSE, "1f7c6b74b169a3de"),
     "down_proj_5120x17408_m1_five_level_calibrated_packed": (49695.3 * 2.0 * 1024 + 1328.6 * 1024, _DENSE5, "5b2d5307061aed1f"),
     "gate_up_17408x5120_m4_student_t_packed": (28703.1 * 2.0 * 1024 + 160.0 * 1024, _TILES, "e4518543e34fde14"),
@@ -92,13 +92,13 @@ MEASURED_TRAFFIC_BYTES = {
 # rocprofv3 --pmc run of this script, mean over the launches), gated by the hash of the kernel's sources like the
 # traffic figures.  Reported per weight: vector and LDS instructions x 64 lanes / weights, scalar instructions / weights.
 MEASURED_INSTRUCTIONS = {
-    "down_proj_5120x17408_m1_student_t": ((3414116.0, 2201438.0, 819680.0), _LANES, "e5dd4cabcbebf53f"),
-    "down_proj_5120x17408_m1_calibrated": ((4829187.0, 3166052.0, 918004.0), _LANES, "e5dd4cabcbebf53f"),
-    "down_proj_5120x17408_m1_five_level_calibrated": ((4829187.0, 3166052.0, 918004.0), _LANES, "e5dd4cabcbebf53f"),
-    "down_proj_5120x17408_m1_student_t_packed": ((5734195.0, 4469166.0, 1360042.0), _ROWS, "9c5848bbce659441"),
-    "gate_up_17408x5120_m1_student_t_packed": ((6030194.0, 4450915.0, 1414314.0), _ROWS, "9c5848bbce659441"),
-    "attn_proj_5120x5120_m1_student_t_packed": ((3570752.0, 2281697.0, 593732.0), _ROWS, "9c5848bbce659441"),
-    "down_proj_5120x17408_m1_level1_only_packed": ((4881551.0, 4104235.0, 1254926.0), _ROWS, "9c5848bbce659441"),
+    "down_proj_5120x17408_m1_student_t": ((3414116.0, 2201438.0, 819680.0), _LANES, "472f0d74c39d2277"),
+    "down_proj_5120x17408_m1_calibrated": ((4829187.0, 3166052.0, 918004.0), _LANES, "472f0d74c39d2277"),
+    "down_proj_5120x17408_m1_five_level_calibrated": ((4829187.0, 3166052.0, 918004.0), _LANES, "472f0d74c39d2277"),
+    "down_proj_5120x17408_m1_student_t_packed": ((5734195.0, 4469166.0, 1360042.0), _ROWS, "c9d70b0faeabf7ee"),
+    "gate_up_17408x5120_m1_student_t_packed": ((6030194.0, 4450915.0, 1414314.0), _ROWS, "c9d70b0faeabf7ee"),
+    "attn_proj_5120x5120_m1_student_t_packed": ((3570752.0, 2281697.0, 593732.0), _ROWS, "c9d70b0faeabf7ee"),
+    "down_proj_5120x17408_m1_level1_only_packed": ((4881551.0, 4104235.0, 1254926.0), _ROWS, "c9d70b0faeabf7ee"),
 }
 
 WORKLOADS = {
