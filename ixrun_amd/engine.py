@@ -463,8 +463,8 @@ class StreamingLinear(nn.Module):
 
         ``multiplier`` and ``residual`` are bf16 of the output's shape, or None: the gate of a gated block takes the other half's
         output as its multiplier, a block's last projection the residual stream.  bf16 activations on the layer's device; no gradients.
-        From the lane layout it is one kernel's epilogue; without one, and for 17 and more rows that are no whole 16-byte pieces,
-        ``forward`` runs and the rest follows as a launch of its own, from the product rounded to bf16."""
+        From the lane layout it is one kernel's epilogue (17 and more rows that are no whole 16-byte pieces are copied to such first);
+        without one ``forward`` runs and the rest follows as a launch of its own, from the product rounded to bf16."""
         act = _lib.ACTIVATIONS.get(activation)
         if self._native is not None and self._use_fused and self._gemm_ok and not self._gemv_flags and act is not None:
             index = self._scale.device.index
@@ -509,16 +509,22 @@ class StreamingLinear(nn.Module):
         with _lib.on_device(dev):
             stream = _raw_stream(dev.index if dev.index is not None else torch.cuda.current_device())
             if (self._lanes is not None and self._use_fused and not self._gemv_flags and (self._bias is None or self._bias_ptr)
-                    and (rows <= MAX_FUSED_ROWS or (self._gemm_ok and in_f % 8 == 0))):
-                if rows > MAX_FUSED_ROWS and (x2.data_ptr() % 16 or x2.stride(0) % 8):
+                    and (rows <= MAX_FUSED_ROWS or (self._gemm_ok and out_f * (in_f + 8) < 1 << 31))):
+                lanes = self._lanes.struct
+                if rows > MAX_FUSED_ROWS and in_f % 8:  # whole 16-byte pieces: zeros, against codes of 0 behind the last column
+                    x2 = F.pad(x2, (0, -in_f % 8))
+                    lanes = _lib.IxhLanes.from_buffer_copy(lanes)
+                    lanes.in_f = x2.shape[1]
+                elif rows > MAX_FUSED_ROWS and (x2.data_ptr() % 16 or x2.stride(0) % 8):
                     x2 = x2.clone(memory_format=torch.contiguous_format)
+                lanes = ctypes.byref(lanes)
                 step = min(MAX_PRODUCT_ROWS, max(((1 << 31) - 1) // x2.stride(0), MAX_FUSED_ROWS))
-                need = L.ixh_lanes_product_workspace_bytes(self._lane_ref, min(rows, step))
+                need = L.ixh_lanes_product_workspace_bytes(lanes, min(rows, step))
                 if rows > step and rows % step:  # (fewer rows may cut the columns finer)
-                    need = max(need, L.ixh_lanes_product_workspace_bytes(self._lane_ref, rows % step))
+                    need = max(need, L.ixh_lanes_product_workspace_bytes(lanes, rows % step))
                 ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
                 for at in range(0, rows, step):
-                    _lib.check(L.ixh_lanes_product(self._lane_ref, x2.data_ptr() + 2 * at * x2.stride(0), x2.stride(0), self._bias_ptr,
+                    _lib.check(L.ixh_lanes_product(lanes, x2.data_ptr() + 2 * at * x2.stride(0), x2.stride(0), self._bias_ptr,
                                                    min(step, rows - at), ctypes.byref(epilogue(at)), y.data_ptr() + 2 * at * out_f, out_f,
                                                    ws.data_ptr() if need else None, need, stream))
                 return y

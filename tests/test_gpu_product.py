@@ -212,3 +212,22 @@ def test_a_layer_off_the_gpu_is_refused(dev):
             layer.product(given, "silu")
     layer.to(dev)
     assert torch.equal(layer.product(x, "silu", m, r), want)
+
+
+@pytest.mark.parametrize("out_f,in_f", [(72, 1023), (100, 513), (33, 263), (640, 2049), (5126, 5003)])
+@pytest.mark.parametrize("rows", [17, 40, 150, 520])
+def test_prompts_of_odd_rows(dev, out_f, in_f, rows):
+    """Rows that are no whole 16-byte pieces, one rounding all the same; views of them, and infinities next to what fills them up."""
+    layer, w, bias = _layer(dev, out_f, in_f, "outlier" if out_f < 5000 else "t", bias=True)
+    assert layer._lanes is not None
+    _check(dev, layer, w, bias, rows, "gelu_tanh", True, True)
+    x, m, r = _operands(dev, rows, out_f, in_f, True, True)
+    want = layer.product(x, "silu", m, r)
+    apart = torch.full((rows, in_f + 5), float("nan"), dtype=torch.bfloat16, device=dev)
+    view = apart[:, 3:3 + in_f]
+    view.copy_(x)
+    assert torch.equal(layer.product(view, "silu", m, r), want)
+    x[3, -1] = float("inf")
+    y = layer.product(x, "silu", m, r)
+    same = torch.arange(rows) != 3
+    assert torch.equal(y[same], want[same])
