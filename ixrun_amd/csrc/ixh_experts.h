@@ -59,7 +59,7 @@ struct ExPlan {
 int launch_experts_prompt(const ExDev &X, const ExCall &call, const ExPlan &plan, uint32_t row_tiles, uint32_t blocks, void *xt, void *inner,
                           float *per_slot, hipStream_t s);
 
-// a slot by itself (ixh_experts_one.hip): rows of up to sixteen cells, eight of a gated first matrix
+// a slot by itself (ixh_experts_one.hip): rows of up to sixteen cells
 struct ExOne {
     const uint16_t *x;
     int64_t ldx;

@@ -576,13 +576,12 @@ static uint32_t ex_layers(const ExDev &X, uint32_t slots) {
     return (slots / (2u * kExLayer) + X.experts) * w_tiles <= 3ull * ln_cus() ? 2u : 4u;
 }
 
-// Slots by expert, not one by one: of k_experts_one from 160 cells a CU on (us one by one / planned: 64 experts of 2048 x 1024, 24 / 48 / 72
-// slots, which are 72 / 144 / 216 cells a CU, 34 / 50 / 67, 53 / 54 / 61; 16 of 4096 x 1536, 8 / 16 / 24 slots 31 / 47 / 60, 46 / 52 / 59; 128 of
-// 2048 x 768, 48 / 96 slots 46 / 72, 58 / 69); of k_experts_rows, whose workgroups begin more slowly, where tiles of several slots are likely.
-static bool ex_planned(const ExDev &X, uint32_t slots) {
-    if (!experts_one_takes(X.first, X.gated) || !experts_one_takes(X.second, false)) return slots > X.experts / 4u;
+// Slots one by one, of k_experts_one, up to 160 cells a CU (us one by one / planned: 64 experts of 2048 x 1024, 24 / 48 / 72 slots, which are 72 / 144 /
+// 216 cells a CU, 34 / 50 / 67, 53 / 54 / 61; 16 of 4096 x 1536, 8 / 16 / 24 slots 31 / 47 / 60, 46 / 52 / 59; 128 of 2048 x 768, 48 / 96 slots 46 / 72,
+// 58 / 69; one token by 8 of 7168 x 2048, 168 cells a CU, 58, by k_experts_rows 55; by 2 of 5120 x 1536 20.8, 27).
+static bool ex_one_by_one(const ExDev &X, uint32_t slots) {
     const auto cells = [](const ExMatrix &W) { return (uint64_t)((W.n_tiles + 3u) / 4u) * W.n_cells; };
-    return slots * (cells(X.first) + cells(X.second)) > 160ull * ln_cus();
+    return experts_one_takes(X.first, X.gated) && experts_one_takes(X.second, false) && slots * (cells(X.first) + cells(X.second)) <= 160ull * ln_cus();
 }
 
 // A call's scratch: the plan, the intermediate, what each slot's expert makes of it, and in k_experts_prompt the gathered rows.
@@ -630,7 +629,8 @@ int launch_experts(const ExDev &X, const ExCall &call, void *workspace, hipStrea
     const uint32_t slots = call.tokens * call.top_k;
     const ExScratch w = ex_scratch(X, call.tokens, call.top_k);
     uint8_t *const ws = reinterpret_cast<uint8_t *>(((uintptr_t)workspace + 255u) & ~(uintptr_t)255u);
-    const bool planned = w.many || (call.tokens > 1u && ex_planned(X, slots));
+    // (else k_experts_rows: by expert where tiles of several slots are likely)
+    const bool apart = !w.many && ex_one_by_one(X, slots), planned = w.many || (!apart && call.tokens > 1u && slots > X.experts / 4u);
     const uint32_t n_tiles = planned ? w.n_tiles : slots;
     uint32_t *const counts = reinterpret_cast<uint32_t *>(ws);
     const ExPlan plan{counts, counts + 1, reinterpret_cast<uint32_t *>(ws + w.tiles), reinterpret_cast<uint32_t *>(ws + w.order)};
@@ -650,19 +650,20 @@ int launch_experts(const ExDev &X, const ExCall &call, void *workspace, hipStrea
         R.x = call.x, R.ldx = call.ldx, R.ids = call.ids, R.experts = X.experts, R.top_k = call.top_k, R.slots = slots;
         if (planned) R.n_tiles = plan.n_tiles, R.tiles = plan.tiles, R.order = plan.order;
         R.out = ws + w.inner, R.ld_out = w.ld_inner, R.activation = X.activation, R.gated = X.gated;
-        ExOne one{call.x, call.ldx, call.tokens, call.ids, R.out, R.ld_out, X.experts, call.tokens, call.top_k, X.activation, X.gated, call.weights, call.residual, call.ld_residual};
-        if (!planned && experts_one_takes(X.first, X.gated)) rc = launch_experts_one(X.first, one, true, s);
+        ExOne one{call.x, call.ldx, call.tokens, call.ids, R.out, R.ld_out, X.experts, call.tokens, call.top_k, X.activation, X.gated,
+                  call.weights, call.residual, call.ld_residual};
+        if (apart) rc = launch_experts_one(X.first, one, true, s);
         else rc = ex_matrix<true>(X.first, R, planned ? w.rows : 1u, n_tiles, s);
         if (rc != IXH_OK) return rc;
         R.x = reinterpret_cast<const uint16_t *>(ws + w.inner), R.ldx = w.ld_inner;
         R.out = per_slot, R.ld_out = X.hidden;
         one.x = R.x, one.ldx = R.ldx, one.rows = slots;
-        if (!planned && experts_joined_takes(X.second, call.tokens, call.top_k)) {
+        if (apart && experts_joined_takes(X.second, call.tokens, call.top_k)) {
             one.out = call.y, one.ld_out = call.ldy;
             return launch_experts_joined(X.second, one, s);
         }
         one.out = R.out, one.ld_out = R.ld_out;
-        if (!planned && experts_one_takes(X.second, false)) rc = launch_experts_one(X.second, one, false, s);
+        if (apart) rc = launch_experts_one(X.second, one, false, s);
         else rc = ex_matrix<false>(X.second, R, planned ? w.rows : 1u, n_tiles, s);
     }
     if (rc != IXH_OK) return rc;

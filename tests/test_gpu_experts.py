@@ -351,7 +351,7 @@ def test_experts_by_tiles(dev, recipe, level_bits, experts, hidden, inner, token
 
 
 @pytest.mark.parametrize("recipe,level_bits", [("t", (3, 5, 8)), ("real", (3, 5, 8)), ("outlier", (4, 8)), ("real", (6, 8))])
-@pytest.mark.parametrize("hidden,inner", [(2048, 1024), (8, 8), (4096, 33), (1037, 520), (4090, 700)])
+@pytest.mark.parametrize("hidden,inner", [(2048, 1024), (8, 8), (4096, 33), (1037, 520), (4090, 700), (4100, 64), (7160, 130), (8192, 72)])
 def test_experts_one_by_one(dev, recipe, level_bits, hidden, inner):
     """Slots by themselves: rows of one to eight cells, the same expert in several slots and twice in a token, places without one, rows of any
     alignment, a row of infinities beside others."""
