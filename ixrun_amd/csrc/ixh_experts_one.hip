@@ -16,7 +16,7 @@ namespace ixh {
 // there, 9.1 / 6.9 us here (1.6 TB/s with their starts and ends).
 //
 // JOIN, the second matrix for a few tokens: a workgroup has a block of rows of all of a token's slots, with a pair table and activations for
-// each, and ends with the sum over them, in their order, so that no launch follows: 20.0 -> 18.3 us for that token (second matrix and sum 6.9 + 2.7 -> 8.5).
+// each, and ends with the sum over them, in their order, so that no launch follows: 20.0 -> 17.8 us for that token (second matrix and sum 6.9 + 2.7 -> 8.5).
 // ---------------------------------------------------------------------------------------------------------------
 struct EoJoin {  // what a token's outputs are made with
     const float *weights;
