@@ -13,6 +13,7 @@ _split_chunk, _use_fused, _w_buf``), which callers of ``fused_gemv`` read.
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes
 import gc
 import os
@@ -528,7 +529,11 @@ class StreamingLinear(nn.Module):
                                                    min(step, rows - at), ctypes.byref(epilogue(at)), y.data_ptr() + 2 * at * out_f, out_f,
                                                    ws.data_ptr() if need else None, need, stream))
                 return y
-            v = self.forward(x2)
+            # (autocast may have a library product in another type than the bf16 that the epilogue reads)
+            with torch.autocast("cuda", enabled=False) if torch.is_autocast_enabled("cuda") else contextlib.nullcontext():
+                v = self.forward(x2)
+            if v.dtype is not torch.bfloat16 or v.shape != (rows, out_f) or v.stride(1) != 1:
+                raise RuntimeError(f"the layer's product is {v.dtype} {tuple(v.shape)}, expected bf16 {(rows, out_f)} in rows")
             _lib.check(L.ixh_epilogue(v.data_ptr(), v.stride(0), rows, out_f, ctypes.byref(epilogue(0)), y.data_ptr(), out_f, stream))
         return y
 

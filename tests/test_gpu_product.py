@@ -231,3 +231,24 @@ def test_prompts_of_odd_rows(dev, out_f, in_f, rows):
     y = layer.product(x, "silu", m, r)
     same = torch.arange(rows) != 3
     assert torch.equal(y[same], want[same])
+
+
+@pytest.mark.parametrize("rows", [1, 9, 33])
+@pytest.mark.parametrize("how", ["lanes", "no lanes", "fp32 bias", "packed streams", "decode and multiply"])
+def test_products_under_autocast(dev, rows, how):
+    """The product is bf16 whatever type autocast would have a library product in: of every way a layer takes, the result without it."""
+    layer, w, bias = _layer(dev, 72, 1024, "outlier", bias=True, lanes=how != "no lanes")
+    layer._set_shared_buf(torch.empty(layer.N, dtype=torch.bfloat16, device=dev))
+    if how == "fp32 bias":
+        layer._bias = layer._bias.float()
+        layer._bind()
+    layer._use_fused = how != "packed streams"
+    layer._gemm_ok = how != "decode and multiply"
+    x, m, r = _operands(dev, rows, 72, 1024, True, True)
+    want = layer.product(x, "silu", m, r)
+    _close(want, *ref.epilogue(x, w, bias, "silu", m, r, apart=how != "lanes"))
+    for dtype in (torch.float16, torch.bfloat16):
+        with torch.autocast("cuda", dtype=dtype):
+            got = layer.product(x, "silu", m, r)
+            assert torch.is_autocast_enabled("cuda") and torch.get_autocast_dtype("cuda") is dtype
+        assert got.dtype is torch.bfloat16 and torch.equal(got, want)
