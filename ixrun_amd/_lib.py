@@ -12,6 +12,7 @@ import ctypes as C
 import os
 
 import torch
+from torch.autograd import forward_ad
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
 # IXH_LIB names another build of the library (development); the default is the in-tree one
@@ -289,6 +290,17 @@ def _require_cuda(t: torch.Tensor, what: str) -> None:
         raise RuntimeError(f"{what} must live on the GPU (got {t.device}); the HIP path has no CPU fallback")
     if not t.is_contiguous():
         raise RuntimeError(f"{what} must be contiguous")
+
+
+def inference_only(name: str, *tensors) -> None:
+    """Refuse tensors whose derivative is asked for, in either mode: an operator without one would drop it in silence."""
+    for t in tensors:
+        if t is None:
+            continue
+        if t.requires_grad and torch.is_grad_enabled():
+            raise RuntimeError(f"{name} has no gradient: call it under torch.no_grad(), or with tensors that need none")
+        if forward_ad._current_level >= 0 and forward_ad.unpack_dual(t).tangent is not None:  # (which no_grad leaves on)
+            raise RuntimeError(f"{name} has no gradient, of forward mode either: unpack the dual tensors first")
 
 
 class DevicePacked:

@@ -506,10 +506,11 @@ PyObject *encode(PyObject *, PyObject *const *args, Py_ssize_t n_args) {
     END_HANDLE_TH_ERRORS
 }
 
-// A contiguous tensor of this type on the current device that asks for no gradient; null for anything else.
+// A contiguous tensor of this type on the current device that asks for no gradient, outside of forward mode (whose tangents Python looks for);
+// null for anything else.
 const at::Tensor *given(PyObject *o, at::ScalarType type, int64_t device) {
     const at::Tensor *t = plain(o, type, device);
-    return t && !(t->requires_grad() && c10::GradMode::is_enabled()) ? t : nullptr;
+    return t && !(t->requires_grad() && c10::GradMode::is_enabled()) && !torch::autograd::ForwardADLevel::try_get_by_idx(0) ? t : nullptr;
 }
 bool alike(const at::Tensor &a, const at::Tensor &b, int64_t last) {  // the same leading dimensions, and `last`
     return a.dim() == b.dim() && a.size(-1) == last && a.sizes().slice(0, a.dim() - 1) == b.sizes().slice(0, b.dim() - 1);

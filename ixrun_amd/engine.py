@@ -479,8 +479,7 @@ class StreamingLinear(nn.Module):
                 raise TypeError(f"{name} must be bf16 (got {t.dtype})")
             if t.device != self._scale.device or not t.is_cuda:
                 raise RuntimeError(f"{name} must live on the layer's GPU (got {t.device}, layer on {self._scale.device}); the HIP path has no CPU fallback")
-            if t.requires_grad and torch.is_grad_enabled():
-                raise RuntimeError("StreamingLinear.product has no gradient: call it under torch.no_grad(), or with tensors that need none")
+            _lib.inference_only("StreamingLinear.product", t)
         if activation not in _lib.ACTIVATIONS:
             raise ValueError(f"activation {activation!r} is none of {[a for a in _lib.ACTIVATIONS if a]}")
         in_f, out_f, dev = self.in_features, self.out_features, x.device

@@ -24,11 +24,6 @@ MOST_EXPERTS = 1024
 MOST_PLACES = 1 << 17  # tokens times experts of each in one call of the library: bounds the call's scratch
 
 
-def _inference_only(name: str, *tensors) -> None:
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
-        raise RuntimeError(f"{name} has no gradient: call it under torch.no_grad(), or with tensors that need none")
-
-
 def route_experts(logits, top_k: int, *, scoring: str = "softmax", bias=None, n_groups: int = 1, top_groups: int | None = None,
                   renormalize: bool = True, scale: float = 1.0):
     """The experts of each token and their weights: ``(ids int32 [..., top_k], weights fp32 [..., top_k])``, best first.
@@ -45,7 +40,7 @@ def route_experts(logits, top_k: int, *, scoring: str = "softmax", bias=None, n_
     done = _lib.host().route(logits, bias, top_k, n_groups, top_groups, SCORINGS.get(scoring), renormalize, scale)
     if done is not None:
         return done
-    _inference_only("route_experts", logits, bias)
+    _lib.inference_only("route_experts", logits, bias)
     if not logits.is_cuda:
         raise RuntimeError(f"logits must live on the GPU (got {logits.device}); the HIP path has no CPU fallback")
     if logits.dtype not in LOGIT_TYPES:
@@ -256,7 +251,7 @@ class StreamingExperts(nn.Module):
             y = _lib.host().experts(self._struct_at, self._device_index, MOST_PLACES, x, ids, weights, residual)
             if y is not None:
                 return y
-        _inference_only("StreamingExperts", x, weights, residual)
+        _lib.inference_only("StreamingExperts", x, weights, residual)
         if self._struct is None:
             raise RuntimeError(f"the layer is on {self._first_plane.device}; the HIP path has no CPU fallback")
         dev = self._first_plane.device

@@ -112,3 +112,19 @@ def test_python_refuses_what_is_not_on_the_gpu_or_has_a_gradient():
         route_experts(torch.zeros(2, 8), 2)
     with pytest.raises(RuntimeError, match="no gradient"):
         route_experts(torch.zeros(2, 8, requires_grad=True), 2)
+
+
+def test_dual_tensors_are_refused_wherever_they_live():
+    from torch.autograd import forward_ad
+
+    x = torch.zeros(2, 4)
+    with forward_ad.dual_level():
+        dual = forward_ad.make_dual(x, x + 1)
+        for grad in (torch.enable_grad, torch.no_grad):
+            with grad():
+                _lib.inference_only("this", x, None, torch.zeros(3, dtype=torch.int32))
+                with pytest.raises(RuntimeError, match="this has no gradient"):
+                    _lib.inference_only("this", x, dual)
+                with pytest.raises(RuntimeError, match="no gradient"):
+                    route_experts(dual, 2)
+    _lib.inference_only("this", x)

@@ -493,3 +493,25 @@ def test_two_calls_at_once_and_graphs_in_turn(dev):
             layer(*calls[turn % 3])
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for a, b in zip(outs, want))
+
+
+def test_dual_tensors_are_refused(dev):
+    """A tangent is not dropped in silence; other tensors are routed and multiplied inside a forward-mode level as anywhere."""
+    from torch.autograd import forward_ad
+
+    from ixrun_amd import route_experts
+
+    layer, _ = _layer(dev, 4, 64, 16)
+    x, ids, weights, residual = _call(dev, 3, 2, 4, 64, residual=True)
+    logits, bias = torch.randn(3, 4, device=dev), torch.randn(4, device=dev)
+    want, routed = layer(x, ids, weights, residual), route_experts(logits, 2, bias=bias)
+    with forward_ad.dual_level():
+        assert torch.equal(layer(x, ids, weights, residual), want)
+        assert all(torch.equal(a, b) for a, b in zip(route_experts(logits, 2, bias=bias), routed))
+        dual = lambda t: forward_ad.make_dual(t, torch.ones_like(t))
+        calls = [lambda: layer(dual(x), ids, weights, residual), lambda: layer(x, ids, dual(weights), residual), lambda: layer(x, ids, weights, dual(residual)),
+                 lambda: route_experts(dual(logits), 2), lambda: route_experts(logits, 2, bias=dual(bias))]
+        for call in calls:
+            for grad in (torch.enable_grad, torch.no_grad):
+                with grad(), pytest.raises(RuntimeError, match="no gradient"):
+                    call()

@@ -252,3 +252,21 @@ def test_products_under_autocast(dev, rows, how):
             got = layer.product(x, "silu", m, r)
             assert torch.is_autocast_enabled("cuda") and torch.get_autocast_dtype("cuda") is dtype
         assert got.dtype is torch.bfloat16 and torch.equal(got, want)
+
+
+@pytest.mark.parametrize("lanes", [True, False])
+@pytest.mark.parametrize("rows", [1, 33])
+def test_products_of_dual_tensors_are_refused(dev, lanes, rows):
+    """A tangent is not dropped in silence; other tensors are multiplied inside a forward-mode level as anywhere."""
+    from torch.autograd import forward_ad
+
+    layer, _, _ = _layer(dev, 64, 128, lanes=lanes)
+    given = _operands(dev, rows, 64, 128, True, True)
+    want = layer.product(given[0], "silu", *given[1:])
+    with forward_ad.dual_level():
+        assert torch.equal(layer.product(given[0], "silu", *given[1:]), want)
+        for i in range(3):
+            duals = [forward_ad.make_dual(t, torch.ones_like(t)) if i == j else t for j, t in enumerate(given)]
+            for grad in (torch.enable_grad, torch.no_grad):
+                with grad(), pytest.raises(RuntimeError, match="no gradient"):
+                    layer.product(duals[0], "silu", *duals[1:])
