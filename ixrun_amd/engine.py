@@ -78,6 +78,12 @@ def _plain_call(x) -> bool:
             and (not torch.is_autocast_enabled("cuda") or torch.get_autocast_dtype("cuda") is torch.bfloat16))
 
 
+def _product_rows(stride: int) -> int:
+    """Most activation rows of one call of ``ixh_lanes_product``, which takes more than ``MAX_FUSED_ROWS`` of a stride below
+    2**31 // rows only."""
+    return min(MAX_PRODUCT_ROWS, max((1 << 31) // (stride + 1), MAX_FUSED_ROWS))
+
+
 def _lane_bytes(level_bits, out_f, in_f, counts) -> int:
     """Bytes of a layer's lane layout, to within the unevenness of its rows; 0 where it would take more than the bf16 weight
     (see ``StreamingLinear._make_lanes``)."""
@@ -518,7 +524,7 @@ class StreamingLinear(nn.Module):
                 elif rows > MAX_FUSED_ROWS and (x2.data_ptr() % 16 or x2.stride(0) % 8):
                     x2 = x2.clone(memory_format=torch.contiguous_format)
                 lanes = ctypes.byref(lanes)
-                step = min(MAX_PRODUCT_ROWS, max(((1 << 31) - 1) // x2.stride(0), MAX_FUSED_ROWS))
+                step = _product_rows(x2.stride(0))
                 need = L.ixh_lanes_product_workspace_bytes(lanes, min(rows, step))
                 if rows > step and rows % step:  # (fewer rows may cut the columns finer)
                     need = max(need, L.ixh_lanes_product_workspace_bytes(lanes, rows % step))

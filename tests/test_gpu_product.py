@@ -270,3 +270,12 @@ def test_products_of_dual_tensors_are_refused(dev, lanes, rows):
             for grad in (torch.enable_grad, torch.no_grad):
                 with grad(), pytest.raises(RuntimeError, match="no gradient"):
                     layer.product(duals[0], "silu", *duals[1:])
+
+
+def test_prompts_at_a_long_stride_are_taken_in_parts(dev):
+    """4096 rows 1 MB apart: a part more than 32-bit offsets hold."""
+    layer, w, bias = _layer(dev, 96, 256, "t", bias=True)
+    far = torch.zeros((4096, 524672), dtype=torch.bfloat16, device=dev)
+    x, m, r = _operands(dev, 4096, 96, 256, True, True)
+    far[:, :256] = x
+    _close(layer.product(far[:, :256], "silu", m, r), *ref.epilogue(x, w, bias, "silu", m, r))

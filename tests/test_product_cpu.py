@@ -48,3 +48,25 @@ def test_malformed_epilogues_are_refused(change, needle):
     assert lib.ixh_epilogue(a["v"], a["ldv"], a["m"], a["out_f"], C.byref(ep), a["y"], a["ldy"], None) == -1
     assert needle in lib.ixh_last_error().decode()
     assert lib.ixh_epilogue(None, 0, 0, 8, C.byref(_lib.IxhEpilogue(0, None, 0, None, 0)), None, 0, None) == 0
+
+
+def test_parts_of_a_long_call_are_taken_at_any_stride():
+    """Every part that StreamingLinear.product makes passes the boundary's look at the stride (the call ends at the missing scratch), and one
+    row more does not."""
+    from ixrun_amd.engine import MAX_FUSED_ROWS, MAX_PRODUCT_ROWS, _product_rows
+
+    lib = _lib.lib()
+    ep = _lib.IxhEpilogue(1, None, 0, None, 0)
+    lanes = _lanes(8192, 8192)
+
+    def code(rows, stride):
+        assert lib.ixh_lanes_product_workspace_bytes(C.byref(lanes), rows) > 0  # (without which nothing is launched)
+        return lib.ixh_lanes_product(C.byref(lanes), 0x1000, stride, None, rows, C.byref(ep), 0x1000, 8192, None, 0, None)
+
+    borders = {(1 << 31) // rows // 8 * 8 + d for rows in range(130, MAX_PRODUCT_ROWS + 1, 7) for d in (-8, 0, 8)}
+    for stride in sorted(borders | {8192, 524672, 1 << 20, 1 << 24}):
+        rows = _product_rows(stride)
+        if rows > 128:
+            assert code(rows, stride) == -4, (rows, stride)
+            assert rows == MAX_PRODUCT_ROWS or code(rows + 1, stride) == -2, (rows, stride)
+    assert _product_rows(8192) == MAX_PRODUCT_ROWS and _product_rows(1 << 40) == MAX_FUSED_ROWS
