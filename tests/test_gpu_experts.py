@@ -515,3 +515,55 @@ def test_dual_tensors_are_refused(dev):
             for grad in (torch.enable_grad, torch.no_grad):
                 with grad(), pytest.raises(RuntimeError, match="no gradient"):
                     call()
+
+
+def _experts_of_columns(x, ids, weights, residual, gate_up, down, gate_up_bias, down_bias):
+    """ref.experts of gated ReLU experts, over those columns of x and of the intermediate that are not 0 everywhere."""
+    y = torch.zeros(x.shape[0], down.shape[1], dtype=torch.float64, device=x.device)
+    off, size = torch.zeros_like(y), torch.zeros_like(y)
+    for e in range(down.shape[0]):
+        t, j = torch.nonzero(ids == e, as_tuple=True)
+        (g, dg), (u, du) = (ref.product(x[t], w, b) for w, b in zip(gate_up[e].chunk(2), gate_up_bias[e].chunk(2)))
+        a, da = ref.activated(g, dg, "relu")
+        h, dh = ref.rounded(a * u, da * (u.abs() + du) + a.abs() * du + ref.U32 * (a * u).abs())
+        v, dv = ref.product(h, down[e], down_bias[e])
+        dv = dv + dh @ down[e].double().abs().t()
+        w = weights[t, j].double().unsqueeze(1)
+        y.index_add_(0, t, w * v)
+        off.index_add_(0, t, w.abs() * dv)
+        size.index_add_(0, t, (w * v).abs())
+    y = y + residual.double()
+    off = off + (ids.shape[1] + 2) * ref.U32 * size + ref.U32 * y.abs()
+    return y, off + ref.U16 * (y.abs() + off)
+
+
+@pytest.mark.parametrize("recipe,level_bits", [("t", (3, 5, 8)), ("outlier", (4, 8)), ("real", (3, 5, 8)), ("real", (6, 8))])
+@pytest.mark.parametrize("hidden,inner", [(32767, 16), (32768, 8), (33001, 24), (66000, 9), (24, 33001), (16, 66048)])
+def test_experts_of_rows_whose_positions_start_over(dev, recipe, level_bits, hidden, inner):
+    """Rows of 64 cells and more, where a list's positions count from column 32768 n on and places without an element point at 0: slots by
+    themselves, tiles of a few, and many tokens to an expert.  All columns but a hundred of the long rows are 0, which adds nothing to a sum and
+    so nothing to its bound: an element that is multiplied with another column's activation is far outside."""
+    layer, dense = _repeated_layer(dev, 4, hidden, inner, recipe, level_bits, distinct=2, activation="relu")
+    long = max(hidden, inner)
+    borders = [c + d for c in (0, 512, 32256, 32768, 33280, 65536, long) for d in (-2, -1, 0, 1, 31)]
+    some = torch.randperm(long, generator=torch.Generator().manual_seed(long))[:70].tolist()
+    at = torch.tensor(sorted({c for c in borders + some if 0 <= c < long}), device=dev)
+    none = torch.ones(long, dtype=torch.bool, device=dev)
+    none[at] = False
+    gate_up, down, bias = dense["gate_up"], dense["down"], layer._first_bias
+    if hidden == long:
+        gate_up = gate_up[:, :, at]
+    else:  # the gate is closed elsewhere
+        bias[:, :inner][:, none] = -1000.0
+        both = torch.cat([at, at + inner])
+        gate_up, down, bias = gate_up[:, both], down[:, :, at], bias[:, both]
+    for tokens, top_k in ((1, 2), (9, 3), (21, 2), (30, 2)):
+        x, ids, weights, residual = _call(dev, tokens, top_k, 4, hidden, seed=tokens, residual=True)
+        if hidden == long:
+            x[:, none] = 0.0
+        y = layer(x, ids, weights, residual)
+        _close(y, *_experts_of_columns(x[:, at] if hidden == long else x, ids, weights, residual, gate_up, down, bias, dense["down_bias"]))
+        if tokens > 1:  # the column that places without an element point at, too
+            x[tokens // 2, 0] = math.inf
+            same = torch.arange(tokens) != tokens // 2
+            assert torch.equal(layer(x, ids, weights, residual)[same], y[same])
