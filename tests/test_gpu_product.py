@@ -260,8 +260,10 @@ def test_products_of_dual_tensors_are_refused(dev, lanes, rows):
     """A tangent is not dropped in silence; other tensors are multiplied inside a forward-mode level as anywhere."""
     from torch.autograd import forward_ad
 
-    layer, _, _ = _layer(dev, 64, 128, lanes=lanes)
-    given = _operands(dev, rows, 64, 128, True, True)
+    layer, _, _ = _layer(dev, 64, 1024, lanes=lanes)
+    layer._set_shared_buf(torch.empty(layer.N, dtype=torch.bfloat16, device=dev))
+    assert (layer._lanes is not None) == lanes
+    given = _operands(dev, rows, 64, 1024, True, True)
     want = layer.product(given[0], "silu", *given[1:])
     with forward_ad.dual_level():
         assert torch.equal(layer.product(given[0], "silu", *given[1:]), want)
