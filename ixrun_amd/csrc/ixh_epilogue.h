@@ -90,8 +90,10 @@ int launch_epilogue(const uint16_t *v, int64_t ldv, uint32_t m, uint32_t out_f, 
 #define EP(name) name##_ep
 #define EP_PARAM , Epilogue ep
 #define EP_ARG , ep
+#define EP_OUT  // (the outputs may be the multiplier or the residual)
 #else
 #define EP(name) name
 #define EP_PARAM
 #define EP_ARG
+#define EP_OUT __restrict__
 #endif

@@ -27,7 +27,7 @@ template <int BITS, bool FIRST, bool JOIN, int CELLS>
 __global__ void __launch_bounds__(1024)
 k_experts_one(const int32_t *__restrict__ ids, const uint32_t *__restrict__ plane, const uint16_t *__restrict__ x, const uint32_t *__restrict__ exc_off,
               const uint16_t *__restrict__ scale_at, uint32_t shape, uint32_t n_tiles, uint32_t plane_words, uint32_t experts, uint32_t in_f, int64_t ldx,
-              const uint16_t *__restrict__ exc_pos, const int8_t *__restrict__ exc_val, const uint16_t *__restrict__ bias, void *__restrict__ out,
+              const uint16_t *__restrict__ exc_pos, const int8_t *__restrict__ exc_val, const uint16_t *__restrict__ bias, void *out,
               int64_t ld_out, uint32_t outputs, int activation, EoJoin join) {
     extern __shared__ __attribute__((aligned(16))) uint8_t eo_smem[];
     using P = LnPairs<BITS, false>;

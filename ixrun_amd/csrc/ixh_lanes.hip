@@ -82,7 +82,7 @@ constexpr uint32_t kLnXPad = 64;      // bytes behind a row of activations in LD
     const uint32_t *__restrict__ plane, const uint16_t *__restrict__ x, const uint32_t *__restrict__ exc_off,                            \
         const uint16_t *__restrict__ scale_at, uint32_t shape, uint32_t all_tiles, uint32_t tiles_per_wg, uint32_t in_f,                 \
         uint32_t inv_tiles, uint32_t list_groups, const uint16_t *__restrict__ exc_pos, const int8_t *__restrict__ exc_val, int64_t ldx, \
-        const uint16_t *__restrict__ bias, uint16_t *__restrict__ y, int64_t ldy, uint32_t out_f EP_PARAM
+        const uint16_t *__restrict__ bias, uint16_t *EP_OUT y, int64_t ldy, uint32_t out_f EP_PARAM
 template <int BITS, int MT, bool WIDE, bool BY_WAVE> __device__ __forceinline__ void lv_gemv(LV_ARGUMENTS) {
     extern __shared__ __attribute__((aligned(16))) uint8_t ln_smem[];
     const uint32_t smem = (uint32_t)(uintptr_t)(LN_LDS(uint8_t) *)ln_smem;
@@ -390,7 +390,7 @@ __global__ void __launch_bounds__(1024)
 EP(k_lanes_gemv_few)(const uint32_t *__restrict__ plane, const uint16_t *__restrict__ x, const uint32_t *__restrict__ exc_off,
                  const uint16_t *__restrict__ scale_at, const uint16_t *__restrict__ bias, uint32_t shape, uint32_t inv_cells,
                  uint32_t out_f, uint32_t in_f, const uint16_t *__restrict__ exc_pos, const int8_t *__restrict__ exc_val,
-                 int64_t ldx, uint16_t *__restrict__ y, int64_t ldy EP_PARAM) {
+                 int64_t ldx, uint16_t *EP_OUT y, int64_t ldy EP_PARAM) {
     extern __shared__ __attribute__((aligned(16))) uint8_t ln_smem[];
     using P = LnPairs<BITS, false>;
     const uint32_t smem = (uint32_t)(uintptr_t)(LN_LDS(uint8_t) *)ln_smem;
@@ -530,7 +530,7 @@ EP(k_lanes_gemv_few)(const uint32_t *__restrict__ plane, const uint16_t *__restr
 // outputs from the slices' sums, in slice order
 __global__ void __launch_bounds__(256)
 EP(k_lanes_reduce)(const float *__restrict__ ws, uint32_t slices, int m, uint32_t out_f, uint32_t ws_ld,
-               const uint16_t *__restrict__ bias, bool once, uint16_t *__restrict__ y, int64_t ldy EP_PARAM) {
+               const uint16_t *__restrict__ bias, bool once, uint16_t *EP_OUT y, int64_t ldy EP_PARAM) {
     const uint32_t row = blockIdx.x * 256u + threadIdx.x, r = blockIdx.y;
     if (row >= out_f) return;
     const float *p = ws + (size_t)r * ws_ld + row;

@@ -64,7 +64,7 @@ __global__ void __launch_bounds__(kLgBlocks *kWave)
 EP(k_lanes_gemm)(const uint32_t *__restrict__ plane, const uint16_t *__restrict__ x, const uint16_t *__restrict__ scale_at, uint32_t c_share,
              uint32_t c_more, uint32_t b_share, uint32_t b_more, uint32_t in_f, uint32_t ldx, uint32_t m_all, uint32_t most_at_once, uint32_t n_cells, uint32_t n_tiles,
              const uint32_t *__restrict__ exc_off, const uint16_t *__restrict__ exc_pos, const int8_t *__restrict__ exc_val, uint32_t out_f,
-             float *__restrict__ ws, bool ws_aligned, const uint16_t *__restrict__ bias, bool once, uint16_t *__restrict__ y, int64_t ldy EP_PARAM) {
+             float *__restrict__ ws, bool ws_aligned, const uint16_t *__restrict__ bias, bool once, uint16_t *EP_OUT y, int64_t ldy EP_PARAM) {
     extern __shared__ __attribute__((aligned(16))) uint8_t lg_smem[];
     using P = LnPairs<BITS, kLgWide<BITS>>;
     constexpr uint32_t kTile = kLgTileBytes;

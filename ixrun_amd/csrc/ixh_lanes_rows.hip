@@ -39,7 +39,7 @@ EP(k_lanes_rows)(const uint32_t *__restrict__ plane, const uint16_t *__restrict_
              const uint16_t *__restrict__ scale_at, uint32_t n_cells, uint32_t n_tiles, uint32_t in_f, uint32_t shape,
              uint32_t cells_split, uint32_t blocks_split, const uint16_t *__restrict__ exc_pos, const int8_t *__restrict__ exc_val,
              int64_t ldx, uint32_t out_f, uint32_t x_rows, float *__restrict__ ws, const uint16_t *__restrict__ bias,
-             uint16_t *__restrict__ y, int64_t ldy EP_PARAM) {
+             uint16_t *EP_OUT y, int64_t ldy EP_PARAM) {
     extern __shared__ __attribute__((aligned(16))) uint8_t lr_smem[];
     using P = LnPairs<BITS, WIDE>;
     const uint32_t smem = (uint32_t)(uintptr_t)(LN_LDS(uint8_t) *)lr_smem;

@@ -281,3 +281,52 @@ def test_prompts_at_a_long_stride_are_taken_in_parts(dev):
     x, m, r = _operands(dev, 4096, 96, 256, True, True)
     far[:, :256] = x
     _close(layer.product(far[:, :256], "silu", m, r), *ref.epilogue(x, w, bias, "silu", m, r))
+
+
+@pytest.mark.parametrize("out_f,in_f,rows", [(256, 512, 1), (2000, 520, 3), (640, 4608, 7), (1001, 2056, 13), (4096, 11008, 13), (40960, 2048, 3), (4096, 36864, 2),
+                                             (72, 1024, 40), (17408, 1024, 100), (12288, 6144, 530), (5126, 5120, 300)])
+def test_products_write_over_their_operands(dev, out_f, in_f, rows):
+    """The C entry: multiplier and residual may be y itself, and what lies behind the rows stays."""
+    import ctypes as C
+
+    from ixrun_amd import _lib
+
+    layer, _, bias = _layer(dev, out_f, in_f, "t" if out_f * in_f > 1 << 22 else "outlier", bias=True)
+    x, m, r = _operands(dev, rows, out_f, in_f, True, True)
+    need = _lib.lib().ixh_lanes_product_workspace_bytes(layer._lane_ref, rows)
+    ws = torch.empty(max(need, 1), dtype=torch.uint8, device=dev)
+    for pad in (0, 3, 8):
+        for over in ("multiplier", "residual", "both"):
+            ld = out_f + pad
+            held = torch.full((rows + 1, ld), 7.0, dtype=torch.bfloat16, device=dev)
+            first, second = (m, r) if over != "both" else (m, m)
+            held[:rows, :out_f] = second if over == "residual" else first
+            want = layer.product(x, "gelu_tanh", first, second)
+            at, other = held.data_ptr(), (r if over == "multiplier" else m)
+            ep = _lib.IxhEpilogue(3, at if over != "residual" else other.data_ptr(), ld if over != "residual" else out_f,
+                                  at if over != "multiplier" else other.data_ptr(), ld if over != "multiplier" else out_f)
+            _lib.check(_lib.lib().ixh_lanes_product(layer._lane_ref, x.data_ptr(), in_f, bias.data_ptr(), rows, C.byref(ep), at, ld, ws.data_ptr(), need,
+                                                    _lib.current_stream(dev)))
+            assert torch.equal(held[:rows, :out_f], want)
+            assert bool((held[rows] == 7).all()) and bool((held[:, out_f:] == 7).all())
+
+
+@pytest.mark.parametrize("m,out_f,pad", [(1, 1, 0), (3, 300, 5), (70, 1024, 0), (700, 33, 3)])
+def test_epilogues_write_over_their_operands(dev, m, out_f, pad):
+    import ctypes as C
+
+    from ixrun_amd import _lib
+
+    v, a, b = _operands(dev, m, out_f, out_f, True, True)
+    ld = out_f + pad
+    want = ref.activation(v.double(), "relu") * a.double() + b.double()
+    bound = ref.U16 * want.abs() + 4 * ref.U32 * ((v.double() * a.double()).abs() + b.double().abs())
+    for over in range(3):
+        held = torch.full((m + 1, ld), 7.0, dtype=torch.bfloat16, device=dev)
+        held[:m, :out_f] = (v, a, b)[over]
+        at = [held.data_ptr() if over == i else t.data_ptr() for i, t in enumerate((v, a, b))]
+        lds = [ld if over == i else out_f for i in range(3)]
+        ep = _lib.IxhEpilogue(4, at[1], lds[1], at[2], lds[2])
+        _lib.check(_lib.lib().ixh_epilogue(at[0], lds[0], m, out_f, C.byref(ep), held.data_ptr(), ld, _lib.current_stream(dev)))
+        _close(held[:m, :out_f].contiguous(), want, bound)
+        assert bool((held[m] == 7).all()) and bool((held[:, out_f:] == 7).all())
