@@ -37,15 +37,16 @@ MFMA_BF16_PEAK = 2.5e15  # FLOP/s dense bf16, MI355X published
 # workloads without a counter run, or measured on other sources, report null.
 # (bytes per launch, the sources the kernel is compiled from, their kernel_sources_sha16 at the counter run); names that end
 # in _packed are --packed runs, of the kernels that read the packed streams
+# (every header of ours that those include, down to the last: the kernels are compiled from these as well)
 _LANES = ("ixh_lanes.hip", "ixh_lanes_rows.hip", "ixh_lanes_gemm.hip", "ixh_lanes_prompt.hip", "ixh_lanes.h",
-          "ixh_lanes_dev.h", "ixh_lanes_bounds.h", "ixh_fast358.h", "ixh_dev.h",
+          "ixh_lanes_dev.h", "ixh_lanes_bounds.h", "ixh_epilogue.h", "ixh_fast358.h", "ixh_dev.h",
           "build.sh")
-_ROWS = ("ixh_rows358.hip", "ixh_rows_common.h", "ixh_dev.h", "build.sh")
-_TILES = ("ixh_tiles358.hip", "ixh_rows_common.h", "ixh_dev.h")
-_DENSE = ("ixh_dense358.hip", "ixh_dense_tiles.h", "ixh_dev.h")
-_DENSE5 = ("ixh_dense5.hip", "ixh_dense_tiles.h", "ixh_dev.h")
-_PREFILL = ("ixh_prefill358.hip", "ixh_prefill358.h", "ixh_rows_common.h", "ixh_dev.h")
-_DECODE_ROWS = ("ixh_decode_rows358.hip", "ixh_rows_common.h", "ixh_dev.h")
+_ROWS = ("ixh_rows358.hip", "ixh_rows_common.h", "ixh_fast358.h", "ixh_dev.h", "build.sh")
+_TILES = ("ixh_tiles358.hip", "ixh_rows_common.h", "ixh_fast358.h", "ixh_dev.h")
+_DENSE = ("ixh_dense358.hip", "ixh_dense_tiles.h", "ixh_fast358.h", "ixh_dev.h")
+_DENSE5 = ("ixh_dense5.hip", "ixh_dense_tiles.h", "ixh_fast358.h", "ixh_dev.h")
+_PREFILL = ("ixh_prefill358.hip", "ixh_prefill358.h", "ixh_rows_common.h", "ixh_fast358.h", "ixh_dev.h")
+_DECODE_ROWS = ("ixh_decode_rows358.hip", "ixh_rows_common.h", "ixh_fast358.h", "ixh_dev.h")
 _ENCODE = ("ixh_encode.hip", "ixh_dev.h")
 _OLD = ((), "measured-on-earlier-sources")  # figures kept for the record; reported as null
 MEASURED_TRAFFIC_BYTES = {

@@ -271,3 +271,18 @@ def test_several_rows_of_many_row_quads_are_not_the_gemv_kernels():
 
     assert need(65536, 5120, 5, 3) > 0 and need(65536, 5120, 5, 4) > 0
     assert need(65536, 5120, 5, 1) == 0 and need(17408, 5120, 5, 4) == 0
+
+
+def test_bench_counters_name_every_source():
+    """The sources that a kept counter figure belongs to are closed under their own #includes: a change in any of them takes the figure back.
+    (include/ixhip.h declares the boundary, which is another matter.)"""
+    import re
+
+    bench, csrc = load_bench(), os.path.join(ROOT, "ixrun_amd", "csrc")
+    groups = {files for table in (bench.MEASURED_TRAFFIC_BYTES, bench.MEASURED_INSTRUCTIONS) for _, files, _ in table.values()}
+    assert len(groups) > 4
+    for files in groups:
+        for name in files:
+            with open(os.path.join(csrc, name)) as f:
+                included = set(re.findall(r'^#include "(ixh_[^"/]+)"', f.read(), re.M))
+            assert included <= set(files), (name, included - set(files))
