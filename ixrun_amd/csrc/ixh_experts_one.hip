@@ -220,12 +220,16 @@ static uint32_t eo_blocks(const ExMatrix &W, uint32_t per, uint32_t slots) {
     return std::max(std::min(std::min(16u / eo_waves(W, per), all * slots / ln_cus()), all) / per * per, per);
 }
 
+template <int BITS, bool JOIN> static size_t eo_lds(uint32_t C, uint32_t items, uint32_t CW) {
+    return (JOIN ? items : 1u) * (LnPairs<BITS, false>::kLutBytes + C * 1024u + 64u) + items * CW * 64u + (JOIN ? items * 72u : 0u);
+}
+
 template <int BITS, bool FIRST, bool JOIN, int CELLS> static int eo_launch(const ExMatrix &W, const ExOne &R, hipStream_t s) {
     const uint32_t per = FIRST && R.gated ? 2u : 1u, C = W.n_cells, CW = CELLS == 2 ? (C + 1u) / 2u : C, all = (W.n_tiles + 3u) / 4u;
-    const uint32_t blocks = JOIN ? 1u : eo_blocks(W, per, R.tokens * R.top_k), items = JOIN ? R.top_k : blocks, tables = JOIN ? items : 1u;
+    const uint32_t blocks = JOIN ? 1u : eo_blocks(W, per, R.tokens * R.top_k), items = JOIN ? R.top_k : blocks;
     if (C > 16u || items * CW > 16u || (CELLS == 2 && (JOIN || items < 2u))) return IXH_EUNSUPPORTED;
     const bool whole = ((uintptr_t)R.x & 15u) == 0 && W.in_f % 8u == 0 && (R.ldx % 8 == 0 || R.rows == 1u);
-    const size_t lds = tables * (LnPairs<BITS, false>::kLutBytes + C * 1024u + 64u) + items * CW * 64u + (JOIN ? items * 72u : 0u);
+    const size_t lds = eo_lds<BITS, JOIN>(C, items, CW);
     if constexpr (JOIN) {
         static const bool raised = hipFuncSetAttribute(reinterpret_cast<const void *>(k_experts_one<BITS, FIRST, JOIN, CELLS>),
                                                        hipFuncAttributeMaxDynamicSharedMemorySize, (int)kLnLds) == hipSuccess;
@@ -251,11 +255,27 @@ int launch_experts_one(const ExMatrix &W, const ExOne &R, bool first, hipStream_
     return eo_cells(W, R.gated ? 2u : 1u) == 2u ? eo_matrix<true, false, 2>(W, R, s) : eo_matrix<true, false, 1>(W, R, s);
 }
 
-// Up to twelve waves a workgroup and six tokens: us of a call apart / joined, 1 / 2 / 4 / 8 tokens by 6 of 64 experts of 2048 x 1024 (12 waves) 16.4 / 26.4 /
-// 34.6 / 50.6 and 16.0 / 22.8 / 32.5 / 51.8; by 2 of 16 of 4096 x 1536 (6) 14.0 / 19.4 / 29.5 / 45.8 and 12.3 / 18.4 / 27.0 / 44.0; by 8 of 128 of
-// 2048 x 512 (8) 13.8 / 19.4 / 28.2 / 42.7 and 14.2 / 19.0 / 27.9 / 44.9; of 2048 x 768 (16) 15.8 / 25.4 / 35.1 / 54 and 17.2 / 24.9 / 39.2 / 67.
+static size_t eo_joined_lds(const ExMatrix &W, uint32_t top_k) {
+    switch (W.bits) {
+        case 3: return eo_lds<3, true>(W.n_cells, top_k, W.n_cells);
+        case 4: return eo_lds<4, true>(W.n_cells, top_k, W.n_cells);
+        case 5: return eo_lds<5, true>(W.n_cells, top_k, W.n_cells);
+        default: return eo_lds<8, true>(W.n_cells, top_k, W.n_cells);
+    }
+}
+// Fewer than one and a half times as many workgroups (one to a block of rows and token, each with the tables and waves of all of the token's slots) as
+// the CUs hold at once.  us of a call apart / joined, ids and weights others from call to call, 1 / 2 / 3 / 4 / 6 / 8 tokens by 6 of 64 experts of 2048 x
+// 1024 at 5 bits (two workgroups a CU: up to five tokens) 18.3 / 24.8 / 31.2 / 32.9 / 42.9 / 48.0 and 16.5 / 21.0 / 28.1 / 30.1 / 41.0 / 48.1; by 8 (one:
+// two tokens) 18.0 / 25.3 / 33.2 / 37.2 / 48.4 / 65.0 and 18.1 / 23.8 / 36.0 / 40.1 / 55.9 / -; by 8 of 128 of 2048 x 512 (two) 14.6 / 18.4 / 25.4 / 25.7 /
+// 33.3 / 37.8 and 13.6 / 16.8 / 22.8 / 24.4 / 33.3 / 39.3; by 2 of 16 of 4096 x 1536 (five: seven tokens) 16.8 / 22.9 / 30.4 / 32.1 / 42.0 / 49.3 and 14.1 /
+// 20.1 / 25.7 / 28.1 / 38.7 / 45.7; by 12 of 128 of 2048 x 512 at 3 bits (one) 15.5 / 19.3 / 23.7 / 24.9 / 32.2 / 35.9 and 13.9 / 16.8 / 25.7 / 27.4 / 38.0 /
+// 46.9.  Over 924 calls (13 layers, planes of 3 to 8 bits, 1 to 16 slots and 1 to 12 tokens) this takes 0.5 % longer than the better one each time, never
+// joined 13.7 %, always 1.5 %.
 bool experts_joined_takes(const ExMatrix &W, uint32_t tokens, uint32_t top_k) {
-    return tokens <= 6u && W.n_cells <= 12u && top_k <= 12u && top_k * W.n_cells <= 12u;
+    const uint64_t waves = (uint64_t)top_k * W.n_cells;
+    if (waves > 16u) return false;
+    const uint64_t a_cu = std::min<uint64_t>(kLnLds / eo_joined_lds(W, top_k), 32u / waves), all = (W.n_tiles + 3u) / 4u;
+    return 2u * all * tokens < 3u * a_cu * ln_cus();
 }
 int launch_experts_joined(const ExMatrix &W, const ExOne &R, hipStream_t s) { return eo_matrix<false, true, 1>(W, R, s); }
 

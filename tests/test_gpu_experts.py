@@ -567,3 +567,22 @@ def test_experts_of_rows_whose_positions_start_over(dev, recipe, level_bits, hid
             x[tokens // 2, 0] = math.inf
             same = torch.arange(tokens) != tokens // 2
             assert torch.equal(layer(x, ids, weights, residual)[same], y[same])
+
+
+@pytest.mark.parametrize("recipe,level_bits", [("t", (3, 5, 8)), ("real", (3, 5, 8)), ("outlier", (4, 8)), ("real", (6, 8))])
+@pytest.mark.parametrize("hidden,inner,top_k", [(264, 100, 16), (100, 40, 13), (72, 8000, 1), (520, 2000, 4), (1037, 700, 7), (40, 3000, 2)])
+def test_experts_whose_sum_is_in_the_second_launch(dev, recipe, level_bits, hidden, inner, top_k):
+    """Up to sixteen cells of a token's slots in one workgroup, and calls of more tokens than that is done for: the same sums."""
+    layer, dense = _repeated_layer(dev, 16, hidden, inner, recipe, level_bits)
+    for tokens in (1, 2, 5, 40):
+        x, ids, weights, residual = _call(dev, tokens, top_k, 16, hidden, seed=tokens, residual=True)
+        if tokens > 1:
+            ids[0] = 4
+            ids[1, 0] = -7
+        clean = torch.where(ids >= 0, weights, 0)
+        y = layer(x, ids, torch.where(ids >= 0, weights, math.nan), residual)
+        _close(y, *ref.experts(x, ids, clean, **dense, residual=residual))
+        _close(layer(x, ids, weights), *ref.experts(x, ids, clean, **dense))
+        for t in range(min(tokens, 3)):
+            _close(layer(x[t:t + 1], ids[t:t + 1], weights[t:t + 1], residual[t:t + 1]), *ref.experts(x[t:t + 1], ids[t:t + 1], clean[t:t + 1], **dense,
+                                                                                                 residual=residual[t:t + 1]))
