@@ -3,7 +3,9 @@
 
 namespace ixh {
 
-// Bound: memory.  A row after another, so that a workgroup's accesses are consecutive in each operand.
+// Bound: its requests, of two bytes a lane, and one row after another a workgroup, so that its accesses are consecutive in each operand.  silu, multiplier
+// and residual at 512 x 5120 6.5 us (3.2 TB/s, from caches), 4096 x 4096 47 us (2.9), 4096 x 17408 290 us (2.0, where a copy reaches 4.9); next to a product that
+// a layer without an epilogue of its own takes 100 us and more for.
 __global__ void __launch_bounds__(256)
 k_epilogue(const uint16_t *v, int64_t ldv, uint32_t m, uint32_t out_f, uint16_t *y, int64_t ldy, Epilogue ep) {
     const uint32_t at = blockIdx.y * 256u + threadIdx.x;

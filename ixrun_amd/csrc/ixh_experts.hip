@@ -152,8 +152,8 @@ k_experts_plan(const int32_t *__restrict__ ids, uint32_t slots, uint32_t experts
 // The intermediate is rounded to bf16, which the matrix unit's operands have to be: half a step, 2^-9 to 2^-8 of each element, which a row of the second
 // matrix averages (relative error of a call 0.0017 from the output's own rounding, 0.0023 with it).
 //
-// Bound: memory, then vector instructions.  64 tokens by 6 of 64 experts of 2048 x 1024, 5 bits: 54 us for the first matrix, which reads 223 MB
-// (4.1 TB/s; 168 MB of codes, some experts' twice), the vector unit busy for 65 % of it, LDS for 55 %; 35 us for the second, 114 MB.
+// Bound: memory, then vector instructions.  64 tokens by 6 of 64 experts of 2048 x 1024, 5 bits: 54 us for the first matrix, which reads 204 MB
+// (3.8 TB/s; 168 MB of codes, some experts' twice), the vector unit busy for 69 % of it, LDS for 59 %; 35 us for the second, 87 MB, 65 % and 49 %.
 // ---------------------------------------------------------------------------------------------------------------
 // (Tiles of 16, which halve the decoding of an expert with more than eight, take longer: their listed elements cost twice as much, and 24 registers
 // go to memory.  us of a call, 8 / 16, 64 experts of 2048 x 1024 with 2, 8 and 16 tokens each: 68 / 91, 101 / 124, 149 / 156.)
@@ -568,9 +568,11 @@ static bool ex_many(const ExDev &X, uint32_t slots) {
     return slots >= kExMany * X.experts && std::max(X.first.n_cells, X.second.n_cells) <= 2048u;
 }
 
-// Layers of a tile of k_experts_prompt, two instead of four where the workgroups then still are all there at once, three a CU (us with four / two: 2279
-// tokens by 3 of 7 experts of 512 x 192, which are 480 of 768 workgroups at most, 50 / 45; 1000 by 2 of 8 of 2048 x 512, 750, 64 / 57; 400 by 2 of 8 of
-// 4096 x 1536, 910, 100 / 110; 512 by 2 of 16 of these, 1500, 119 / 156; 1333 by 3 of 20 of 1400 x 744, 1200, 87 / 104).
+// Layers of a tile of k_experts_prompt, two instead of four where the workgroups then still are all there at once, three a CU.  us with four / two at 5
+// bits: 2279 tokens by 3 of 7 experts of 512 x 192, which are 480 of 768 workgroups at most, 49 / 44; 500 and 1000 by 2 of 8 of 2048 x 512, 480 and 736,
+// 53 / 50 and 65 / 58; beyond, 4000 by 3 of 7 of 512 x 192, 800, 58.7 / 59.5; 600, 800 and 1500 by 2 of 8 of 4096 x 1536, 1088, 1280 and 1984, 99 / 109,
+// 115 / 124 and 170 / 198; 1600 by 2 of 8 of 2048 x 512, 1056, 70 / 72; 1333 by 3 of 20 of 1400 x 744, 1224, 83 / 87 (800, 912, 64.9 / 63.7); 512 and 1600 by
+// 2 of 16 of 4096 x 1536, 1536 and 2624, 106 / 106 and 199 / 232; with 3 bits and with 10 % listed the same sides.
 static uint32_t ex_layers(const ExDev &X, uint32_t slots) {
     const uint64_t w_tiles = (std::max(X.first.n_tiles, X.second.n_tiles) + 15u) / 16u;
     return (slots / (2u * kExLayer) + X.experts) * w_tiles <= 3ull * ln_cus() ? 2u : 4u;

@@ -12,11 +12,11 @@ namespace ixh {
 //
 // Bound: a launch, one chain of requests (the expert's id, then its codes, the extents of their lists, scale and activations at once, then the
 // lists) and the instructions of a cell.  Products and listed elements as in k_experts_rows, of whose kernel for one row some 350 of 1100
-// instructions a wave only find its share: one token by 6 experts of 2048 x 1024, 25 MB of codes and lists, first / second matrix 13.2 / 9.6 us
-// there, 9.1 / 6.9 us here (1.6 TB/s with their starts and ends).
+// instructions a wave only find its share: one token by 6 experts of 2048 x 1024 at 5 bits, first / second matrix 13.2 / 9.6 us there, 9.2 / 6.4 us here
+// (20.6 and 10.7 MB read; vector unit busy for 43 and 50 % of the CUs' time, LDS for 34 and 37 %, the second one joined as below).
 //
 // JOIN, the second matrix for a few tokens: a workgroup has a block of rows of all of a token's slots, with a pair table and activations for
-// each, and ends with the sum over them, in their order, so that no launch follows: 20.0 -> 17.8 us for that token (second matrix and sum 6.9 + 2.7 -> 8.5).
+// each, and ends with the sum over them, in their order, so that no launch follows: second matrix and sum 6.4 + 2.8 -> 7.8 us for that token.
 // ---------------------------------------------------------------------------------------------------------------
 struct EoJoin {  // what a token's outputs are made with
     const float *weights;

@@ -21,7 +21,7 @@ __all__ = ["StreamingExperts", "route_experts"]
 LOGIT_TYPES = {torch.float32: _lib.IXH_F32, torch.float16: _lib.IXH_F16, torch.bfloat16: _lib.IXH_BF16}
 SCORINGS = {"softmax": _lib.IXH_SCORE_SOFTMAX, "sigmoid": _lib.IXH_SCORE_SIGMOID}
 MOST_EXPERTS = 1024
-MOST_PLACES = 1 << 17  # tokens times experts of each in one call of the library: bounds the call's scratch
+MOST_PLACES = 1 << 17  # tokens times experts of each in one call of the library: bounds the call's scratch (4 bytes a column of each: 3.8 GB at 7168)
 
 
 def route_experts(logits, top_k: int, *, scoring: str = "softmax", bias=None, n_groups: int = 1, top_groups: int | None = None,
