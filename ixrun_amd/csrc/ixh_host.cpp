@@ -506,11 +506,12 @@ PyObject *encode(PyObject *, PyObject *const *args, Py_ssize_t n_args) {
     END_HANDLE_TH_ERRORS
 }
 
-// A contiguous tensor of this type on the current device that asks for no gradient, outside of forward mode (whose tangents Python looks for);
-// null for anything else.
+// Whether tensors may have tangents, which Python looks for.
+bool forward_mode() { return torch::autograd::ForwardADLevel::try_get_by_idx(0) != nullptr; }
+// A contiguous tensor of this type on the current device that asks for no gradient; null for anything else.
 const at::Tensor *given(PyObject *o, at::ScalarType type, int64_t device) {
     const at::Tensor *t = plain(o, type, device);
-    return t && !(t->requires_grad() && c10::GradMode::is_enabled()) && !torch::autograd::ForwardADLevel::try_get_by_idx(0) ? t : nullptr;
+    return t && !(t->requires_grad() && c10::GradMode::is_enabled()) ? t : nullptr;
 }
 bool alike(const at::Tensor &a, const at::Tensor &b, int64_t last) {  // the same leading dimensions, and `last`
     return a.dim() == b.dim() && a.size(-1) == last && a.sizes().slice(0, a.dim() - 1) == b.sizes().slice(0, b.dim() - 1);
@@ -524,7 +525,7 @@ PyObject *route(PyObject *, PyObject *const *args, Py_ssize_t n_args) {
         PyErr_SetString(PyExc_TypeError, "route: eight arguments, after bind");
         return nullptr;
     }
-    if (!THPVariable_CheckExact(args[0]) || !watching().empty()) Py_RETURN_NONE;
+    if (!THPVariable_CheckExact(args[0]) || !watching().empty() || forward_mode()) Py_RETURN_NONE;
     const at::Tensor &l = THPVariable_Unpack(args[0]);
     if (!l.is_cuda()) Py_RETURN_NONE;
     const at::ScalarType type = l.scalar_type();
@@ -581,7 +582,7 @@ PyObject *product(PyObject *, PyObject *const *args, Py_ssize_t n_args) {
     const uint16_t *bias = reinterpret_cast<const uint16_t *>(PyLong_AsUnsignedLongLong(args[1]));
     const long long device = PyLong_AsLongLong(args[2]), activation = PyLong_AsLongLong(args[4]);
     if (PyErr_Occurred()) return nullptr;
-    if (!THPVariable_CheckExact(args[3]) || !watching().empty() || !THPVariable_Unpack(args[3]).is_cuda() || c10::hip::current_device() != device)
+    if (!THPVariable_CheckExact(args[3]) || !watching().empty() || forward_mode() || !THPVariable_Unpack(args[3]).is_cuda() || c10::hip::current_device() != device)
         Py_RETURN_NONE;
     const at::Tensor *x = given(args[3], at::kBFloat16, device);
     if (!x || x->dim() < 1 || x->size(-1) != lanes->in_f) Py_RETURN_NONE;
@@ -623,7 +624,7 @@ PyObject *experts(PyObject *, PyObject *const *args, Py_ssize_t n_args) {
     const IxhExperts *of = reinterpret_cast<const IxhExperts *>(PyLong_AsUnsignedLongLong(args[0]));
     const long long device = PyLong_AsLongLong(args[1]), most = PyLong_AsLongLong(args[2]);
     if (PyErr_Occurred()) return nullptr;
-    if (!THPVariable_CheckExact(args[3]) || !watching().empty() || !THPVariable_Unpack(args[3]).is_cuda() || c10::hip::current_device() != device)
+    if (!THPVariable_CheckExact(args[3]) || !watching().empty() || forward_mode() || !THPVariable_Unpack(args[3]).is_cuda() || c10::hip::current_device() != device)
         Py_RETURN_NONE;
     const at::Tensor *x = given(args[3], at::kBFloat16, device), *ids = given(args[4], at::kInt, device), *weights = given(args[5], at::kFloat, device);
     if (!x || !ids || !weights || x->dim() < 1 || x->size(-1) != of->hidden || x->numel() == 0 || ids->sizes() != weights->sizes()) Py_RETURN_NONE;
